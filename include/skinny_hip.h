@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define SKINNY_ABI_VERSION 21
+#define SKINNY_ABI_VERSION 22
 
 /* Error codes. */
 #define SKINNY_OK 0
@@ -539,6 +539,63 @@ int skinny_sample_rows_bf16(const uint16_t* logits, int rows, int V, int ld, flo
 int skinny_spec_accept_sampled(const uint16_t* target, int ldt, const float* stats_t, const uint16_t* draft, int ldd,
                                const float* stats_d, int Vd, const int32_t* drafts, int K, int V, float inv_temp,
                                uint64_t seed, const int64_t* counter, int32_t* out, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Several sequences over a key-value cache in pages (no reference counterpart: the reference
+ * decodes one sequence, spec.py:98-156; the layer's arithmetic is that of spec.py:24-29).
+ *
+ * K pages [n_pages][n_kv][page][head_dim] and V^T pages [n_pages][n_kv][head_dim][page], bf16, each
+ * page contiguous and k_stride / vt_stride elements after the one before it (multiples of 8);
+ * head_dim 64, 128 or 256; page a power of two from 16 to 256. Sequence b holds lengths[b] tokens
+ * before the call and brings counts[b] of the call's T new ones (counts NULL: T each), at positions
+ * lengths[b] + t; position p is slot p % page of page pages[b * ld_pages + p / page]. Nothing on the
+ * device is advanced: the caller adds the counts to the lengths after the step. Entries of `pages`
+ * that no token needs may hold anything. Rows t >= counts[b] are padding.
+ * A sequence that cannot be (a negative length, a count outside [0, T], more tokens than the call's
+ * bound) or a needed page outside [0, n_pages) is not read or written: its query rows and the
+ * attention rows that would see it are NaN. */
+typedef struct {
+  const int32_t* lengths;  /* [B] */
+  const int32_t* counts;   /* [B] or NULL */
+  const int32_t* pages;    /* [B][>= max_pages] */
+  int ld_pages, max_pages;
+  uint16_t* k_pages;
+  uint16_t* vt_pages;
+  int64_t k_stride, vt_stride;
+  int n_pages, page, n_kv, head_dim;
+} skinny_paged_kv;
+/* Raw q|k|v rows [B*T] (stride ldq; heads laid out as for skinny_attention_general_bf16: query head
+ * h at h*q_stride, key / value head j at k_offset / v_offset + j*D): per-head q/k RMSNorm (NULL
+ * weights: none), rotate-half RoPE over the first rotary_dim dims from a skinny_rope_table_dim table
+ * of at least max_pages*page positions; keys and values into their slots, queries to q_out
+ * [B*T][Hq][D] (padding rows zero). fp32 inside, rounded once. B and T at most 65535. A page that the
+ * call writes must belong to one sequence. */
+int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int T, int Hq, int q_stride, int k_offset, int v_offset,
+                            const uint16_t* q_norm, const uint16_t* k_norm, float eps, int rotary_dim,
+                            const float* rope_table, int rope_positions, const skinny_paged_kv* kv, uint16_t* q_out,
+                            void* stream);
+/* Attention of q [B*T][Hq][D] over the cached and the new tokens (which must be in the pages):
+ * token t of sequence b sees positions <= lengths[b] + t. T * Hq / n_kv <= 64. `keys` is the host's
+ * bound on lengths[b] + counts[b] (at most max_pages*page); a sequence past it is NaN. With `gate`
+ * (row stride ld_gate, head stride gate_stride) the output is multiplied by sigmoid(gate). out
+ * [B*T][Hq*D], padding rows zero. A row's bits depend only on its own sequence and position: not on
+ * B, T, the page size or the pages' places. The workspace (16-byte aligned, of
+ * skinny_paged_attn_workspace_bytes; 0 bytes: NULL will do) carries nothing from call to call; calls
+ * that may overlap need their own. */
+size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int keys);
+int skinny_paged_attention_bf16(const uint16_t* q, int B, int T, int Hq, const skinny_paged_kv* kv, int keys, float scale,
+                                const uint16_t* gate, int64_t ld_gate, int gate_stride, void* workspace,
+                                size_t workspace_bytes, uint16_t* out, void* stream);
+/* For each bf16 row of scores (V <= 524288, row stride ld), with the distribution softmax(row / T):
+ * logprob = ln p(tokens[row]) (-inf for a token outside [0, V)), entropy = -sum p ln p (nats), and
+ * the `top` <= 32 most probable tokens (decreasing, ties by index, NaN scores last) with their
+ * log-probabilities, ids and top_logprob [rows][top]. Scores of -inf have probability 0; a row with a
+ * NaN, a +inf or nothing but -inf has NaN for its numbers. fp32 sums. No reference counterpart (the
+ * reference reports tokens only). The workspace (skinny_token_logprobs_workspace_bytes) as above. */
+size_t skinny_token_logprobs_workspace_bytes(int rows, int V, int top);
+int skinny_token_logprobs_bf16(const uint16_t* logits, int rows, int V, int64_t ld, const int32_t* tokens, float inv_temp,
+                               int top, void* workspace, size_t workspace_bytes, float* logprob, float* entropy,
+                               int32_t* ids, float* top_logprob, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Streaming-read ceiling (harness). Reads `bytes` (multiple of 16, 16-byte aligned)

@@ -22,7 +22,7 @@ LIB_NAME = "libskinny_hip.so"
 # SKINNY_HIP_LIB names another build of the same library (the host-only sanitizer build the CPU
 # tests load); unset, the in-tree build next to this file.
 LIB_PATH = os.environ.get("SKINNY_HIP_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
@@ -52,6 +52,18 @@ class NormIn(ctypes.Structure):
 
 
 _normin_p = ctypes.POINTER(NormIn)
+
+
+class PagedKV(ctypes.Structure):
+    """skinny_paged_kv of include/skinny_hip.h."""
+
+    _fields_ = [("lengths", ctypes.c_void_p), ("counts", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("ld_pages", ctypes.c_int), ("max_pages", ctypes.c_int), ("k_pages", ctypes.c_void_p),
+                ("vt_pages", ctypes.c_void_p), ("k_stride", ctypes.c_int64), ("vt_stride", ctypes.c_int64),
+                ("n_pages", ctypes.c_int), ("page", ctypes.c_int), ("n_kv", ctypes.c_int), ("head_dim", ctypes.c_int)]
+
+
+_paged_p = ctypes.POINTER(PagedKV)
 
 # name -> (restype, argtypes). Every symbol declared in include/skinny_hip.h is listed.
 SIGNATURES: dict[str, tuple] = {
@@ -176,6 +188,14 @@ SIGNATURES: dict[str, tuple] = {
     "skinny_spec_accept_sampled": (_c_int, [_c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int,
                                             _c_void_p, _c_int, _c_int, _c_float, _c_u64, _c_void_p, _c_void_p,
                                             _c_void_p]),
+    "skinny_paged_store_bf16": (_c_int, [_c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p,
+                                         _c_void_p, _c_float, _c_int, _c_void_p, _c_int, _paged_p, _c_void_p, _c_void_p]),
+    "skinny_paged_attn_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "skinny_paged_attention_bf16": (_c_int, [_c_void_p, _c_int, _c_int, _c_int, _paged_p, _c_int, _c_float, _c_void_p,
+                                             _c_i64, _c_int, _c_void_p, _c_size_t, _c_void_p, _c_void_p]),
+    "skinny_token_logprobs_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
+    "skinny_token_logprobs_bf16": (_c_int, [_c_void_p, _c_int, _c_int, _c_i64, _c_void_p, _c_float, _c_int, _c_void_p,
+                                            _c_size_t, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lib = None
