@@ -10,18 +10,20 @@
 // dim are one 16-byte piece, as the matrix cores take them. Sequence b holds lengths[b] tokens before the
 // call and brings counts[b] of at most T new ones, at positions lengths[b] + t; position p lives in slot
 // p % P of page pages[b][p / P].
+#include <type_traits>
 #include "common.h"
 
 namespace {
 
 constexpr float kPLog2e = 1.4426950408889634f;
-constexpr int kPWaves = 4;      // waves of an attention workgroup: one run of atom keys each
-constexpr int kPMaxRows = 64;   // query rows per kv head: T x (Hq / Hkv)
-constexpr int kPMergeWaves = 4;
+constexpr int kPMaxRows = 64;  // query rows per kv head: T x (Hq / Hkv)
+constexpr int kPBlock = 128;   // keys of a block
+constexpr int kPPair = 2;      // blocks joined left to right: what a workgroup takes at least
+constexpr int kPGroup = 8;     // blocks whose pairs are joined left to right, by the workgroup that takes them all or by the merge
 
-// Keys that one wave takes at once: 32 KB of K and V at 128 and 256 dims, held in registers.
-__host__ __device__ constexpr int paged_atom(int D) { return D == 256 ? 32 : 64; }
-__host__ __device__ constexpr int paged_block(int D) { return paged_atom(D) * kPWaves; }
+// Memory that this kernel only reads, for uniform addresses: loaded into scalar registers.
+typedef const __attribute__((address_space(4))) int32_t* words_t;
+__device__ __forceinline__ words_t words(const int32_t* p) { return (words_t)(uintptr_t)p; }
 
 struct Pages {
   const int32_t* lengths;
@@ -29,8 +31,8 @@ struct Pages {
   const int32_t* table;   // [B][>= max_pages], row stride ld
   uint16_t* k;
   uint16_t* vt;
-  int64_t k_stride, vt_stride;  // elements from page to page
-  int ld, n_pages, log2p;
+  uint32_t k_stride, vt_stride;  // elements from page to page
+  int ld, max_pages, n_pages, log2p;
 };
 
 // A sequence's cached length and new tokens. `ok` is false where they cannot be: a negative length, a count
@@ -40,7 +42,7 @@ struct Sequence {
   bool ok;
 };
 __device__ __forceinline__ Sequence sequence_of(const Pages& pg, int b, int T, int room) {
-  const int len = pg.lengths[b], count = pg.counts ? pg.counts[b] : T;
+  const int len = words(pg.lengths)[b], count = pg.counts ? words(pg.counts)[b] : T;
   return {len, count, len >= 0 && count >= 0 && count <= T && count <= room && len <= room - count};
 }
 
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(64) void paged_store_kernel(Pages pg, const uint16_
   else src += voff + (head - Hq - Hkv) * D;
   const int slot = pos & (P - 1);
   if (head >= Hq + Hkv) {
-    uint16_t* vd = pg.vt + (int64_t)page * pg.vt_stride + (size_t)(head - Hq - Hkv) * D * P + slot;
+    uint16_t* vd = pg.vt + (int64_t)page * (int64_t)pg.vt_stride + (size_t)(head - Hq - Hkv) * D * P + slot;
 #pragma unroll
     for (int e = 0; e < E; ++e) vd[(size_t)(lane + 64 * e) * P] = src[lane + 64 * e];
     return;
@@ -105,7 +107,7 @@ __global__ __launch_bounds__(64) void paged_store_kernel(Pages pg, const uint16_
   for (int e = 0; e < E; ++e) row[lane + 64 * e] = x[e];
   __syncthreads();
   const int half = R >> 1;
-  uint16_t* dst = head < Hq ? qd : pg.k + (int64_t)page * pg.k_stride + ((size_t)(head - Hq) * P + slot) * D;
+  uint16_t* dst = head < Hq ? qd : pg.k + (int64_t)page * (int64_t)pg.k_stride + ((size_t)(head - Hq) * P + slot) * D;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + 64 * e;
@@ -121,17 +123,25 @@ __global__ __launch_bounds__(64) void paged_store_kernel(Pages pg, const uint16_
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Attention. A block of paged_block(D) keys of one sequence and kv head is one workgroup's: each wave takes an
-// atom of paged_atom(D) keys straight from memory into matrix-core operands, S^T = K Q^T, an exact softmax of the
-// atom, O^T = V^T P^T, and the four atoms are folded in order. Blocks are joined in order by the merge. Atoms and
-// blocks are cut at fixed positions of the sequence, and a row that does not see an atom adds nothing to it, so a
-// row's bits depend on its own sequence and position alone: not on the batch, on T, or on where the pages lie.
+// Attention. A workgroup takes a run of blocks of 128 keys of one sequence and kv head, with a wave for every 32 dims.
+// In a block each wave scores its share of the keys (S^T = K Q^T, the K rows straight from memory into matrix-core
+// operands); the row maxima and then the weights P go through LDS, and each wave forms its 32 dims over all the block's
+// keys (O^T = V^T P^T). So K and V are read once, by one wave each, and no output is summed across waves. As soon as a
+// block's scores (outputs) are formed, its K (V) registers take the next block's loads, which are in flight through the
+// rest of the block.
+//
+// What bounds it is memory, if the instructions of a block (64 KB of K and V for 128 dims) stay few: everything that
+// only a block at the sequence's end, or one with a missing page, needs stands behind one branch, and addresses are
+// formed in scalars once per page.
+//
+// Blocks are joined left to right in pairs, pairs in groups of kPGroup blocks, the groups by the merge. All are cut at
+// fixed positions of the sequence, and keys that a row does not see add exact zeros, so a row's bits depend on its own
+// sequence and position alone: not on the batch, on T, on who joins the pairs, or on where the pages lie.
 
 // The first n (0 to 8) of eight consecutive keys' values, the others zero.
 __device__ __forceinline__ u32x4_t first_keys(u32x4_t v, int n) {
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
-    v[w] &= (2 * w < n ? 0xffffu : 0u) | (2 * w + 1 < n ? 0xffff0000u : 0u);
+  for (int w = 0; w < 4; ++w) v[w] &= n >= 2 * w + 2 ? ~0u : n == 2 * w + 1 ? 0xffffu : 0u;
   return v;
 }
 
@@ -142,281 +152,521 @@ struct Out {
   int gs;                // and from head to head
 };
 
-// One output value o / l, gated, rounded.
-__device__ __forceinline__ uint16_t finished(float o, float l, const uint16_t* gate, int d) {
-  o /= l;
-  if (gate) o /= 1.f + __builtin_amdgcn_exp2f(bf16_bits_to_f32(gate[d]) * -kPLog2e);
+// One output value, divided by the sum of its weights, gated, rounded.
+__device__ __forceinline__ uint16_t finished(float o, float inv, const uint16_t* gate, int d) {
+  o *= inv;
+  if (gate) o *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(bf16_bits_to_f32(gate[d]) * -kPLog2e));
   return f32_to_bf16_bits(o);
 }
 
-template <int D>
-__global__ __launch_bounds__(64 * kPWaves, 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T,
-                                                                      int Hq, int Hkv, int room, float scale, int nblk,
-                                                                      float* __restrict__ part_o,
-                                                                      float* __restrict__ part_ml, Out o) {
-  constexpr int ATOM = paged_atom(D), BLK = paged_block(D);
-  constexpr int KS = D / 32, DT = D / 16, KT = ATOM / 16, PS = ATOM / 32, GR = ATOM / 16;
-  constexpr int OP = D + 4;  // LDS pitch of an output row
-  __shared__ __attribute__((aligned(16))) float o_lds[kPWaves][16 * OP];
-  __shared__ float ml_lds[kPWaves][16][2];
-  const int c = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+// Part (m, l, o) of a row joined to the parts before it: their factor and its own.
+struct Join {
+  float before, part;
+};
+__device__ __forceinline__ Join join(float& m, float& l, float pm, float pl) {
+  const float mm = fmaxf(m, pm), ref = mm == -INFINITY ? 0.f : mm;
+  const Join j{__builtin_amdgcn_exp2f(m - ref), __builtin_amdgcn_exp2f(pm - ref)};
+  m = mm;
+  l = fmaf(pl, j.part, l * j.before);
+  return j;
+}
+
+// The larger of, and the sum over, the four quads' values of a column, in every lane.
+__device__ __forceinline__ float quads_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float quads_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+}
+
+// W tiles of 16 query rows; a call of more rows per kv head than 32 (`halves` 1) takes two workgroups a run, the second
+// of which finds K and V in the caches. GS: keys of a block that share a page: the page size where that is 16 or 32, else 64.
+template <int D, int W, int GS>
+__global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T, int Hq,
+                                                               int Hkv, int room, float scale, int span, int slots, int halves,
+                                                               float* __restrict__ part_o, float* __restrict__ part_ml,
+                                                               Out o) {
+  constexpr int WAVES = D / 32, KT = 8 / WAVES, KS = D / 32;  // a wave's 16-key tiles; dim steps of a score
+  constexpr int ST = kPBlock / 32, NG = kPBlock / GS;         // a block's 32-key steps and pages
+  constexpr int KG = KT * 16 > GS ? KT * 16 / GS : 1;         // pages of a wave's keys
+  constexpr int DW = 2;                                       // a wave's 16-dim tiles
+  constexpr int QP = D + 8;
+  __shared__ u32x4_t p_lds[W][2][ST][64];
+  __shared__ __attribute__((aligned(16))) float m_lds[W * 16][WAVES], l_lds[W * 16][WAVES];
+  __shared__ __attribute__((aligned(16))) uint16_t q_lds[W == 1 ? 8 : W * 16 * QP];
+  const int h = blockIdx.y >> halves, b = blockIdx.z;
+  const int row0 = blockIdx.y & halves ? 16 * W : 0;  // of the rows per kv head
   const int G = Hq / Hkv, lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quad = lane >> 4;
+  const int c0 = blockIdx.x * span;
+  // The queries, the first block's pages and the lengths are asked for at once.
+  constexpr int QN = W == 1 ? KS : (W * 16 * (D / 8) + 2 * D - 1) / (2 * D);
+  auto q_row = [&](int r) { return q + (((size_t)b * T + r / G) * Hq + h * G + r % G) * D; };
+  u32x4_t qr[QN];
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    const int e = threadIdx.x + i * 2 * D;
+    const int r = W == 1 ? col : e / (D / 8), d = W == 1 ? i * 32 + quad * 8 : e % (D / 8) * 8;
+    qr[i] = *reinterpret_cast<const u32x4_t*>(q_row(min(row0 + r, T * G - 1)) + d);
+  }
+  // A block's pages (idk: those of the wave's own keys).
+  const words_t table = words(pg.table + (size_t)b * pg.ld);
+  const int log2p = GS == 16 ? 4 : GS == 32 ? 5 : pg.log2p;
+  const int P = 1 << log2p;
+  const int own = wave * (KT * 16) / GS;
+  int ids[NG], idk[KG];
+  auto find = [&](int c) {
+    if ((c + 1) * kPBlock <= pg.max_pages << log2p) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) ids[g] = GS < 64 ? table[c * NG + g] : table[(c * kPBlock + g * GS) >> log2p];
+#pragma unroll
+      for (int g = 0; g < KG; ++g) idk[g] = GS < 64 ? table[c * NG + own + g] : table[(c * kPBlock + (own + g) * GS) >> log2p];
+    } else {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) ids[g] = table[min((c * kPBlock + g * GS) >> log2p, pg.max_pages - 1)];
+#pragma unroll
+      for (int g = 0; g < KG; ++g) idk[g] = table[min((c * kPBlock + (own + g) * GS) >> log2p, pg.max_pages - 1)];
+    }
+  };
+  find(c0);
   const Sequence sq = sequence_of(pg, b, T, room);
-  if (nblk == 1) {  // no merge follows: the rows that are no tokens are written here
+  if (slots == 1 && row0 == 0) {  // no merge follows: the rows that are no tokens are written here
     const int first = sq.ok ? sq.count : 0;
-    for (int e = threadIdx.x; e < (T - first) * G * D; e += 64 * kPWaves) {
+    for (int e = threadIdx.x; e < (T - first) * G * D; e += 2 * D) {
       const int t = first + e / (G * D);
       o.out[(((size_t)b * T + t) * Hq + h * G) * D + e % (G * D)] = sq.ok ? 0 : kNanBits;
     }
   }
-  const int total = sq.len + sq.count, key0 = c * BLK;
-  if (!sq.ok || sq.count == 0 || key0 >= total) return;
-  const int a0 = key0 + wave * ATOM;
-  const bool active = a0 < total;
-
-  // The pages of the atom's 16-key granules; one past the sequence's end repeats the first, one whose page is none
-  // takes page 0, masked below.
-  bf16x8_t kf[KT][KS];
-  u32x4_t vf[PS * DT];
+  const int total = sq.len + sq.count;
+  if (!sq.ok || sq.count == 0 || c0 * kPBlock >= total) return;
+  const int c1 = min(c0 + span, (total + kPBlock - 1) / kPBlock);
+  const int rows = sq.count * G;
+  if (row0 >= rows) return;
+  const float sc = scale * kPLog2e;
+  // Pages past the sequence become the block's first; one that is none becomes page 0, its bit set.
   uint32_t bad = 0;
-  if (active) {
-    const int32_t* row = pg.table + (size_t)b * pg.ld;
-    const int P = 1 << pg.log2p;
-    const uint16_t *kb[GR], *vb[GR];
+  auto settle = [&](int c) {
+    uint32_t top = 0, none = 0;
 #pragma unroll
-    for (int j = 0; j < GR; ++j) {
-      const int at = a0 + 16 * j < total ? a0 + 16 * j : a0;
-      int page = row[at >> pg.log2p];
-      if ((unsigned)page >= (unsigned)pg.n_pages) {
-        page = 0;
-        bad |= 1u << j;
+    for (int g = 0; g < NG; ++g) top = max(top, (uint32_t)ids[g]);
+    if ((c + 1) * kPBlock > total || top >= (uint32_t)pg.n_pages) {
+      auto fit = [&](int id, int g) { return c * kPBlock + g * GS < total ? id : ids[0]; };
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        const int id = fit(idk[g], own + g);
+        idk[g] = (unsigned)id < (unsigned)pg.n_pages ? id : 0;
       }
-      const int in = at & (P - 1);
-      kb[j] = pg.k + (int64_t)page * pg.k_stride + ((size_t)h * P + in) * D;
-      vb[j] = pg.vt + (int64_t)page * pg.vt_stride + (size_t)h * D * P + in;
+#pragma unroll
+      for (int g = NG - 1; g >= 0; --g) {
+        const int id = fit(ids[g], g);
+        const bool there = (unsigned)id < (unsigned)pg.n_pages;
+        ids[g] = there ? id : 0;
+        none |= there ? 0u : 1u << g;
+      }
     }
-    // K rows of tile kt in the order row r -> key 32(kt/2) + 8(r/4) + 4(kt%2) + r%4, so that a lane's scores are
-    // the eight consecutive keys of its quad that P's operand wants.
+    return none;
+  };
+  bf16x8_t kf[KT][KS];
+  u32x4_t vf[ST][DW];
+  const uint16_t* k_head = pg.k + (size_t)h * P * D;
+  const uint16_t* v_head = pg.vt + ((size_t)h * D + 32 * wave) * P;
+  const uint32_t k_lane = col * D + quad * 8;
+  auto load_k = [&](int c) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const int kk = 8 * (col >> 2) + 4 * (kt & 1) + (col & 3);
-      const uint16_t* kr = (col >= 8 ? kb[2 * (kt >> 1) + 1] : kb[2 * (kt >> 1)]) + (kk & 15) * D + quad * 8;
+      const int in = (c * kPBlock + 16 * (wave * KT + kt)) & (P - 1);
+      const uint16_t* kr = k_head + ((uint64_t)(uint32_t)idk[kt * 16 / GS] * pg.k_stride + in * D);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = *reinterpret_cast<const bf16x8_t*>(kr + ks * 32);
+      for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = *reinterpret_cast<const bf16x8_t*>(kr + (k_lane + ks * 32));
     }
+  };
+  // V^T rows: dims 32 wave + 16dt + col, keys 32s + 8quad + 0..7 of the block.
+  const uint32_t v_lane = col * P + 8 * (GS == 16 ? quad & 1 : quad);
+  auto load_v = [&](int c) {
 #pragma unroll
-    for (int s = 0; s < PS; ++s) {
-      const uint16_t* vr = (quad >= 2 ? vb[2 * s + 1] : vb[2 * s]) + (size_t)col * P + 8 * (quad & 1);
+    for (int s = 0; s < ST; ++s) {
+      auto base = [&](int i) {
+        const int key = 32 * s + 16 * i;
+        return v_head + ((uint64_t)(uint32_t)ids[key / GS] * pg.vt_stride + (GS < 64 ? key & (P - 1) : (c * kPBlock + key) & (P - 1)));
+      };
+      if constexpr (GS == 16) {
+        const uint16_t *b0 = base(0), *b1 = base(1);
+        const uint16_t* vr = (quad >= 2 ? b1 : b0) + v_lane;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) vf[s * DT + dt] = *reinterpret_cast<const u32x4_t*>(vr + (size_t)dt * 16 * P);
-    }
-    // Slots past the sequence hold anything: their values are zeroed, for 0 * NaN is NaN.
-    if (a0 + ATOM > total || bad) {
+        for (int dt = 0; dt < DW; ++dt) vf[s][dt] = *reinterpret_cast<const u32x4_t*>(vr + dt * 16 * P);
+      } else {
+        const uint16_t* vr = base(0);
 #pragma unroll
-      for (int s = 0; s < PS; ++s) {
-        int n = min(max(total - (a0 + 32 * s + 8 * quad), 0), 8);
-        if ((bad >> (2 * s + (quad >> 1))) & 1) n = 0;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) vf[s * DT + dt] = first_keys(vf[s * DT + dt], n);
+        for (int dt = 0; dt < DW; ++dt) vf[s][dt] = *reinterpret_cast<const u32x4_t*>(vr + (v_lane + dt * 16 * P));
       }
     }
-  }
-  // New tokens' values that are no numbers must not reach the rows before them.
-  const bool odd = active && sq.count > 1 && a0 + ATOM > sq.len + 1 && any_not_finite(vf);
+  };
 
-  const int rows = sq.count * G;
-  const int nact = min(kPWaves, (total - key0 + ATOM - 1) / ATOM);
-  const float sc = scale * kPLog2e;
-  for (int r0 = 0; r0 < rows; r0 += 16) {
-    const int n = min(16, rows - r0);
-    if (active) {
-      const int qr = r0 + min(col, n - 1);
-      const int t = qr / G;
-      const int last = col < n ? sq.len + t : -1;  // the last position this row sees
-      const uint16_t* qp = q + (((size_t)b * T + t) * Hq + h * G + qr % G) * D + quad * 8;
-      bf16x8_t qf[KS];
+  bad = settle(c0);
+  load_k(c0);
+  load_v(c0);
+  bf16x8_t qf[KS];
+  if constexpr (W == 1) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
-      float s[KT][4];
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(bf16x8_t, qr[ks]);
+  } else {
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < QN; ++i) {
+      const int e = threadIdx.x + i * 2 * D;
+      if (e < W * 16 * (D / 8)) *reinterpret_cast<u32x4_t*>(&q_lds[e / (D / 8) * QP + e % (D / 8) * 8]) = qr[i];
+    }
+    lds_barrier();
+  }
+
+  // The pair's and the group's maximum (log2 units) and sum of this lane's row of every tile, and its outputs.
+  float am[W], al[W], gm[W], gl[W];
+  f32x4_t ao[W][DW], go[W][DW];
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) acc = mfma16x16x32(kf[kt][ks], qf[ks], acc);
+  for (int w = 0; w < W; ++w) {
+    am[w] = gm[w] = -INFINITY;
+    al[w] = gl[w] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[kt][i] = acc[i] * sc;
+    for (int dt = 0; dt < DW; ++dt) ao[w][dt] = go[w][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int c = c0; c < c1; ++c) {
+    const int key0 = c * kPBlock;
+    const bool more = c + 1 < c1;
+    const bool edge = key0 + kPBlock > sq.len + 1 || bad;  // some row does not see, or may not read, some key
+    if (more) find(c + 1);
+    float s[W][KT][4];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w && row0 + 16 * w >= rows) continue;
+      if constexpr (W != 1) {
+        const uint16_t* qp = &q_lds[(16 * w + col) * QP + quad * 8];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
       }
-      if (bad) {
+      f32x4_t acc[KT];
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-          if ((bad >> (2 * (kt >> 1) + (quad >> 1))) & 1)
+      for (int kt = 0; kt < KT; ++kt) acc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[kt][i] = __builtin_nanf("");
-      }
-      const int k0 = a0 + 8 * quad;
-      float mx = -INFINITY;
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) acc[kt] = mfma16x16x32(kf[kt][ks], qf[ks], acc[kt]);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (k0 + 32 * (kt >> 1) + 4 * (kt & 1) + i > last) s[kt][i] = -INFINITY;
-          mx = fmaxf(mx, s[kt][i]);
+        for (int i = 0; i < 4; ++i) s[w][kt][i] = acc[kt][i];
+    }
+    uint32_t bad_next = 0;
+    if (more) {
+      bad_next = settle(c + 1);
+      load_k(c + 1);
+    }
+    if (edge) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const int r = row0 + 16 * w + col;
+        const int last = (r < rows ? sq.len + r / G : -1) - (key0 + 16 * wave * KT + 4 * quad);  // of the lane's keys
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const bool none = (bad >> (own + kt * 16 / GS)) & 1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[w][kt][i] = 16 * kt + i > last ? -INFINITY : none ? __builtin_nanf("") : s[w][kt][i];
         }
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mref = mx == -INFINITY ? 0.f : mx;
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w && row0 + 16 * w >= rows) continue;
+      float mx = s[w][0][0];
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[w][kt][i]);
+      mx = quads_max(mx);
+      if (quad == 0) m_lds[16 * w + col][wave] = mx;
+    }
+    lds_barrier();
+    float mx[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w && row0 + 16 * w >= rows) continue;
+      float m = m_lds[16 * w + col][0];
+#pragma unroll
+      for (int v = 1; v < WAVES; ++v) m = fmaxf(m, m_lds[16 * w + col][v]);
+      mx[w] = m * sc;
+      const float ref = m == -INFINITY ? 0.f : mx[w];
       // P as the sum of two bf16 terms (2^-17 of each weight; one term's 2^-9 would be as large as the output's own
-      // rounding). The matrix cores wait for memory either way.
-      u32x4_t hi[PS], lo[PS];
+      // rounding).
       float sum = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < PS; ++ks)
+      for (int kt = 0; kt < KT; ++kt) {
+        u32x2_t hi, lo;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int kt = 2 * ks + (w >> 1), i = 2 * (w & 1);
-          const float p0 = __builtin_amdgcn_exp2f(s[kt][i] - mref), p1 = __builtin_amdgcn_exp2f(s[kt][i + 1] - mref);
+        for (int v = 0; v < 2; ++v) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[w][kt][2 * v], sc, -ref));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[w][kt][2 * v + 1], sc, -ref));
           sum += p0;
           sum += p1;
-          const uint32_t h0 = f32_to_bf16_bits(p0), h1 = f32_to_bf16_bits(p1);
-          hi[ks][w] = h0 | (h1 << 16);
-          lo[ks][w] = (uint32_t)f32_to_bf16_bits(p0 - bf16_bits_to_f32(h0)) |
-                      ((uint32_t)f32_to_bf16_bits(p1 - bf16_bits_to_f32(h1)) << 16);
+          hi[v] = two_bf16(p0, p1);
+          lo[v] = two_bf16(p0 - __uint_as_float(hi[v] << 16), p1 - __uint_as_float(hi[v] & 0xffff0000u));
         }
-      sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      f32x4_t acc[DT];
+        // keys 16g + 4quad .. + 3: half of the piece that lane (col, quad g, quad / 2) of step g / 2 takes
+        const int g = wave * KT + kt, at = col + 16 * (2 * (g & 1) + (quad >> 1));
+        reinterpret_cast<u32x2_t*>(&p_lds[w][0][g >> 1][at])[quad & 1] = hi;
+        reinterpret_cast<u32x2_t*>(&p_lds[w][1][g >> 1][at])[quad & 1] = lo;
+      }
+      sum = quads_sum(sum);
+      if (quad == 0) l_lds[16 * w + col][wave] = sum;
+    }
+    lds_barrier();
+    f32x4_t acc[W][DW];
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-      if (!odd) {
+    for (int w = 0; w < W; ++w)
 #pragma unroll
-        for (int ks = 0; ks < PS; ++ks)
+      for (int dt = 0; dt < DW; ++dt) acc[w][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    // Slots past the sequence hold anything: their values are zeroed, for 0 * NaN is NaN. So are new tokens' values that
+    // are no numbers, which no earlier row may meet: the outputs that see one begin as NaN instead.
+    if (edge) {
+      uint32_t odd[DW] = {};  // bits 4st + v and 16 + 4st + v: the halves of word v of the step's piece are no numbers
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, vf[ks * DT + dt]);
-            acc[dt] = mfma16x16x32(v, __builtin_bit_cast(bf16x8_t, hi[ks]), acc[dt]);
-            acc[dt] = mfma16x16x32(v, __builtin_bit_cast(bf16x8_t, lo[ks]), acc[dt]);
+      for (int st = 0; st < ST; ++st) {
+        int n = min(max(total - (key0 + 32 * st + 8 * quad), 0), 8);
+        if ((bad >> (GS == 16 ? 2 * st + (quad >> 1) : 32 * st / GS)) & 1) n = 0;
+#pragma unroll
+        for (int dt = 0; dt < DW; ++dt) {
+          vf[st][dt] = first_keys(vf[st][dt], n);
+          if (sq.count == 1) continue;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            // an exponent of all ones carries into the half's top bit
+            const uint32_t no = ((vf[st][dt][v] & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u;
+            vf[st][dt][v] &= ~(no * 0xffffu);
+            odd[dt] |= no << (4 * st + v);
           }
-      } else {  // token by token, each with the values that it sees
-        const int t1 = (r0 + n - 1) / G;
+          asm volatile("" : "+v"(vf[st][dt]), "+v"(odd[dt]));  // piece by piece: interleaved, they take twice the registers
+        }
+      }
+      if (__any((odd[0] | odd[1]) != 0)) {
+        // How many of them each output's row sees: a product of the odd values' and the seen keys' ones.
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          for (int tt = r0 / G; tt <= t1; ++tt) {
-            f32x4_t one = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < W; ++w) {
+          const int r = row0 + 16 * w + col, seen = (r < rows ? sq.len + r / G + 1 : 0) - (key0 + 8 * quad);
 #pragma unroll
-            for (int ks = 0; ks < PS; ++ks) {
-              const int nk = min(max(sq.len + tt + 1 - (k0 + 32 * ks), 0), 8);
-              const bf16x8_t v = __builtin_bit_cast(bf16x8_t, first_keys(vf[ks * DT + dt], nk));
-              one = mfma16x16x32(v, __builtin_bit_cast(bf16x8_t, hi[ks]), one);
-              one = mfma16x16x32(v, __builtin_bit_cast(bf16x8_t, lo[ks]), one);
+          for (int dt = 0; dt < DW; ++dt) {
+            for (int st = 0; st < ST; ++st) {
+              u32x4_t a, k = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+              for (int v = 0; v < 4; ++v) a[v] = (odd[dt] >> (4 * st + v) & 0x00010001u) * 0x3f80u;
+              k = first_keys(k, min(max(seen - 32 * st, 0), 8));
+              acc[w][dt] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, k), acc[w][dt]);
             }
-            if (tt == t) acc[dt] = one;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[w][dt][i] = acc[w][dt][i] > 0.f ? __builtin_nanf("") : 0.f;
           }
-      }
-      if (col < n) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          *reinterpret_cast<f32x4_t*>(&o_lds[wave][col * OP + dt * 16 + quad * 4]) = acc[dt];
-        if (quad == 0) {
-          ml_lds[wave][col][0] = mx;
-          ml_lds[wave][col][1] = sum;
         }
       }
     }
-    __syncthreads();
-    // Fold the atoms in order: thread e takes four dims of a row.
-    for (int e = threadIdx.x; e < n * (D / 4); e += 64 * kPWaves) {
-      const int r = e / (D / 4), d = (e % (D / 4)) * 4;
-      float m = -INFINITY;
-      for (int w = 0; w < nact; ++w) m = fmaxf(m, ml_lds[w][r][0]);
-      const float mref = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
-      f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-      for (int w = 0; w < nact; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ml_lds[w][r][0] - mref);
-        l = fmaf(f, ml_lds[w][r][1], l);
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(&o_lds[w][r * OP + d]);
+    float l[W];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = fmaf(f, v[i], acc[i]);
-      }
-      const int qr = r0 + r;
-      if (nblk == 1) {
-        const size_t orow = (size_t)b * T + qr / G;
-        const int head = h * G + qr % G;
-        const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
-        uint16_t* op = o.out + (orow * Hq + head) * D + d;
+    for (int w = 0; w < W; ++w) {
+      if (w && row0 + 16 * w >= rows) continue;
+      l[w] = l_lds[16 * w + col][0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) op[i] = finished(acc[i], l, gp, d + i);
-      } else {
-        const size_t at = (((size_t)b * Hkv + h) * nblk + c) * (size_t)(T * G) + qr;
-        *reinterpret_cast<f32x4_t*>(part_o + at * D + d) = acc;
-        if (d == 0) {
-          part_ml[2 * at] = m;
-          part_ml[2 * at + 1] = l;
-        }
+      for (int v = 1; v < WAVES; ++v) l[w] += l_lds[16 * w + col][v];
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const bf16x8_t hi = __builtin_bit_cast(bf16x8_t, p_lds[w][0][st][lane]);
+        const bf16x8_t lo = __builtin_bit_cast(bf16x8_t, p_lds[w][1][st][lane]);
+#pragma unroll
+        for (int dt = 0; dt < DW; ++dt) acc[w][dt] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, vf[st][dt]), hi, acc[w][dt]);
+#pragma unroll
+        for (int dt = 0; dt < DW; ++dt) acc[w][dt] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, vf[st][dt]), lo, acc[w][dt]);
       }
     }
-    __syncthreads();
+    if (more) load_v(c + 1);
+    bad = bad_next;
+    const bool end = !more || (c + 1) % kPPair == 0;  // of the pair
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w && row0 + 16 * w >= rows) continue;
+      const Join j = join(am[w], al[w], mx[w], l[w]);
+#pragma unroll
+      for (int dt = 0; dt < DW; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ao[w][dt][i] = fmaf(acc[w][dt][i], j.part, ao[w][dt][i] * j.before);
+      if (!end) continue;
+      const Join g = join(gm[w], gl[w], am[w], al[w]);
+#pragma unroll
+      for (int dt = 0; dt < DW; ++dt) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) go[w][dt][i] = fmaf(ao[w][dt][i], g.part, go[w][dt][i] * g.before);
+        ao[w][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+      am[w] = -INFINITY;
+      al[w] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const int r = row0 + 16 * w + col, d0 = wave * 32 + quad * 4;
+    if (r >= rows) continue;
+    if (slots > 1) {  // a part, for the merge
+      const size_t at = (((size_t)b * Hkv + h) * slots + blockIdx.x) * (size_t)(T * G) + r;
+#pragma unroll
+      for (int dt = 0; dt < DW; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * D + d0 + dt * 16) = go[w][dt];
+      if (wave == 0 && quad == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{gm[w], gl[w]};
+      continue;
+    }
+    const size_t orow = (size_t)b * T + r / G;
+    const int head = h * G + r % G;
+    const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
+    const float inv = 1.f / gl[w];
+#pragma unroll
+    for (int dt = 0; dt < DW; ++dt) {
+      u32x2_t two;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        two[i] = finished(go[w][dt][2 * i], inv, gp, d0 + dt * 16 + 2 * i) |
+                 (uint32_t)finished(go[w][dt][2 * i + 1], inv, gp, d0 + dt * 16 + 2 * i + 1) << 16;
+      *reinterpret_cast<u32x2_t*>(o.out + (orow * Hq + head) * D + d0 + dt * 16) = two;
+    }
   }
 }
 
-// One workgroup per (query head, token, sequence): the row's blocks joined, wave w taking blocks w, w + 4, ..., the
-// waves' sums then in order.
-template <int D>
-__global__ __launch_bounds__(64 * kPMergeWaves) void paged_merge_kernel(Pages pg, int T, int Hq, int Hkv, int room, int nblk,
-                                                                        const float* __restrict__ part_o,
-                                                                        const float* __restrict__ part_ml, Out o) {
-  constexpr int E = D / 64;
-  __shared__ float red[kPMergeWaves], suml[kPMergeWaves], sumo[kPMergeWaves][D];
-  const int head = blockIdx.x, t = blockIdx.y, b = blockIdx.z, G = Hq / Hkv, h = head / G;
+// The rows' groups joined: group g in order onto lane g % 4 of four, then the four in order. A row is one wave's (kSplit
+// 1), holding all four, or four waves' (kSplit 4) where there are many groups. A slot of the workspace is a group
+// (kJoined), or a pair, joined to its group here as the block kernel would.
+template <int D, bool kJoined, int kSplit>
+__global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int B, int T, int Hq, int Hkv, int room, int slots,
+                                                          const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                                                          Out o) {
+  constexpr int E = D / 64, L = 4 / kSplit;  // lanes of groups that a wave holds
+  constexpr int N = kJoined ? 1 : kPGroup / kPPair;        // slots of a group
+  constexpr int UN = (kSplit == 1 ? 8 : 16) / (L * N) < 1 ? 1 : (kSplit == 1 ? 8 : 16) / (L * N);  // rounds of groups loaded at once
+  __shared__ float ml[kSplit == 1 ? 1 : 4][2], sum[kSplit == 1 ? 1 : 4][kSplit == 1 ? 1 : D];
   const int lane = threadIdx.x & 63, wave = wave_id();
+  const int heads = kSplit == 1 ? (Hq + 3) / 4 : Hq;  // workgroups of a token
+  const int head = kSplit == 1 ? (int)(blockIdx.x % heads) * 4 + wave : (int)(blockIdx.x % heads), t = blockIdx.x / heads;
+  const int b = blockIdx.y, G = Hq / Hkv, h = head / G;
+  if (head >= Hq) return;
   const Sequence sq = sequence_of(pg, b, T, room);
   const size_t orow = (size_t)b * T + t;
   uint16_t* op = o.out + (orow * Hq + head) * D;
   if (!sq.ok || t >= sq.count) {
-    for (int d = threadIdx.x; d < D; d += 64 * kPMergeWaves) op[d] = sq.ok ? 0 : kNanBits;
+    if (kSplit == 1 || wave == 0)
+      for (int d = lane; d < D; d += 64) op[d] = sq.ok ? 0 : kNanBits;
     return;
   }
-  const int nb = (sq.len + t) / paged_block(D) + 1;  // the blocks that this row sees
-  const size_t base = ((size_t)b * Hkv + h) * nblk * (size_t)(T * G) + (size_t)t * G + head % G;
+  // the blocks, pairs and groups that this row sees
+  const int nb = (sq.len + t) / kPBlock + 1, np = (nb + kPPair - 1) / kPPair, ng = (nb + kPGroup - 1) / kPGroup;
   const size_t step = (size_t)T * G;
-  float m = -INFINITY;
-  for (int c = threadIdx.x; c < nb; c += 64 * kPMergeWaves) m = fmaxf(m, part_ml[2 * (base + c * step)]);
+  const size_t base = ((size_t)b * Hkv + h) * slots * step + (size_t)t * G + head % G;
+  float m[L], l[L], acc[L][E];
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s, 64));
-  if (lane == 0) red[wave] = m;
-  __syncthreads();
+  for (int i = 0; i < L; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
 #pragma unroll
-  for (int w = 0; w < kPMergeWaves; ++w) m = fmaxf(m, red[w]);
-  const float mref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc[E] = {};
-  for (int c = wave; c < nb; c += kPMergeWaves) {
-    const size_t at = base + c * step;
-    const float f = __builtin_amdgcn_exp2f(part_ml[2 * at] - mref);
-    l = fmaf(f, part_ml[2 * at + 1], l);
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(f, part_o[at * D + lane + 64 * e], acc[e]);
+    for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
   }
-  if (lane == 0) suml[wave] = l;
+  for (int g0 = kSplit == 1 ? 0 : wave; g0 < ng; g0 += 4 * UN) {
+    float pm[UN][L][N], pl[UN][L][N], po[UN][L][N][E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) sumo[wave][lane + 64 * e] = acc[e];
-  __syncthreads();
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const int slot = min((g0 + 4 * u + i) * N + n, (kJoined ? ng : np) - 1);
+          const size_t at = base + (size_t)slot * step;
+          const float2 two = reinterpret_cast<const float2*>(part_ml)[at];
+          pm[u][i][n] = two.x;
+          pl[u][i][n] = two.y;
+#pragma unroll
+          for (int e = 0; e < E; ++e) po[u][i][n][e] = part_o[at * D + lane + 64 * e];
+        }
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const int g = g0 + 4 * u + i;
+        if (g >= ng) continue;
+        float gm = -INFINITY, gl = 0.f, go[E] = {};
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (kJoined || g * N + n < np) {
+            const Join j = join(gm, gl, pm[u][i][n], pl[u][i][n]);
+#pragma unroll
+            for (int e = 0; e < E; ++e) go[e] = fmaf(po[u][i][n][e], j.part, go[e] * j.before);
+          }
+        const Join j = join(m[i], l[i], gm, gl);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[i][e] = fmaf(go[e], j.part, acc[i][e] * j.before);
+      }
+  }
   const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
-  for (int d = threadIdx.x; d < D; d += 64 * kPMergeWaves) {
-    float lt = 0.f, ot = 0.f;
+  if constexpr (kSplit == 1) {
+    float rm = -INFINITY, rl = 0.f, ro[E] = {};
 #pragma unroll
-    for (int w = 0; w < kPMergeWaves; ++w) {
-      lt += suml[w];
-      ot += sumo[w][d];
+    for (int i = 0; i < 4; ++i) {
+      const Join j = join(rm, rl, m[i], l[i]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) ro[e] = fmaf(acc[i][e], j.part, ro[e] * j.before);
     }
-    op[d] = finished(ot, lt, gp, d);
+    const float inv = 1.f / rl;
+#pragma unroll
+    for (int e = 0; e < E; ++e) op[lane + 64 * e] = finished(ro[e], inv, gp, lane + 64 * e);
+  } else {
+    if (lane == 0) {
+      ml[wave][0] = m[0];
+      ml[wave][1] = l[0];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum[wave][lane + 64 * e] = acc[0][e];
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += 256) {
+      float rm = -INFINITY, rl = 0.f, ro = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const Join j = join(rm, rl, ml[w][0], ml[w][1]);
+        ro = fmaf(sum[w][d], j.part, ro * j.before);
+      }
+      op[d] = finished(ro, 1.f / rl, gp, d);
+    }
   }
 }
 
+int paged_blocks(int keys) { return (keys + kPBlock - 1) / kPBlock; }
+
+// Blocks per workgroup: a pair, or a group. Groups move the least (an eighth of the blocks' parts is written and read
+// again, which counts for many rows) and keep loads in flight from block to block, but need enough of them to fill the
+// card, also where sequences end early; sequences of at most one group then also need no merge. Measured, us a call, pairs /
+// groups, 8 kv heads of 128 dims, 4 query heads each, B sequences: one token: 1 x 32768 keys (264 groups) 41.4 / 47.2, 32 of
+// up to 2048 (768, half of them past their end) 31.9 / 37.8, 16 x 8000 (1024) 114 / 107, 64 x 4000 (2048) 211 / 200; of one
+// group, 4 x 1000 13.0 / 22.4, 16 x 500 14.4 / 14.7, 64 x 300 29.6 / 21.3. Eight tokens: 4 x 4000 (128) 24.5 / 29.4,
+// 1 x 32768 48.2 / 49.7, 16 x 2000 (256) 41.5 / 35.5, 64 x 4000 258 / 220.
+int paged_span(int B, int Hkv, int nblk, int rows) {
+  const int64_t all = (int64_t)B * Hkv * ((nblk + kPGroup - 1) / kPGroup);
+  return all >= (nblk <= kPGroup ? 128 : rows <= 16 ? 1024 : 256) ? kPGroup : kPPair;
+}
+
+int paged_slots(int nblk, int span) { return (nblk + span - 1) / span; }
+
 size_t paged_workspace(int B, int T, int Hq, int Hkv, int D, int keys) {
-  const size_t nblk = ((size_t)keys + paged_block(D) - 1) / paged_block(D);
-  if (nblk == 1) return 0;
-  return (size_t)B * Hkv * nblk * T * (Hq / Hkv) * (D + 2) * sizeof(float);
+  const int nblk = paged_blocks(keys), slots = paged_slots(nblk, paged_span(B, Hkv, nblk, T * (Hq / Hkv)));
+  if (slots == 1) return 0;
+  return (size_t)B * Hkv * slots * T * (Hq / Hkv) * (D + 2) * sizeof(float);
 }
 
 bool head_dim_ok(int D) { return D == 64 || D == 128 || D == 256; }
@@ -425,7 +675,7 @@ bool head_dim_ok(int D) { return D == 64 || D == 128 || D == 256; }
 int check_pages(const skinny_paged_kv* kv, int B, int T, int Hq, Pages& pg, const char* what) {
   SKINNY_CHECK_ARG(kv && kv->lengths && kv->pages && kv->k_pages && kv->vt_pages, "%s: null pointer", what);
   SKINNY_CHECK_ARG(head_dim_ok(kv->head_dim), "%s: head dim %d unsupported (64, 128 or 256)", what, kv->head_dim);
-  SKINNY_CHECK_ARG(kv->n_kv >= 1 && kv->n_kv <= 65535 && Hq >= kv->n_kv && Hq <= 65535 && Hq % kv->n_kv == 0,
+  SKINNY_CHECK_ARG(kv->n_kv >= 1 && kv->n_kv <= 32767 && Hq >= kv->n_kv && Hq <= 65535 && Hq % kv->n_kv == 0,
                    "%s: Hq=%d must be a multiple of Hkv=%d", what, Hq, kv->n_kv);
   SKINNY_CHECK_ARG(B >= 1 && B <= 65535 && T >= 1 && T <= 65535, "%s: B=%d sequences of T=%d tokens (1 to 65535 each)",
                    what, B, T);
@@ -435,28 +685,49 @@ int check_pages(const skinny_paged_kv* kv, int B, int T, int Hq, Pages& pg, cons
                        (int64_t)kv->max_pages * P <= (1 << 30),
                    "%s: n_pages=%d, max_pages=%d, ld_pages=%d", what, kv->n_pages, kv->max_pages, kv->ld_pages);
   const int64_t need = (int64_t)kv->n_kv * P * kv->head_dim;
-  SKINNY_CHECK_ARG(kv->k_stride >= need && kv->vt_stride >= need && kv->k_stride % 8 == 0 && kv->vt_stride % 8 == 0,
-                   "%s: page strides %lld, %lld (multiples of 8, at least Hkv*P*D=%lld)", what, (long long)kv->k_stride,
+  SKINNY_CHECK_ARG(kv->k_stride >= need && kv->vt_stride >= need && kv->k_stride % 8 == 0 && kv->vt_stride % 8 == 0 &&
+                       kv->k_stride <= INT32_MAX && kv->vt_stride <= INT32_MAX,
+                   "%s: page strides %lld, %lld (multiples of 8 below 2^31, at least Hkv*P*D=%lld)", what, (long long)kv->k_stride,
                    (long long)kv->vt_stride, (long long)need);
   SKINNY_CHECK_ARG(skinny_aligned(kv->k_pages, 16) && skinny_aligned(kv->vt_pages, 16) && skinny_aligned(kv->lengths, 4) &&
                        skinny_aligned(kv->counts, 4) && skinny_aligned(kv->pages, 4),
                    "%s: misaligned cache", what);
-  pg = Pages{kv->lengths, kv->counts, kv->pages, kv->k_pages, kv->vt_pages, kv->k_stride, kv->vt_stride, kv->ld_pages,
-             kv->n_pages, __builtin_ctz(P)};
+  pg = Pages{kv->lengths, kv->counts, kv->pages, kv->k_pages, kv->vt_pages, (uint32_t)kv->k_stride, (uint32_t)kv->vt_stride, kv->ld_pages,
+             kv->max_pages, kv->n_pages, __builtin_ctz(P)};
   return SKINNY_OK;
 }
 
 template <int D>
 int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, float* ws,
                            const Out& o, hipStream_t s) {
-  const int nblk = (keys + paged_block(D) - 1) / paged_block(D);
-  const size_t parts = (size_t)B * Hkv * nblk * T * (Hq / Hkv);
-  hipLaunchKernelGGL(paged_block_kernel<D>, dim3(nblk, Hkv, B), dim3(64 * kPWaves), 0, s, pg, q, T, Hq, Hkv, keys, scale, nblk,
-                     ws, ws + parts * D, o);
+  const int rows = T * (Hq / Hkv);
+  const int nblk = paged_blocks(keys), span = paged_span(B, Hkv, nblk, rows), slots = paged_slots(nblk, span);
+  float* ml = ws + (size_t)B * Hkv * slots * rows * D;
+  const int halves = rows > 32;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(slots, Hkv << halves, B), dim3(2 * D), 0, s, pg, q, T, Hq, Hkv, keys, scale, span, slots,
+                       halves, ws, ml, o);
+  };
+  auto page = [&](auto w) {
+    constexpr int W = decltype(w)::value;
+    if (pg.log2p == 4) go(paged_block_kernel<D, W, 16>);
+    else if (pg.log2p == 5) go(paged_block_kernel<D, W, 32>);
+    else go(paged_block_kernel<D, W, 64>);
+  };
+  if (rows <= 16) page(std::integral_constant<int, 1>{});
+  else page(std::integral_constant<int, 2>{});
   if (const int rc = skinny_check_launch("paged_attention")) return rc;
-  if (nblk == 1) return SKINNY_OK;
-  hipLaunchKernelGGL(paged_merge_kernel<D>, dim3(Hq, T, B), dim3(64 * kPMergeWaves), 0, s, pg, T, Hq, Hkv, keys, nblk, ws,
-                     ws + parts * D, o);
+  if (slots == 1) return SKINNY_OK;
+  const int groups = (nblk + kPGroup - 1) / kPGroup;
+  // four waves a row where a wave's groups would be many, or the rows alone would not fill the card
+  const bool split = groups > 8 || (int64_t)B * T * Hq <= 1024;
+  auto merge = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((split ? Hq : (Hq + 3) / 4) * T, B), dim3(256), 0, s, pg, B, T, Hq, Hkv, keys, slots, ws, ml, o);
+  };
+  if (span == kPGroup && split) merge(paged_merge_kernel<D, true, 4>);
+  else if (span == kPGroup) merge(paged_merge_kernel<D, true, 1>);
+  else if (split) merge(paged_merge_kernel<D, false, 4>);
+  else merge(paged_merge_kernel<D, false, 1>);
   return skinny_check_launch("paged_attention merge");
 }
 

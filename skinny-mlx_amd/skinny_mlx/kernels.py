@@ -331,34 +331,42 @@ def attention_general_prompt(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: i
 
 def _on_device(t: torch.Tensor):
     """Makes t's device current where it is not: the C side launches on the current device."""
-    return _NO_GUARD if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NO_GUARD if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
-def _paged_kv(like: torch.Tensor, lengths: torch.Tensor, counts, pages: torch.Tensor, k_pages: torch.Tensor,
+def _paged_kv(dev: int, lengths: torch.Tensor, counts, pages: torch.Tensor, k_pages: torch.Tensor,
               vt_pages: torch.Tensor) -> tuple["_lib.PagedKV", int]:
-    """The cache of the paged calls as the C side takes it, and its number of sequences."""
-    dev = like.get_device()
-    _req(k_pages.dtype == BF16 and k_pages.dim() == 4 and k_pages.get_device() == dev and k_pages.numel() > 0,
-         "k_pages must be bf16 [n_pages, Hkv, page, D], on the rows' device")
+    """The cache of the paged calls as the C side takes it, and its number of sequences; all on device `dev`."""
+    # (these calls are the short ones of a decode step: no message is formed before it is needed)
+    if not (k_pages.dtype == BF16 and k_pages.dim() == 4 and k_pages.get_device() == dev and k_pages.numel() > 0):
+        raise ValueError("k_pages must be bf16 [n_pages, Hkv, page, D], on the rows' device")
     n, h, p, d = k_pages.shape
-    _req(vt_pages.dtype == BF16 and vt_pages.shape == (n, h, d, p) and vt_pages.get_device() == dev,
-         f"vt_pages must be bf16 [{n}, {h}, {d}, {p}] (V transposed), on the rows' device")
-    _req((k_pages.stride()[1:] == (p * d, d, 1) or k_pages[0].is_contiguous())
-         and (vt_pages.stride()[1:] == (p * d, p, 1) or vt_pages[0].is_contiguous()), "a page must be contiguous")
-    _req(lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.is_contiguous() and lengths.get_device() == dev
-         and lengths.shape[0] > 0, "lengths must be contiguous int32 [B] on the rows' device")
-    b = lengths.shape[0]
-    _req(counts is None or (counts.dtype == torch.int32 and tuple(counts.shape) == (b,) and counts.is_contiguous()
-                            and counts.get_device() == dev), f"counts must be contiguous int32 [{b}] on the rows' device")
-    _req(pages.dtype == torch.int32 and pages.dim() == 2 and pages.shape[0] == b and pages.shape[1] > 0
-         and pages.get_device() == dev and (pages.shape[1] == 1 or pages.stride(1) == 1)
-         and (b == 1 or pages.stride(0) >= pages.shape[1]),
-         f"pages must be int32 [{b}, max_pages] rows on the rows' device")
-    w = pages.shape[1]
+    if not (vt_pages.dtype == BF16 and vt_pages.shape == (n, h, d, p) and vt_pages.get_device() == dev):
+        raise ValueError(f"vt_pages must be bf16 [{n}, {h}, {d}, {p}] (V transposed), on the rows' device")
+    ks, vs, pd = k_pages.stride(), vt_pages.stride(), p * d
+    if not ((ks[1:] == (pd, d, 1) or k_pages[0].is_contiguous()) and (vs[1:] == (pd, p, 1) or vt_pages[0].is_contiguous())):
+        raise ValueError("a page must be contiguous")
+    if not (lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.is_contiguous() and lengths.get_device() == dev
+            and lengths.numel() > 0):
+        raise ValueError("lengths must be contiguous int32 [B] on the rows' device")
+    b = lengths.numel()
+    if counts is not None and not (counts.dtype == torch.int32 and counts.shape == (b,) and counts.is_contiguous()
+                                   and counts.get_device() == dev):
+        raise ValueError(f"counts must be contiguous int32 [{b}] on the rows' device")
+    if not (pages.dtype == torch.int32 and pages.dim() == 2 and pages.get_device() == dev):
+        raise ValueError(f"pages must be int32 [{b}, max_pages] on the rows' device")
+    rows, w = pages.shape
+    ld, step = pages.stride()
     # the stride of an axis of one entry is never stepped and may be anything
-    return _lib.PagedKV(lengths.data_ptr(), _lib.ptr(counts), pages.data_ptr(), w if b == 1 else pages.stride(0), w,
-                        k_pages.data_ptr(), vt_pages.data_ptr(), h * p * d if n == 1 else k_pages.stride(0),
-                        h * p * d if n == 1 else vt_pages.stride(0), n, p, h, d), b
+    if not (rows == b and w > 0 and (w == 1 or step == 1) and (b == 1 or w <= ld < 2 ** 31)):
+        raise ValueError(f"pages must be int32 [{b}, max_pages] rows")
+    return _lib.PagedKV(lengths.data_ptr(), None if counts is None else counts.data_ptr(), pages.data_ptr(),
+                        w if b == 1 else ld, w, k_pages.data_ptr(), vt_pages.data_ptr(), h * pd if n == 1 else ks[0],
+                        h * pd if n == 1 else vs[0], n, p, h, d), b
+
+
+def _fits(t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: int) -> bool:
+    return t.dtype == dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev
 
 
 def paged_store(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_stride: int, k_offset: int, v_offset: int,
@@ -375,35 +383,39 @@ def paged_store(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_stride:
     nowhere, their queries zero. A sequence that its row of `pages` cannot hold is not stored and its queries are NaN.
     lengths are not advanced: that is the caller's, after the step. A page written to must be one sequence's own."""
     _bf16_2d(qkv, "qkv")
-    kv, b = _paged_kv(qkv, lengths, counts, pages, k_pages, vt_pages)
-    rows, cols = qkv.shape
-    _req(kv.n_kv == n_kv and kv.head_dim == head_dim,
-         f"pages of {kv.n_kv} heads of {kv.head_dim} dims, the rows have {n_kv} of {head_dim}")
-    _req(rows > 0 and rows % b == 0, f"{rows} rows do not divide into {b} sequences")
-    _req(rows == 1 or cols <= qkv.stride(0) < 2 ** 31, "qkv rows overlap, or lie too far apart")
-    _req(n_q >= 1 and q_stride >= head_dim and (n_q - 1) * q_stride + head_dim <= cols and k_offset >= 0 and v_offset >= 0
-         and max(k_offset, v_offset) + n_kv * head_dim <= cols, f"heads do not fit the q|k|v rows of {cols}")
     dev = qkv.get_device()
-    _req(table.dtype == torch.float32 and table.dim() == 3 and tuple(table.shape[1:]) == (rotary_dim // 2, 2)
-         and rotary_dim % 2 == 0 and table.is_contiguous() and table.get_device() == dev,
-         f"table must be a rope_table_dim table for rotary_dim={rotary_dim}")
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        _req(w is None or (w.dtype == BF16 and tuple(w.shape) == (head_dim,) and w.is_contiguous()
-                           and w.get_device() == dev), f"{name} must be contiguous bf16 [{head_dim}]")
-    _req(out is None or (out.dtype == BF16 and tuple(out.shape) == (rows, n_q, head_dim) and out.is_contiguous()
-                         and out.get_device() == dev), f"out must be contiguous bf16 [{rows}, {n_q}, {head_dim}]")
+    kv, b = _paged_kv(dev, lengths, counts, pages, k_pages, vt_pages)
+    rows, cols = qkv.shape
+    ld = cols if rows == 1 else qkv.stride(0)
+    if not (kv.n_kv == n_kv and kv.head_dim == head_dim):
+        raise ValueError(f"pages of {kv.n_kv} heads of {kv.head_dim} dims, the rows have {n_kv} of {head_dim}")
+    if not (rows > 0 and rows % b == 0):
+        raise ValueError(f"{rows} rows do not divide into {b} sequences")
+    if not cols <= ld < 2 ** 31:
+        raise ValueError("qkv rows overlap, or lie too far apart")
+    if not (n_q >= 1 and q_stride >= head_dim and (n_q - 1) * q_stride + head_dim <= cols and k_offset >= 0
+            and v_offset >= 0 and max(k_offset, v_offset) + n_kv * head_dim <= cols):
+        raise ValueError(f"heads do not fit the q|k|v rows of {cols}")
+    positions = table.shape[0] if table.dim() == 3 else 0
+    if rotary_dim % 2 or not _fits(table, torch.float32, (positions, rotary_dim // 2, 2), dev):
+        raise ValueError(f"table must be a rope_table_dim table for rotary_dim={rotary_dim}")
+    if q_norm is not None and not _fits(q_norm, BF16, (head_dim,), dev):
+        raise ValueError(f"q_norm must be contiguous bf16 [{head_dim}]")
+    if k_norm is not None and not _fits(k_norm, BF16, (head_dim,), dev):
+        raise ValueError(f"k_norm must be contiguous bf16 [{head_dim}]")
+    if out is not None and not _fits(out, BF16, (rows, n_q, head_dim), dev):
+        raise ValueError(f"out must be contiguous bf16 [{rows}, {n_q}, {head_dim}]")
     with _on_device(qkv):
-        q = torch.empty((rows, n_q, head_dim), dtype=BF16, device=qkv.device) if out is None else out
+        q = qkv.new_empty((rows, n_q, head_dim)) if out is None else out
         _lib.check(_lib.lib().skinny_paged_store_bf16(
-            qkv.data_ptr(), cols if rows == 1 else qkv.stride(0), b, rows // b, n_q, q_stride, k_offset, v_offset,
-            _lib.ptr(q_norm), _lib.ptr(k_norm), eps, rotary_dim, table.data_ptr(), table.shape[0], kv, q.data_ptr(),
-            _lib.stream_of(qkv)), "paged_store")
+            qkv.data_ptr(), ld, b, rows // b, n_q, q_stride, k_offset, v_offset, _lib.ptr(q_norm), _lib.ptr(k_norm), eps,
+            rotary_dim, table.data_ptr(), positions, kv, q.data_ptr(), _lib.stream_of(qkv)), "paged_store")
     return q
 
 
 def paged_attn_workspace(batch: int, tokens: int, n_q: int, n_kv: int, head_dim: int, keys: int, device) -> torch.Tensor:
-    """Workspace of paged_attention for calls of up to these sizes. It carries nothing from call to call; calls that may
-    overlap, on different streams or in graphs replayed side by side, each need their own."""
+    """Workspace of paged_attention for calls of these sizes. It carries nothing from call to call; calls that may overlap,
+    on different streams or in graphs replayed side by side, each need their own."""
     nbytes = int(_lib.lib().skinny_paged_attn_workspace_bytes(batch, tokens, n_q, n_kv, head_dim, keys))
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
@@ -420,34 +432,43 @@ def paged_attention(q: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor,
     keys: the host's bound on lengths[b] + counts[b] (None: what a row of `pages` holds), which sizes the launch; a
     sequence past it comes out NaN. workspace: from paged_attn_workspace (None: allocated for the call). A row's bits
     depend on its own sequence and position alone: not on the batch, T, the page size or the pages' places."""
-    _req(q.is_cuda and q.dtype == BF16 and q.dim() == 3 and q.is_contiguous() and q.numel() > 0,
-         "q must be contiguous bf16 [B*T, Hq, D] on the GPU")
-    kv, b = _paged_kv(q, lengths, counts, pages, k_pages, vt_pages)
-    rows, hq, d = q.shape
-    _req(d == kv.head_dim, f"pages of {kv.head_dim}-dim heads, q has {d}")
-    _req(rows % b == 0, f"{rows} rows do not divide into {b} sequences")
+    if not (q.is_cuda and q.dtype == BF16 and q.dim() == 3 and q.is_contiguous() and q.numel() > 0):
+        raise ValueError("q must be contiguous bf16 [B*T, Hq, D] on the GPU")
     dev = q.get_device()
+    kv, b = _paged_kv(dev, lengths, counts, pages, k_pages, vt_pages)
+    rows, hq, d = q.shape
+    if d != kv.head_dim:
+        raise ValueError(f"pages of {kv.head_dim}-dim heads, q has {d}")
+    if rows % b:
+        raise ValueError(f"{rows} rows do not divide into {b} sequences")
+    gate_row = gate_head = 0
     if gate is not None:
-        _req(gate.dtype == BF16 and gate.shape == q.shape and gate.stride(2) == 1 and gate.stride(1) < 2 ** 31
-             and gate.get_device() == dev, f"gate must be bf16 [{rows}, {hq}, {d}] with contiguous dims")
+        if not (gate.dtype == BF16 and gate.shape == (rows, hq, d) and gate.get_device() == dev and gate.stride(2) == 1
+                and gate.stride(1) < 2 ** 31):
+            raise ValueError(f"gate must be bf16 [{rows}, {hq}, {d}] with contiguous dims")
+        gate_row, gate_head, _ = gate.stride()
     room = kv.max_pages * kv.page
-    keys = room if keys is None else keys
-    _req(1 <= keys <= room, f"keys={keys}: a row of pages holds {room}")
-    _req(out is None or (out.dtype == BF16 and tuple(out.shape) == (rows, hq * d) and out.is_contiguous()
-                         and out.get_device() == dev), f"out must be contiguous bf16 [{rows}, {hq * d}]")
-    _req(workspace is None or (workspace.is_contiguous() and workspace.get_device() == dev),
-         "workspace must be contiguous, on q's device")
+    if keys is None:
+        keys = room
+    elif not 1 <= keys <= room:
+        raise ValueError(f"keys={keys}: a row of pages holds {room}")
+    if out is not None and not _fits(out, BF16, (rows, hq * d), dev):
+        raise ValueError(f"out must be contiguous bf16 [{rows}, {hq * d}]")
+    if workspace is not None and not (workspace.is_contiguous() and workspace.get_device() == dev):
+        raise ValueError("workspace must be contiguous, on q's device")
     with _on_device(q):
         L = _lib.lib()
-        if workspace is None:
-            n = int(L.skinny_paged_attn_workspace_bytes(b, rows // b, hq, kv.n_kv, d, keys))
-            workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        o = torch.empty((rows, hq * d), dtype=BF16, device=q.device) if out is None else out
+        nbytes = 0
+        if workspace is not None:
+            nbytes = workspace.numel() * workspace.element_size()
+        else:
+            nbytes = L.skinny_paged_attn_workspace_bytes(b, rows // b, hq, kv.n_kv, d, keys)
+            if nbytes:
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        o = q.new_empty((rows, hq * d)) if out is None else out
         _lib.check(L.skinny_paged_attention_bf16(
-            q.data_ptr(), b, rows // b, hq, kv, keys, scale, _lib.ptr(gate),
-            0 if gate is None else gate.stride(0), 0 if gate is None else gate.stride(1), _lib.ptr(workspace),
-            0 if workspace is None else workspace.numel() * workspace.element_size(), o.data_ptr(), _lib.stream_of(q)),
-            "paged_attention")
+            q.data_ptr(), b, rows // b, hq, kv, keys, scale, _lib.ptr(gate), gate_row, gate_head, _lib.ptr(workspace), nbytes,
+            o.data_ptr(), _lib.stream_of(q)), "paged_attention")
     return o
 
 
@@ -753,21 +774,25 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     _bf16_2d(logits, "logits")
     rows, V = logits.shape
     dev = logits.get_device()
-    _req(tokens.dtype == torch.int32 and tuple(tokens.shape) == (rows,) and tokens.is_contiguous()
-         and tokens.get_device() == dev, f"tokens must be contiguous int32 [{rows}] on the logits' device")
-    _req(temperature > 0, f"temperature={temperature} must be positive")
-    _req(0 <= top <= max(V, 1), f"top={top} of {V} scores")
-    _req(rows <= 1 or V <= logits.stride(0), "rows overlap")
+    if not _fits(tokens, torch.int32, (rows,), dev):
+        raise ValueError(f"tokens must be contiguous int32 [{rows}] on the logits' device")
+    if not temperature > 0:
+        raise ValueError(f"temperature={temperature} must be positive")
+    if not 0 <= top <= max(V, 1):
+        raise ValueError(f"top={top} of {V} scores")
+    ld = V if rows <= 1 else logits.stride(0)
+    if V > ld:
+        raise ValueError("rows overlap")
     with _on_device(logits):
         L = _lib.lib()
-        num = torch.empty((2, rows), dtype=torch.float32, device=logits.device)
-        ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
-        alt = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-        if rows == 0:
-            return num[0], num[1], ids, alt
-        ws = torch.empty(int(L.skinny_token_logprobs_workspace_bytes(rows, V, top)), dtype=torch.uint8, device=logits.device)
-        _lib.check(L.skinny_token_logprobs_bf16(
-            logits.data_ptr(), rows, V, V if rows == 1 else logits.stride(0), tokens.data_ptr(), 1.0 / temperature, top,
-            ws.data_ptr(), ws.numel(), num[0].data_ptr(), num[1].data_ptr(), ids.data_ptr(), alt.data_ptr(),
-            _lib.stream_of(logits)), "token_logprobs")
-    return num[0], num[1], ids, alt
+        lp = logits.new_empty(rows, dtype=torch.float32)
+        ent = logits.new_empty(rows, dtype=torch.float32)
+        ids = tokens.new_empty((rows, top))
+        alt = logits.new_empty((rows, top), dtype=torch.float32)
+        if rows:
+            nbytes = L.skinny_token_logprobs_workspace_bytes(rows, V, top)
+            ws = tokens.new_empty(nbytes // 4)
+            _lib.check(L.skinny_token_logprobs_bf16(
+                logits.data_ptr(), rows, V, ld, tokens.data_ptr(), 1.0 / temperature, top, ws.data_ptr(), nbytes,
+                lp.data_ptr(), ent.data_ptr(), ids.data_ptr(), alt.data_ptr(), _lib.stream_of(logits)), "token_logprobs")
+    return lp, ent, ids, alt
