@@ -48,78 +48,172 @@ __device__ __forceinline__ Sequence sequence_of(const Pages& pg, int b, int T, i
 
 constexpr uint16_t kNanBits = 0x7fc0;
 
-// ---------------------------------------------------------------------------------------------------------
-// New rows into the cache.
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
+}
 
-// One wave per (head, token, sequence): heads [0, Hq) are queries, then Hkv keys, then Hkv values. Lane l holds dims
-// l + 64e. fp32 from the row to the result, rounded once.
+// ---------------------------------------------------------------------------------------------------------
+// New rows into the cache. A wave takes 64 / (D / 8) query or key heads of a token, eight dims a lane; or 64 value dims of
+// the tokens of 16 slots, a dim per lane, which it turns over in registers, so that they go out in 16-byte pieces. Bound by
+// latency for few tokens and by memory for many.
+
+// Eight bf16 at any even address.
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(8)));
+
+struct StoreRows {
+  const uint16_t* qkv;
+  int ldq, qs, koff, voff;
+  const uint16_t *qn, *kn;  // null: no norm
+};
+
 template <int D>
-__global__ __launch_bounds__(64) void paged_store_kernel(Pages pg, const uint16_t* __restrict__ qkv, int ldq, int T,
-                                                         int Hq, int Hkv, int qs, int koff, int voff,
-                                                         const uint16_t* __restrict__ qn, const uint16_t* __restrict__ kn,
-                                                         float eps, int R, const float* __restrict__ rope, int room,
-                                                         uint16_t* __restrict__ q_out) {
-  constexpr int E = D / 64;
-  __shared__ float row[D];
-  const int head = blockIdx.x, t = blockIdx.y, b = blockIdx.z, lane = threadIdx.x;
-  const Sequence sq = sequence_of(pg, b, T, room);
+__device__ __forceinline__ void store_heads(const Pages& pg, const StoreRows& rows, int T, int Hq, int Hkv, float eps, int R,
+                                            const float* __restrict__ rope, int room, uint16_t* __restrict__ q_out, int unit,
+                                            float* __restrict__ lds) {
+  constexpr int LPH = D / 8, HPW = 64 / LPH;
+  const int lane = threadIdx.x & 63, t = blockIdx.y, b = blockIdx.z;
+  const int head = unit * HPW + lane / LPH, d0 = lane % LPH * 8;
+  const bool there = head < Hq + Hkv;
   const size_t r = (size_t)b * T + t;
-  uint16_t* qd = q_out + (r * Hq + head) * D;
+  const bool query = head < Hq;
+  u32x4_t x4 = {0, 0, 0, 0}, w4 = {0, 0, 0, 0};
+  const uint16_t* norm = query ? rows.qn : rows.kn;
+  if (there) {
+    x4 = *reinterpret_cast<const u32x4_any_t*>(rows.qkv + r * rows.ldq + (query ? head * (size_t)rows.qs : rows.koff + (size_t)(head - Hq) * D) + d0);
+    if (norm) w4 = *reinterpret_cast<const u32x4_any_t*>(norm + d0);
+  }
+  const Sequence sq = sequence_of(pg, b, T, room);
   const bool live = sq.ok && t < sq.count;
   const int pos = live ? sq.len + t : 0;
-  const int P = 1 << pg.log2p;
-  int page = -1;
-  if (live) page = pg.table[(size_t)b * pg.ld + (pos >> pg.log2p)];
-  const bool placed = (unsigned)page < (unsigned)pg.n_pages;
-  if (!live || !placed) {
-    if (head < Hq) {
-      const uint16_t fill = sq.ok && t >= sq.count ? 0 : kNanBits;
-#pragma unroll
-      for (int e = 0; e < E; ++e) qd[lane + 64 * e] = fill;
-    }
+  const int page = live ? words(pg.table)[(size_t)b * pg.ld + (pos >> pg.log2p)] : -1;
+  u32x4_t* qd = reinterpret_cast<u32x4_t*>(q_out + (r * Hq + head) * D + d0);
+  if ((unsigned)page >= (unsigned)pg.n_pages) {  // no token, or nowhere to put it
+    const uint32_t fill = sq.ok && t >= sq.count ? 0u : kNanBits * 0x10001u;
+    if (query) *qd = u32x4_t{fill, fill, fill, fill};
     return;
   }
-  const uint16_t* src = qkv + r * ldq;
-  if (head < Hq) src += (size_t)head * qs;
-  else if (head < Hq + Hkv) src += koff + (head - Hq) * D;
-  else src += voff + (head - Hq - Hkv) * D;
-  const int slot = pos & (P - 1);
-  if (head >= Hq + Hkv) {
-    uint16_t* vd = pg.vt + (int64_t)page * (int64_t)pg.vt_stride + (size_t)(head - Hq - Hkv) * D * P + slot;
+  const int half = R >> 1;
+  const bool turns = d0 < R;
+  // the table's entries of these dims: pair i = d, or d - half
+  const float* cs = rope + ((size_t)pos * half) * 2;
+  const bool whole = half % 8 == 0;  // eight dims turn together, with the eight of one other lane
+  f32x4_t c4[4];
+  if (whole && turns)
 #pragma unroll
-    for (int e = 0; e < E; ++e) vd[(size_t)(lane + 64 * e) * P] = src[lane + 64 * e];
-    return;
-  }
-  float x[E];
-  float ss = 0.f;
+    for (int i = 0; i < 4; ++i)
+      c4[i] = *reinterpret_cast<const f32x4_any_t*>(cs + 2 * (d0 < half ? d0 : d0 - half) + 4 * i);
+  float x[8], ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    x[e] = bf16_bits_to_f32(src[lane + 64 * e]);
+  for (int e = 0; e < 8; ++e) {
+    x[e] = bf16_bits_to_f32(e & 1 ? x4[e >> 1] >> 16 : x4[e >> 1] & 0xffffu);
     ss = fmaf(x[e], x[e], ss);
   }
-  const uint16_t* nw = head < Hq ? qn : kn;
-  if (nw) {
-    const float inv = rsqrtf(wave_sum(ss) / (float)D + eps);
+  if (rows.qn || rows.kn) {
+    ss = dpp_add<0xB1>(ss);
+    ss = dpp_add<0x4E>(ss);
+    ss = dpp_add<0x141>(ss);
+    if (LPH >= 16) ss = dpp_add<0x140>(ss);
+    if (LPH >= 32) ss += __shfl_xor(ss, 16, 64);
+    const float inv = rsqrtf(ss / (float)D + eps);
+    if (norm)
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] *= inv * bf16_bits_to_f32(nw[lane + 64 * e]);
+      for (int e = 0; e < 8; ++e) x[e] *= inv * bf16_bits_to_f32(e & 1 ? w4[e >> 1] >> 16 : w4[e >> 1] & 0xffffu);
   }
+  // The pairs' other halves through LDS: [head][D], this wave's own.
+  float* mine = lds + lane / LPH * D;
 #pragma unroll
-  for (int e = 0; e < E; ++e) row[lane + 64 * e] = x[e];
-  __syncthreads();
-  const int half = R >> 1;
-  uint16_t* dst = head < Hq ? qd : pg.k + (int64_t)page * (int64_t)pg.k_stride + ((size_t)(head - Hq) * P + slot) * D;
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<f32x4_t*>(mine + d0 + 4 * i) = f32x4_t{x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  if (whole) {
+    if (turns) {
+      const float sign = d0 < half ? -1.f : 1.f;
+      const float* other = mine + (d0 < half ? d0 + half : d0 - half);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int d = lane + 64 * e;
-    float y = x[e];
-    if (d < R) {
-      const int i = d < half ? d : d - half;
-      const float2 cs = reinterpret_cast<const float2*>(rope)[(size_t)pos * half + i];
-      const float a = row[i], c = row[i + half];
-      y = d < half ? a * cs.x - c * cs.y : c * cs.x + a * cs.y;
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * c4[e >> 1][2 * (e & 1)] + sign * other[e] * c4[e >> 1][2 * (e & 1) + 1];
     }
-    dst[d] = f32_to_bf16_bits(y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = d0 + e;
+      if (d < R) {
+        const int i = d < half ? d : d - half;
+        const float other = mine[d < half ? d + half : d - half];
+        x[e] = x[e] * cs[2 * i] + (d < half ? -other : other) * cs[2 * i + 1];
+      }
+    }
   }
+  u32x4_t y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = two_bf16(x[2 * i], x[2 * i + 1]);
+  if (!there) return;
+  const int slot = pos & ((1 << pg.log2p) - 1);
+  if (query) *qd = y;
+  else
+    *reinterpret_cast<u32x4_t*>(pg.k + (int64_t)page * (int64_t)pg.k_stride +
+                                (((size_t)(head - Hq) << pg.log2p) + slot) * D + d0) = y;
+}
+
+// 64 dims from `dim` on, of the value rows' Hkv * D, of the tokens in a granule's 16 slots: a dim per lane.
+template <int D>
+__device__ __forceinline__ void store_values(const Pages& pg, const StoreRows& rows, int T, int Hkv, int room, int dim) {
+  const int lane = threadIdx.x & 63, b = blockIdx.z;
+  if (dim >= Hkv * D) return;
+  const Sequence sq = sequence_of(pg, b, T, room);
+  if (!sq.ok || sq.count == 0) return;
+  const int p0 = ((sq.len >> 4) + (int)blockIdx.y) << 4;  // the granule's first position
+  if (p0 >= sq.len + sq.count) return;
+  const int page = words(pg.table)[(size_t)b * pg.ld + (p0 >> pg.log2p)];
+  if ((unsigned)page >= (unsigned)pg.n_pages) return;
+  const int s0 = max(sq.len - p0, 0), s1 = min(sq.len + sq.count - p0, 16);  // its slots that are written
+  const uint16_t* src = rows.qkv + ((int64_t)b * T + (p0 - sq.len)) * rows.ldq + rows.voff + dim + lane;
+  const int P = 1 << pg.log2p;
+  uint16_t* dst = pg.vt + (int64_t)page * (int64_t)pg.vt_stride + (size_t)(dim + lane) * P + (p0 & (P - 1));
+  if (s1 - s0 == 1) {
+    dst[s0] = src[(int64_t)s0 * rows.ldq];
+    return;
+  }
+  // Pieces of eight slots, with what a piece's other slots hold: stores of single values wait for each other where they
+  // meet in a line (8 tokens of 16 sequences, 4 heads of 256 dims: 11 us so).
+  u32x4_t old[2];
+  uint32_t v[16];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    old[i] = u32x4_t{0, 0, 0, 0};
+    if (s0 < 8 * i + 8 && s1 > 8 * i && (s0 > 8 * i || s1 < 8 * i + 8)) old[i] = *reinterpret_cast<const u32x4_t*>(dst + 8 * i);
+  }
+#pragma unroll
+  for (int s = 0; s < 16; ++s) v[s] = src[(int64_t)min(max(s, s0), s1 - 1) * rows.ldq];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (s0 >= 8 * i + 8 || s1 <= 8 * i) continue;
+    u32x4_t w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int s = 8 * i + 2 * k;
+      const uint32_t lo = s < s0 || s >= s1 ? old[i][k] & 0xffffu : v[s];
+      const uint32_t hi = s + 1 < s0 || s + 1 >= s1 ? old[i][k] >> 16 : v[s + 1];
+      w[k] = lo | hi << 16;
+    }
+    *reinterpret_cast<u32x4_t*>(dst + 8 * i) = w;
+  }
+}
+
+// Grid (workgroups of four head units, then of 256 value dims; tokens; sequences): a value workgroup's second index
+// counts the granules.
+template <int D>
+__global__ __launch_bounds__(256) void paged_store_kernel(Pages pg, StoreRows rows, int T, int Hq, int Hkv, float eps, int R,
+                                                          const float* __restrict__ rope, int room, int head_groups,
+                                                          uint16_t* __restrict__ q_out) {
+  __shared__ __attribute__((aligned(16))) float lds[4][512];
+  const int wave = wave_id();
+  if ((int)blockIdx.x < head_groups)
+    store_heads<D>(pg, rows, T, Hq, Hkv, eps, R, rope, room, q_out, (int)blockIdx.x * 4 + wave, lds[wave]);
+  else
+    store_values<D>(pg, rows, T, Hkv, room, (((int)blockIdx.x - head_groups) * 4 + wave) * 64);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -183,12 +277,6 @@ __device__ __forceinline__ float quads_sum(float v) {
   v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 
 // W tiles of 16 query rows; a call of more rows per kv head than 32 (`halves` 1) takes two workgroups a run, the second
@@ -750,11 +838,12 @@ extern "C" int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int 
   SKINNY_CHECK_ARG(skinny_aligned(qkv, 2) && skinny_aligned(rope_table, 8) && skinny_aligned(q_out, 16) &&
                        skinny_aligned(q_norm, 2) && skinny_aligned(k_norm, 2),
                    "paged_store: misaligned buffer");
-  const dim3 grid(Hq + 2 * Hkv, T, B);
+  const int heads = 64 / (D / 8) * 4, groups = (Hq + Hkv + heads - 1) / heads;  // query and key heads of a workgroup
+  const StoreRows rows{qkv, ldq, q_stride, k_offset, v_offset, q_norm, k_norm};
   const hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(64), 0, s, pg, qkv, ldq, T, Hq, Hkv, q_stride, k_offset, v_offset, q_norm, k_norm,
-                       eps, rotary_dim, rope_table, room, q_out);
+    hipLaunchKernelGGL(kernel, dim3(groups + (Hkv * (D / 64) + 3) / 4, T, B), dim3(256), 0, s, pg, rows, T, Hq, Hkv, eps, rotary_dim,
+                       rope_table, room, groups, q_out);
   };
   if (D == 64) go(paged_store_kernel<64>);
   else if (D == 128) go(paged_store_kernel<128>);
