@@ -9,9 +9,11 @@
 // (every term of W is positive, so nothing cancels). Alternatives are the largest scores, ties by the lower index.
 //
 // A row is cut into slices of 8192 scores at fixed places. A workgroup holds a slice in registers, so that it is read
-// once: its maximum, its sums, and its largest scores, which are picked out by a bound that `top` of them reach; a wave
-// per row joins the slices in order. Many rows are bound by memory and the vector units alike: a score costs about ten
-// instructions, one of them an exponential at a quarter of the rate.
+// once: its maximum, its sums, and its candidates, the scores that reach a bound which `top` of them are known to reach; a
+// workgroup per row joins the slices, sums in order and keys by the same kind of bound. Few rows are bound by the two
+// launches' latency. Many are bound by memory and the vector units alike (a score costs some ten instructions, an
+// exponential at a quarter of the rate among them): 1021 rows of 151936 scores in 58 us, 5.4 TB/s, without alternatives,
+// 81 with 5, 93 with 32. Loads for the next slice kept in flight took registers that the other waves need: 69 and 97 us.
 #include "common.h"
 
 namespace {
@@ -38,9 +40,13 @@ __device__ __forceinline__ float value_of(uint32_t order) {
   return bf16_bits_to_f32((order & 0x8000u) ? (order & 0x7fffu) : (~order & 0xffffu));
 }
 
-// Workspace: per (row, slice) the maximum, Z and W, then `top` keys (order << 16 | 0xffff - index in the slice),
-// decreasing, 0 where the slice has fewer scores.
-__host__ __device__ constexpr int part_words(int top) { return 4 + top; }
+// Workspace: per (row, slice) the maximum, Z, W, a word of nothing, then keys (order << 16 | 0xffff - index in the slice) in
+// any order, the slice's `top` largest among them, and zeros.
+__host__ __device__ constexpr int part_keys(int top) { return top ? 2 * top + 8 : 0; }
+__host__ __device__ constexpr int part_words(int top) { return 4 + part_keys(top); }
+
+// The lanes for which a condition holds, straight from its compare.
+__device__ __forceinline__ uint64_t ballot(bool b) { return __builtin_amdgcn_ballot_w64(b); }
 
 // The largest value over the wave, in every lane.
 template <int kCtrl>
@@ -58,6 +64,22 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return max(b[0], b[1]);
 }
 
+// The largest value that `need` lanes reach (0: not so many have one), their largest being `largest`.
+__device__ __forceinline__ uint32_t reached_by(uint32_t v, uint32_t largest, int need) {
+  if (need <= 4) {  // from the top
+    uint32_t least = largest;
+    while (least && __popcll(ballot(v >= least)) < need) least = wave_max(v < least ? v : 0u);
+    return least;
+  }
+  uint32_t least = 0;  // bit by bit
+#pragma unroll
+  for (int bit = 15; bit >= 0; --bit) {
+    const uint32_t next = least | 1u << bit;
+    least = __popcll(ballot(v >= next)) >= need ? next : least;
+  }
+  return least;
+}
+
 constexpr int kWaves = kThreads / 64;
 constexpr int kList = 64;  // candidates that a wave may have; a slice with more (many equal scores) goes the long way
 constexpr uint32_t kNegInf = 0x7fu;  // order_of(-inf)
@@ -72,54 +94,59 @@ __global__ __launch_bounds__(kThreads) void logprobs_slice_kernel(const uint16_t
   const uint16_t* row = logits + (int64_t)r * ld;
   const int base = slice * kSlice, n = min(kSlice, V - base);
   const uint16_t* src = row + base;
-  float x[kPieces][8];
+  u32x4_t raw[kPieces];
+  if (n == kSlice) {
 #pragma unroll
-  for (int j = 0; j < kPieces; ++j) {
-    const int e0 = 8 * (threadIdx.x + j * kThreads);
-    u32x4_t w;
-    if (e0 + 8 <= n) {
-      w = *reinterpret_cast<const u32x4_any_t*>(src + e0);
-    } else {  // the row's last scores; what is past them is -inf, which adds nothing
+    for (int j = 0; j < kPieces; ++j) raw[j] = *reinterpret_cast<const u32x4_any_t*>(src + 8 * (threadIdx.x + j * kThreads));
+  } else {  // the row's last slice: what is past it is -inf, which adds nothing
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int e = e0 + 2 * i;
-        w[i] = (e < n ? src[e] : 0xff80u) | (e + 1 < n ? (uint32_t)src[e + 1] << 16 : 0xff800000u);
+    for (int j = 0; j < kPieces; ++j) {
+      const int e0 = 8 * (threadIdx.x + j * kThreads);
+      raw[j] = u32x4_t{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+      if (e0 + 8 <= n) {
+        raw[j] = *reinterpret_cast<const u32x4_any_t*>(src + e0);
+      } else if (e0 < n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = e0 + 2 * i;
+          raw[j][i] = (e < n ? src[e] : 0xff80u) | (e + 1 < n ? (uint32_t)src[e + 1] << 16 : 0xff800000u);
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[j][2 * i] = __uint_as_float(w[i] << 16);
-      x[j][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
   }
-  float m = -INFINITY;
+  float x[kPieces][8];
 #pragma unroll
   for (int j = 0; j < kPieces; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, x[j][e]);
-  // The slice's maximum, and a value that at least `top` of its scores reach: the largest for which that many threads of
-  // some wave have one.
-  const uint32_t mine = order_of(__float_as_uint(m) >> 16);
-  uint32_t least = 0;
-  if (top) {
-#pragma unroll
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t next = least | 1u << bit;
-      least = __popcll(__ballot(mine >= next)) >= top ? next : least;
+    for (int i = 0; i < 4; ++i) {
+      x[j][2 * i] = __uint_as_float(raw[j][i] << 16);
+      x[j][2 * i + 1] = __uint_as_float(raw[j][i] & 0xffff0000u);
     }
+  float m = -INFINITY, most[kPieces];
+#pragma unroll
+  for (int j = 0; j < kPieces; ++j) {
+    most[j] = x[j][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) most[j] = fmaxf(most[j], x[j][e]);
+    m = fmaxf(m, most[j]);
   }
+  // The slice's maximum, and a value that at least `top` of its scores reach, from the threads' maxima: every wave has
+  // ceil(top / 4) that reach the least of the waves' values for that count; for one or two, the greatest of the waves'
+  // values for the whole count lies nearer.
+  const uint32_t mine = order_of(__float_as_uint(m) >> 16);
+  const int need = top <= 2 ? top : (top + kWaves - 1) / kWaves;
   const uint32_t largest = wave_max(mine);
+  const uint32_t least0 = top ? reached_by(mine, largest, need) : 0u;
   if (lane == 0) {
     red[0][wave] = largest;
-    red[1][wave] = least;
+    red[1][wave] = least0;
   }
   __syncthreads();
-  uint32_t om = red[0][0];
-  least = red[1][0];
+  uint32_t om = red[0][0], least = red[1][0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) {
     om = max(om, red[0][w]);
-    least = max(least, red[1][w]);
+    least = top <= 2 ? max(least, red[1][w]) : min(least, red[1][w]);
   }
   m = value_of(om);
   const float mref = om <= kNegInf ? 0.f : m, c = inv_temp * kLog2e;
@@ -141,10 +168,11 @@ __global__ __launch_bounds__(kThreads) void logprobs_slice_kernel(const uint16_t
   int found = 0;
   if (top && least > kNegInf) {
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j)
+    for (int j = 0; j < kPieces; ++j) {
+      if (!ballot(most[j] >= bound)) continue;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint64_t who = __ballot(x[j][e] >= bound);
+        const uint64_t who = ballot(x[j][e] >= bound);
         if (who) {
           const int at = found + __popcll(who & ((1ull << lane) - 1));
           if ((who >> lane & 1) && at < kList)
@@ -152,6 +180,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_slice_kernel(const uint16_t
           found += __popcll(who);
         }
       }
+    }
     if (lane < 4) list[wave][min(found, kList) + lane] = 0;  // to a whole piece
   }
   if (lane == 0) {
@@ -172,14 +201,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_slice_kernel(const uint16_t
     part[2] = __float_as_uint(-st);
   }
   if (!top) return;
-  int all = 0;
+  int all = 0, before = 0;
   bool fits = true;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) {
+    before += w < wave ? (int)count[w] : 0;
     all += count[w];
     fits &= count[w] <= kList;
   }
-  if (fits && all >= top) {
+  fits &= all >= top;
+  const bool listed = fits && all <= part_keys(top);
+  for (int i = (listed ? all : top) + threadIdx.x; i < part_keys(top); i += kThreads) part[4 + i] = 0;
+  if (listed) {
+    if (lane < (int)count[wave]) part[4 + before + lane] = list[wave][lane];
+    return;
+  }
+  if (fits) {
     // Keys are all different: a candidate's place is the number of those above it.
     if (lane >= (int)count[wave]) return;
     const uint32_t key = list[wave][lane];
@@ -216,23 +253,47 @@ __global__ __launch_bounds__(kThreads) void logprobs_slice_kernel(const uint16_t
   }
 }
 
-// One wave per row; lane j holds slice j.
-__global__ __launch_bounds__(64) void logprobs_join_kernel(const uint16_t* __restrict__ logits, int64_t ld, int V,
-                                                           const int32_t* __restrict__ tokens, float inv_temp, int top,
-                                                           int slices, const uint32_t* __restrict__ parts,
-                                                           float* __restrict__ logprob, float* __restrict__ entropy,
-                                                           int32_t* __restrict__ ids, float* __restrict__ top_logprob) {
-  __shared__ uint32_t keys[kMaxSlices * kMaxTop];
-  const int lane = threadIdx.x;
+// One workgroup per row. Lane j of each wave holds slice j's sums; the slices' keys are spread over the threads, and the
+// row's largest are found as a slice's are: by a bound from the threads' maxima, then by counting those above.
+constexpr int kJoinKeys = kMaxSlices * part_keys(kMaxTop);
+constexpr int kJoinList = 512;
+
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const uint16_t* __restrict__ logits, int64_t ld, int V,
+                                                                 const int32_t* __restrict__ tokens, float inv_temp, int top,
+                                                                 int slices, const uint32_t* __restrict__ parts,
+                                                                 float* __restrict__ logprob, float* __restrict__ entropy,
+                                                                 int32_t* __restrict__ ids, float* __restrict__ top_logprob) {
+  __shared__ uint32_t keys[kJoinKeys], red[kWaves], count;
+  __shared__ __attribute__((aligned(16))) uint64_t list[kJoinList + 1];
+  const int lane = threadIdx.x & 63, wave = wave_id();
   const size_t r = blockIdx.x;
-  const uint32_t* rows = parts + r * slices * part_words(top);
-  const uint32_t* mine = rows + min(lane, slices - 1) * part_words(top);
+  const int words = part_words(top), per = part_keys(top);
+  const uint32_t* rows = parts + r * slices * words;
+  const uint32_t* mine = rows + min(lane, slices - 1) * words;
   const bool have = lane < slices;
   const int token = tokens[r];
   const float x = token >= 0 && token < V ? bf16_bits_to_f32(logits[(int64_t)r * ld + token]) : -INFINITY;
   const float ms = have ? __uint_as_float(mine[0]) : -INFINITY;
   float z = have ? __uint_as_float(mine[1]) : 0.f, w = have ? __uint_as_float(mine[2]) : 0.f;
-  for (int i = lane; i < slices * top; i += 64) keys[i] = rows[i / top * part_words(top) + 4 + i % top];
+  // A thread's keys: number i of the row is number i % per of slice i / per.
+  const int total = slices * per;
+  uint32_t best = 0;
+  if (top) {
+    if (threadIdx.x == 0) count = 0;
+    const int ds = kThreads / per, dq = kThreads % per;
+    int s = threadIdx.x / per, q = threadIdx.x % per;
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      const uint32_t key = rows[s * words + 4 + q];
+      keys[i] = key;
+      best = max(best, key >> 16);
+      s += ds;
+      q += dq;
+      if (q >= per) {
+        q -= per;
+        ++s;
+      }
+    }
+  }
   float m = ms;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -241,22 +302,64 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const uint16_t* __res
   z = wave_sum(ms == -INFINITY ? z : z * f);
   w = wave_sum(f == 0.f ? 0.f : w * f);
   const float ln_z = logf(z);
-  if (lane == 0) {
+  if (threadIdx.x == 0) {
     logprob[r] = (x - m) * inv_temp - ln_z;
     entropy[r] = ln_z + w / z * inv_temp;
   }
-  // The slices' keys are in order: the next of the row is at the head of one of them.
-  lds_barrier();
-  int head = 0;
-  for (int k = 0; k < top; ++k) {
-    const uint32_t key = have && head < top ? keys[lane * top + head] : 0u;
-    const uint32_t order = wave_max(key >> 16);
-    const uint64_t who = __ballot(key != 0u && (key >> 16) == order);  // the first slice has the lower indices
-    if (lane == __ffsll((unsigned long long)who) - 1) {
-      ids[r * top + k] = lane * kSlice + (int)(0xffffu - (key & 0xffffu));
-      top_logprob[r * top + k] = (value_of(order) - m) * inv_temp - ln_z;
-      ++head;
+  if (!top) return;
+  const int need = top <= 2 ? top : (top + kWaves - 1) / kWaves;
+  uint32_t least = reached_by(best, wave_max(best), need);
+  if (lane == 0) red[wave] = least;
+  __syncthreads();
+  least = red[0];
+#pragma unroll
+  for (int v = 1; v < kWaves; ++v) least = top <= 2 ? max(least, red[v]) : min(least, red[v]);
+  // A key of the row orders by its score, then by the lower index.
+  auto whole = [&](int i) {
+    const uint32_t key = keys[i];
+    return (uint64_t)(key >> 16) << 32 | (0xffffffffu - (i / per * kSlice + (0xffffu - (key & 0xffffu))));
+  };
+  auto put = [&](int place, uint64_t k) {
+    ids[r * top + place] = (int)(0xffffffffu - (uint32_t)k);
+    top_logprob[r * top + place] = (value_of((uint32_t)(k >> 32)) - m) * inv_temp - ln_z;
+  };
+  if (best >= max(least, 1u))
+    for (int i = threadIdx.x; i < total; i += kThreads)
+      if (keys[i] >> 16 >= max(least, 1u)) {
+        const uint32_t at = atomicAdd(&count, 1u);
+        if (at < kJoinList) list[at] = whole(i);
+      }
+  __syncthreads();
+  const int n = count;
+  if (n <= kJoinList) {
+    for (int c = threadIdx.x; c < n; c += kThreads) {
+      const uint64_t k = list[c];
+      int place = 0;
+      for (int i = 0; i < n; ++i) place += list[i] > k ? 1 : 0;
+      if (place < top) put(place, k);
     }
+    return;
+  }
+  // Very many equal scores: one after the other.
+  uint64_t prev = ~0ull;
+  for (int k = 0; k < top; ++k) {
+    uint64_t next = 0;
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+      const uint64_t v = whole(i);
+      if (keys[i] && v < prev && v > next) next = v;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t v = __shfl_xor((unsigned long long)next, o, 64);
+      next = v > next ? v : next;
+    }
+    __syncthreads();
+    if (lane == 0) list[wave] = next;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) next = list[v] > next ? list[v] : next;
+    if (threadIdx.x == 0) put(k, next);
+    prev = next;
   }
 }
 
@@ -286,7 +389,7 @@ extern "C" int skinny_token_logprobs_bf16(const uint16_t* logits, int rows, int 
   uint32_t* parts = static_cast<uint32_t*>(workspace);
   hipLaunchKernelGGL(logprobs_slice_kernel, dim3(slices, rows), dim3(kThreads), 0, s, logits, V, ld, inv_temp, top, parts);
   if (const int rc = skinny_check_launch("token_logprobs")) return rc;
-  hipLaunchKernelGGL(logprobs_join_kernel, dim3(rows), dim3(64), 0, s, logits, ld, V, tokens, inv_temp, top, slices, parts,
+  hipLaunchKernelGGL(logprobs_join_kernel, dim3(rows), dim3(top ? kThreads : 64), 0, s, logits, ld, V, tokens, inv_temp, top, slices, parts,
                      logprob, entropy, ids, top_logprob);
   return skinny_check_launch("token_logprobs join");
 }
