@@ -17,7 +17,10 @@ namespace {
 
 constexpr float kPLog2e = 1.4426950408889634f;
 constexpr int kPMaxRows = 64;  // query rows per kv head: T x (Hq / Hkv)
-constexpr int kPBlock = 128;   // keys of a block
+
+// A block's keys, and the waves that share it: 64 KB of K and V for 128 and 256 dims, a wave's part of which is 64 registers.
+__host__ __device__ constexpr int paged_block(int D) { return D == 256 ? 64 : 128; }
+__host__ __device__ constexpr int paged_waves(int D) { return D == 64 ? 2 : 4; }
 constexpr int kPPair = 2;      // blocks joined left to right: what a workgroup takes at least
 constexpr int kPGroup = 8;     // blocks whose pairs are joined left to right, by the workgroup that takes them all or by the merge
 
@@ -217,9 +220,9 @@ __global__ __launch_bounds__(256) void paged_store_kernel(Pages pg, StoreRows ro
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Attention. A workgroup takes a run of blocks of 128 keys of one sequence and kv head, with a wave for every 32 dims.
-// In a block each wave scores its share of the keys (S^T = K Q^T, the K rows straight from memory into matrix-core
-// operands); the row maxima and then the weights P go through LDS, and each wave forms its 32 dims over all the block's
+// Attention. A workgroup takes a run of blocks of keys of one sequence and kv head. In a block each wave scores its share
+// of the keys (S^T = K Q^T, the K rows straight from memory into matrix-core
+// operands); the row maxima and then the weights P go through LDS, and each wave forms its share of the dims over all the block's
 // keys (O^T = V^T P^T). So K and V are read once, by one wave each, and no output is summed across waves. As soon as a
 // block's scores (outputs) are formed, its K (V) registers take the next block's loads, which are in flight through the
 // rest of the block.
@@ -280,33 +283,37 @@ __device__ __forceinline__ float quads_sum(float v) {
 }
 
 // W tiles of 16 query rows; a call of more rows per kv head than 32 (`halves` 1) takes two workgroups a run, the second
-// of which finds K and V in the caches. GS: keys of a block that share a page: the page size where that is 16 or 32, else 64.
+// of which finds K and V in the caches. by_g: 65536 / G rounded up, G = Hq / Hkv. GS: keys of a block that share a page: the page size where that is 16 or 32, else 64.
 template <int D, int W, int GS>
-__global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T, int Hq,
+__global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T, int G, int by_g, int Hq,
                                                                int Hkv, int room, float scale, int span, int slots, int halves,
                                                                float* __restrict__ part_o, float* __restrict__ part_ml,
                                                                Out o) {
-  constexpr int WAVES = D / 32, KT = 8 / WAVES, KS = D / 32;  // a wave's 16-key tiles; dim steps of a score
-  constexpr int ST = kPBlock / 32, NG = kPBlock / GS;         // a block's 32-key steps and pages
+  constexpr int BLK = paged_block(D), WAVES = paged_waves(D);
+  constexpr int KT = BLK / 16 / WAVES, KS = D / 32;           // a wave's 16-key tiles; dim steps of a score
+  constexpr int ST = BLK / 32, NG = BLK / GS;                 // a block's 32-key steps and pages
   constexpr int KG = KT * 16 > GS ? KT * 16 / GS : 1;         // pages of a wave's keys
-  constexpr int DW = 2;                                       // a wave's 16-dim tiles
-  constexpr int QP = D + 8;
+  constexpr int DW = D / 16 / WAVES;                          // a wave's 16-dim tiles
+  constexpr bool kKept = W == 1 && D != 256;                  // the queries stay in registers
+  constexpr int QP = D + 8;                                   // else their pitch in LDS
   __shared__ u32x4_t p_lds[W][2][ST][64];
   __shared__ __attribute__((aligned(16))) float m_lds[W * 16][WAVES], l_lds[W * 16][WAVES];
-  __shared__ __attribute__((aligned(16))) uint16_t q_lds[W == 1 ? 8 : W * 16 * QP];
+  __shared__ __attribute__((aligned(16))) uint16_t q_lds[kKept ? 8 : W * 16 * QP];
   const int h = blockIdx.y >> halves, b = blockIdx.z;
   const int row0 = blockIdx.y & halves ? 16 * W : 0;  // of the rows per kv head
-  const int G = Hq / Hkv, lane = threadIdx.x & 63, wave = wave_id();
+  const int lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quad = lane >> 4;
   const int c0 = blockIdx.x * span;
   // The queries, the first block's pages and the lengths are asked for at once.
-  constexpr int QN = W == 1 ? KS : (W * 16 * (D / 8) + 2 * D - 1) / (2 * D);
-  auto q_row = [&](int r) { return q + (((size_t)b * T + r / G) * Hq + h * G + r % G) * D; };
+  constexpr int QN = kKept ? KS : (W * 16 * (D / 8) + 64 * WAVES - 1) / (64 * WAVES);
+  auto token = [&](int r) { return r * by_g >> 16; };  // of row r, which is head r - token * G
+  auto q_row = [&](int r) { return q + (uint32_t)((token(r) * (Hq - G) + r) * D); };
+  q += ((size_t)b * T * Hq + (size_t)h * G) * D;
   u32x4_t qr[QN];
 #pragma unroll
   for (int i = 0; i < QN; ++i) {
-    const int e = threadIdx.x + i * 2 * D;
-    const int r = W == 1 ? col : e / (D / 8), d = W == 1 ? i * 32 + quad * 8 : e % (D / 8) * 8;
+    const int e = threadIdx.x + i * 64 * WAVES;
+    const int r = kKept ? col : e / (D / 8), d = kKept ? i * 32 + quad * 8 : e % (D / 8) * 8;
     qr[i] = *reinterpret_cast<const u32x4_t*>(q_row(min(row0 + r, T * G - 1)) + d);
   }
   // A block's pages (idk: those of the wave's own keys).
@@ -316,30 +323,30 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
   const int own = wave * (KT * 16) / GS;
   int ids[NG], idk[KG];
   auto find = [&](int c) {
-    if ((c + 1) * kPBlock <= pg.max_pages << log2p) {
+    if ((c + 1) * BLK <= pg.max_pages << log2p) {
 #pragma unroll
-      for (int g = 0; g < NG; ++g) ids[g] = GS < 64 ? table[c * NG + g] : table[(c * kPBlock + g * GS) >> log2p];
+      for (int g = 0; g < NG; ++g) ids[g] = GS < 64 ? table[c * NG + g] : table[(c * BLK + g * GS) >> log2p];
 #pragma unroll
-      for (int g = 0; g < KG; ++g) idk[g] = GS < 64 ? table[c * NG + own + g] : table[(c * kPBlock + (own + g) * GS) >> log2p];
+      for (int g = 0; g < KG; ++g) idk[g] = GS < 64 ? table[c * NG + own + g] : table[(c * BLK + (own + g) * GS) >> log2p];
     } else {
 #pragma unroll
-      for (int g = 0; g < NG; ++g) ids[g] = table[min((c * kPBlock + g * GS) >> log2p, pg.max_pages - 1)];
+      for (int g = 0; g < NG; ++g) ids[g] = table[min((c * BLK + g * GS) >> log2p, pg.max_pages - 1)];
 #pragma unroll
-      for (int g = 0; g < KG; ++g) idk[g] = table[min((c * kPBlock + (own + g) * GS) >> log2p, pg.max_pages - 1)];
+      for (int g = 0; g < KG; ++g) idk[g] = table[min((c * BLK + (own + g) * GS) >> log2p, pg.max_pages - 1)];
     }
   };
   find(c0);
   const Sequence sq = sequence_of(pg, b, T, room);
   if (slots == 1 && row0 == 0) {  // no merge follows: the rows that are no tokens are written here
     const int first = sq.ok ? sq.count : 0;
-    for (int e = threadIdx.x; e < (T - first) * G * D; e += 2 * D) {
+    for (int e = threadIdx.x; e < (T - first) * G * D; e += 64 * WAVES) {
       const int t = first + e / (G * D);
       o.out[(((size_t)b * T + t) * Hq + h * G) * D + e % (G * D)] = sq.ok ? 0 : kNanBits;
     }
   }
   const int total = sq.len + sq.count;
-  if (!sq.ok || sq.count == 0 || c0 * kPBlock >= total) return;
-  const int c1 = min(c0 + span, (total + kPBlock - 1) / kPBlock);
+  if (!sq.ok || sq.count == 0 || c0 * BLK >= total) return;
+  const int c1 = min(c0 + span, (total + BLK - 1) / BLK);
   const int rows = sq.count * G;
   if (row0 >= rows) return;
   const float sc = scale * kPLog2e;
@@ -349,8 +356,8 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
     uint32_t top = 0, none = 0;
 #pragma unroll
     for (int g = 0; g < NG; ++g) top = max(top, (uint32_t)ids[g]);
-    if ((c + 1) * kPBlock > total || top >= (uint32_t)pg.n_pages) {
-      auto fit = [&](int id, int g) { return c * kPBlock + g * GS < total ? id : ids[0]; };
+    if ((c + 1) * BLK > total || top >= (uint32_t)pg.n_pages) {
+      auto fit = [&](int id, int g) { return c * BLK + g * GS < total ? id : ids[0]; };
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
         const int id = fit(idk[g], own + g);
@@ -369,25 +376,25 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
   bf16x8_t kf[KT][KS];
   u32x4_t vf[ST][DW];
   const uint16_t* k_head = pg.k + (size_t)h * P * D;
-  const uint16_t* v_head = pg.vt + ((size_t)h * D + 32 * wave) * P;
+  const uint16_t* v_head = pg.vt + ((size_t)h * D + 16 * DW * wave) * P;
   const uint32_t k_lane = col * D + quad * 8;
   auto load_k = [&](int c) {
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const int in = (c * kPBlock + 16 * (wave * KT + kt)) & (P - 1);
+      const int in = (c * BLK + 16 * (wave * KT + kt)) & (P - 1);
       const uint16_t* kr = k_head + ((uint64_t)(uint32_t)idk[kt * 16 / GS] * pg.k_stride + in * D);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = *reinterpret_cast<const bf16x8_t*>(kr + (k_lane + ks * 32));
     }
   };
-  // V^T rows: dims 32 wave + 16dt + col, keys 32s + 8quad + 0..7 of the block.
+  // V^T rows: dims 16DW wave + 16dt + col, keys 32s + 8quad + 0..7 of the block.
   const uint32_t v_lane = col * P + 8 * (GS == 16 ? quad & 1 : quad);
   auto load_v = [&](int c) {
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
       auto base = [&](int i) {
         const int key = 32 * s + 16 * i;
-        return v_head + ((uint64_t)(uint32_t)ids[key / GS] * pg.vt_stride + (GS < 64 ? key & (P - 1) : (c * kPBlock + key) & (P - 1)));
+        return v_head + ((uint64_t)(uint32_t)ids[key / GS] * pg.vt_stride + (GS < 64 ? key & (P - 1) : (c * BLK + key) & (P - 1)));
       };
       if constexpr (GS == 16) {
         const uint16_t *b0 = base(0), *b1 = base(1);
@@ -406,13 +413,13 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
   load_k(c0);
   load_v(c0);
   bf16x8_t qf[KS];
-  if constexpr (W == 1) {
+  if constexpr (kKept) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(bf16x8_t, qr[ks]);
   } else {
 #pragma unroll
     for (int i = 0; i < QN; ++i) {
-      const int e = threadIdx.x + i * 2 * D;
+      const int e = threadIdx.x + i * 64 * WAVES;
       if (e < W * 16 * (D / 8)) *reinterpret_cast<u32x4_t*>(&q_lds[e / (D / 8) * QP + e % (D / 8) * 8]) = qr[i];
     }
     lds_barrier();
@@ -429,15 +436,15 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
     for (int dt = 0; dt < DW; ++dt) ao[w][dt] = go[w][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   for (int c = c0; c < c1; ++c) {
-    const int key0 = c * kPBlock;
+    const int key0 = c * BLK;
     const bool more = c + 1 < c1;
-    const bool edge = key0 + kPBlock > sq.len + 1 || bad;  // some row does not see, or may not read, some key
+    const bool edge = key0 + BLK > sq.len + 1 || bad;  // some row does not see, or may not read, some key
     if (more) find(c + 1);
     float s[W][KT][4];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       if (w && row0 + 16 * w >= rows) continue;
-      if constexpr (W != 1) {
+      if constexpr (!kKept) {
         const uint16_t* qp = &q_lds[(16 * w + col) * QP + quad * 8];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
@@ -463,7 +470,7 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         const int r = row0 + 16 * w + col;
-        const int last = (r < rows ? sq.len + r / G : -1) - (key0 + 16 * wave * KT + 4 * quad);  // of the lane's keys
+        const int last = (r < rows ? sq.len + token(r) : -1) - (key0 + 16 * wave * KT + 4 * quad);  // of the lane's keys
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
           const bool none = (bad >> (own + kt * 16 / GS)) & 1;
@@ -545,13 +552,17 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
           asm volatile("" : "+v"(vf[st][dt]), "+v"(odd[dt]));  // piece by piece: interleaved, they take twice the registers
         }
       }
-      if (__any((odd[0] | odd[1]) != 0)) {
+      uint32_t any = odd[0];
+#pragma unroll
+      for (int dt = 1; dt < DW; ++dt) any |= odd[dt];
+      if (__any(any != 0)) {
         // How many of them each output's row sees: a product of the odd values' and the seen keys' ones.
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-          const int r = row0 + 16 * w + col, seen = (r < rows ? sq.len + r / G + 1 : 0) - (key0 + 8 * quad);
+          const int r = row0 + 16 * w + col, seen = (r < rows ? sq.len + token(r) + 1 : 0) - (key0 + 8 * quad);
 #pragma unroll
           for (int dt = 0; dt < DW; ++dt) {
+#pragma unroll 1
             for (int st = 0; st < ST; ++st) {
               u32x4_t a, k = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
@@ -607,7 +618,7 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
   }
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    const int r = row0 + 16 * w + col, d0 = wave * 32 + quad * 4;
+    const int r = row0 + 16 * w + col, d0 = wave * 16 * DW + quad * 4;
     if (r >= rows) continue;
     if (slots > 1) {  // a part, for the merge
       const size_t at = (((size_t)b * Hkv + h) * slots + blockIdx.x) * (size_t)(T * G) + r;
@@ -616,8 +627,8 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
       if (wave == 0 && quad == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{gm[w], gl[w]};
       continue;
     }
-    const size_t orow = (size_t)b * T + r / G;
-    const int head = h * G + r % G;
+    const int t = token(r), head = h * G + r - t * G;
+    const size_t orow = (size_t)b * T + t;
     const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
     const float inv = 1.f / gl[w];
 #pragma unroll
@@ -636,18 +647,37 @@ __global__ __launch_bounds__(2 * D, 2) void paged_block_kernel(Pages pg, const u
 // 1), holding all four, or four waves' (kSplit 4) where there are many groups. A slot of the workspace is a group
 // (kJoined), or a pair, joined to its group here as the block kernel would.
 template <int D, bool kJoined, int kSplit>
-__global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int B, int T, int Hq, int Hkv, int room, int slots,
+__global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int T, int Hq, int G, int Hkv, int room, int slots,
                                                           const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                           Out o) {
   constexpr int E = D / 64, L = 4 / kSplit;  // lanes of groups that a wave holds
   constexpr int N = kJoined ? 1 : kPGroup / kPPair;        // slots of a group
-  constexpr int UN = (kSplit == 1 ? 8 : 16) / (L * N) < 1 ? 1 : (kSplit == 1 ? 8 : 16) / (L * N);  // rounds of groups loaded at once
+  constexpr int UN = kSplit == 1 ? (kJoined ? 2 : 1) : (kJoined ? 8 : 2);  // rounds of groups loaded at once
   __shared__ float ml[kSplit == 1 ? 1 : 4][2], sum[kSplit == 1 ? 1 : 4][kSplit == 1 ? 1 : D];
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const int heads = kSplit == 1 ? (Hq + 3) / 4 : Hq;  // workgroups of a token
-  const int head = kSplit == 1 ? (int)(blockIdx.x % heads) * 4 + wave : (int)(blockIdx.x % heads), t = blockIdx.x / heads;
-  const int b = blockIdx.y, G = Hq / Hkv, h = head / G;
+  const int head = kSplit == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x, t = blockIdx.y, b = blockIdx.z;
   if (head >= Hq) return;
+  const WorkIndex in = work_index(head, G);  // the kv head, and the head's place in its group
+  const size_t step = (size_t)T * G;
+  const size_t base = ((size_t)b * Hkv + in.quot) * slots * step + (size_t)t * G + in.rem;
+  float pm[UN][L][N], pl[UN][L][N], po[UN][L][N][E];
+  auto load = [&](int g0) {
+#pragma unroll
+    for (int u = 0; u < UN; ++u)
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const size_t at = base + (size_t)min((g0 + 4 * u + i) * N + n, slots - 1) * step;
+          const float2 two = reinterpret_cast<const float2*>(part_ml)[at];
+          pm[u][i][n] = two.x;
+          pl[u][i][n] = two.y;
+#pragma unroll
+          for (int e = 0; e < E; ++e) po[u][i][n][e] = part_o[at * D + lane + 64 * e];
+        }
+  };
+  int g0 = kSplit == 1 ? 0 : wave;
+  load(g0);  // beside the lengths: slots that this row turns out not to have are not used
   const Sequence sq = sequence_of(pg, b, T, room);
   const size_t orow = (size_t)b * T + t;
   uint16_t* op = o.out + (orow * Hq + head) * D;
@@ -657,9 +687,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int B, int T
     return;
   }
   // the blocks, pairs and groups that this row sees
-  const int nb = (sq.len + t) / kPBlock + 1, np = (nb + kPPair - 1) / kPPair, ng = (nb + kPGroup - 1) / kPGroup;
-  const size_t step = (size_t)T * G;
-  const size_t base = ((size_t)b * Hkv + h) * slots * step + (size_t)t * G + head % G;
+  const int nb = (sq.len + t) / paged_block(D) + 1, np = (nb + kPPair - 1) / kPPair, ng = (nb + kPGroup - 1) / kPGroup;
   float m[L], l[L], acc[L][E];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
@@ -668,22 +696,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int B, int T
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
   }
-  for (int g0 = kSplit == 1 ? 0 : wave; g0 < ng; g0 += 4 * UN) {
-    float pm[UN][L][N], pl[UN][L][N], po[UN][L][N][E];
-#pragma unroll
-    for (int u = 0; u < UN; ++u)
-#pragma unroll
-      for (int i = 0; i < L; ++i)
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const int slot = min((g0 + 4 * u + i) * N + n, (kJoined ? ng : np) - 1);
-          const size_t at = base + (size_t)slot * step;
-          const float2 two = reinterpret_cast<const float2*>(part_ml)[at];
-          pm[u][i][n] = two.x;
-          pl[u][i][n] = two.y;
-#pragma unroll
-          for (int e = 0; e < E; ++e) po[u][i][n][e] = part_o[at * D + lane + 64 * e];
-        }
+  while (g0 < ng) {
 #pragma unroll
     for (int u = 0; u < UN; ++u)
 #pragma unroll
@@ -702,6 +715,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int B, int T
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[i][e] = fmaf(go[e], j.part, acc[i][e] * j.before);
       }
+    g0 += 4 * UN;
+    if (g0 < ng) load(g0);
   }
   const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
   if constexpr (kSplit == 1) {
@@ -735,7 +750,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int B, int T
   }
 }
 
-int paged_blocks(int keys) { return (keys + kPBlock - 1) / kPBlock; }
+int paged_blocks(int keys, int D) { return (keys + paged_block(D) - 1) / paged_block(D); }
 
 // Blocks per workgroup: a pair, or a group. Groups move the least (an eighth of the blocks' parts is written and read
 // again, which counts for many rows) and keep loads in flight from block to block, but need enough of them to fill the
@@ -752,7 +767,7 @@ int paged_span(int B, int Hkv, int nblk, int rows) {
 int paged_slots(int nblk, int span) { return (nblk + span - 1) / span; }
 
 size_t paged_workspace(int B, int T, int Hq, int Hkv, int D, int keys) {
-  const int nblk = paged_blocks(keys), slots = paged_slots(nblk, paged_span(B, Hkv, nblk, T * (Hq / Hkv)));
+  const int nblk = paged_blocks(keys, D), slots = paged_slots(nblk, paged_span(B, Hkv, nblk, T * (Hq / Hkv)));
   if (slots == 1) return 0;
   return (size_t)B * Hkv * slots * T * (Hq / Hkv) * (D + 2) * sizeof(float);
 }
@@ -788,12 +803,12 @@ int check_pages(const skinny_paged_kv* kv, int B, int T, int Hq, Pages& pg, cons
 template <int D>
 int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, float* ws,
                            const Out& o, hipStream_t s) {
-  const int rows = T * (Hq / Hkv);
-  const int nblk = paged_blocks(keys), span = paged_span(B, Hkv, nblk, rows), slots = paged_slots(nblk, span);
+  const int G = Hq / Hkv, rows = T * G;
+  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows), slots = paged_slots(nblk, span);
   float* ml = ws + (size_t)B * Hkv * slots * rows * D;
   const int halves = rows > 32;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(slots, Hkv << halves, B), dim3(2 * D), 0, s, pg, q, T, Hq, Hkv, keys, scale, span, slots,
+    hipLaunchKernelGGL(kernel, dim3(slots, Hkv << halves, B), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G, 65535 / G + 1, Hq, Hkv, keys, scale, span, slots,
                        halves, ws, ml, o);
   };
   auto page = [&](auto w) {
@@ -810,7 +825,7 @@ int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int
   // four waves a row where a wave's groups would be many, or the rows alone would not fill the card
   const bool split = groups > 8 || (int64_t)B * T * Hq <= 1024;
   auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((split ? Hq : (Hq + 3) / 4) * T, B), dim3(256), 0, s, pg, B, T, Hq, Hkv, keys, slots, ws, ml, o);
+    hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(256), 0, s, pg, T, Hq, G, Hkv, keys, slots, ws, ml, o);
   };
   if (span == kPGroup && split) merge(paged_merge_kernel<D, true, 4>);
   else if (span == kPGroup) merge(paged_merge_kernel<D, true, 1>);
