@@ -21,8 +21,9 @@ constexpr int kPMaxRows = 64;  // query rows per kv head: T x (Hq / Hkv)
 // A block's keys, and the waves that share it: 64 KB of K and V for 128 and 256 dims, a wave's part of which is 64 registers.
 __host__ __device__ constexpr int paged_block(int D) { return D == 256 ? 64 : 128; }
 __host__ __device__ constexpr int paged_waves(int D) { return D == 64 ? 2 : 4; }
-constexpr int kPPair = 2;      // blocks joined left to right: what a workgroup takes at least
-constexpr int kPGroup = 8;     // blocks whose pairs are joined left to right, by the workgroup that takes them all or by the merge
+constexpr int kPQuad = 4;      // blocks joined left to right
+constexpr int kPLanes = 8;     // running joins of groups in the merge
+constexpr int kPGroup = 8;     // blocks whose quads are joined left to right
 
 // Memory that this kernel only reads, for uniform addresses: loaded into scalar registers.
 typedef const __attribute__((address_space(4))) int32_t* words_t;
@@ -231,9 +232,9 @@ __global__ __launch_bounds__(256) void paged_store_kernel(Pages pg, StoreRows ro
 // only a block at the sequence's end, or one with a missing page, needs stands behind one branch, and addresses are
 // formed in scalars once per page.
 //
-// Blocks are joined left to right in pairs, pairs in groups of kPGroup blocks, the groups by the merge. All are cut at
-// fixed positions of the sequence, and keys that a row does not see add exact zeros, so a row's bits depend on its own
-// sequence and position alone: not on the batch, on T, on who joins the pairs, or on where the pages lie.
+// Blocks are joined left to right in quads, quads in groups of kPGroup blocks, groups by the merge. All are cut at fixed
+// positions of the sequence, and keys that a row does not see add exact zeros, so a row's bits depend on its own sequence
+// and position alone: not on the batch, on T, on who joins the blocks, or on where the pages lie.
 
 // The first n (0 to 8) of eight consecutive keys' values, the others zero.
 __device__ __forceinline__ u32x4_t first_keys(u32x4_t v, int n) {
@@ -425,7 +426,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
     lds_barrier();
   }
 
-  // The pair's and the group's maximum (log2 units) and sum of this lane's row of every tile, and its outputs.
+  // The quad's and the group's maximum (log2 units) and sum of this lane's row of every tile, and its outputs.
   float am[W], al[W], gm[W], gl[W];
   f32x4_t ao[W][DW], go[W][DW];
 #pragma unroll
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
     }
     if (more) load_v(c + 1);
     bad = bad_next;
-    const bool end = !more || (c + 1) % kPPair == 0;  // of the pair
+    const bool end = !more || (c + 1) % kPQuad == 0;  // of the quad
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       if (w && row0 + 16 * w >= rows) continue;
@@ -643,19 +644,19 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
   }
 }
 
-// The rows' groups joined: group g in order onto lane g % 4 of four, then the four in order. A row is one wave's (kSplit
-// 1), holding all four, or four waves' (kSplit 4) where there are many groups. A slot of the workspace is a group
-// (kJoined), or a pair, joined to its group here as the block kernel would.
-template <int D, bool kJoined, int kSplit>
-__global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int T, int Hq, int G, int Hkv, int room, int slots,
+// The rows' groups joined: group g in order onto lane g % kPLanes, then the lanes in order. A row is one wave's, holding all
+// lanes, or (kSplit) a workgroup's with a wave for each. A slot of the workspace is kSlot blocks: a
+// group, or a quad or a block, joined to its group here as the block kernel would.
+template <int D, int kSlot, bool kSplit>
+__global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kernel(Pages pg, int T, int Hq, int G, int Hkv, int room, int slots,
                                                           const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                           Out o) {
-  constexpr int E = D / 64, L = 4 / kSplit;  // lanes of groups that a wave holds
-  constexpr int N = kJoined ? 1 : kPGroup / kPPair;        // slots of a group
-  constexpr int UN = kSplit == 1 ? (kJoined ? 2 : 1) : (kJoined ? 8 : 2);  // rounds of groups loaded at once
-  __shared__ float ml[kSplit == 1 ? 1 : 4][2], sum[kSplit == 1 ? 1 : 4][kSplit == 1 ? 1 : D];
+  constexpr int E = D / 64, L = kSplit ? 1 : kPLanes;      // lanes of groups that a wave holds
+  constexpr int N = kPGroup / kSlot;                       // slots of a group
+  constexpr int UN = 8 / (L * N) > 1 ? 8 / (L * N) : 1;    // rounds of groups loaded at once
+  __shared__ float ml[kSplit ? kPLanes : 1][2], sum[kSplit ? kPLanes : 1][kSplit ? D : 1];
   const int lane = threadIdx.x & 63, wave = wave_id();
-  const int head = kSplit == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x, t = blockIdx.y, b = blockIdx.z;
+  const int head = kSplit ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave, t = blockIdx.y, b = blockIdx.z;
   if (head >= Hq) return;
   const WorkIndex in = work_index(head, G);  // the kv head, and the head's place in its group
   const size_t step = (size_t)T * G;
@@ -668,7 +669,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int T, int H
       for (int i = 0; i < L; ++i)
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-          const size_t at = base + (size_t)min((g0 + 4 * u + i) * N + n, slots - 1) * step;
+          const size_t at = base + (size_t)min((g0 + kPLanes * u + i) * N + n, slots - 1) * step;
           const float2 two = reinterpret_cast<const float2*>(part_ml)[at];
           pm[u][i][n] = two.x;
           pl[u][i][n] = two.y;
@@ -676,18 +677,18 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int T, int H
           for (int e = 0; e < E; ++e) po[u][i][n][e] = part_o[at * D + lane + 64 * e];
         }
   };
-  int g0 = kSplit == 1 ? 0 : wave;
+  int g0 = kSplit ? wave : 0;
   load(g0);  // beside the lengths: slots that this row turns out not to have are not used
   const Sequence sq = sequence_of(pg, b, T, room);
   const size_t orow = (size_t)b * T + t;
   uint16_t* op = o.out + (orow * Hq + head) * D;
   if (!sq.ok || t >= sq.count) {
-    if (kSplit == 1 || wave == 0)
+    if (!kSplit || wave == 0)
       for (int d = lane; d < D; d += 64) op[d] = sq.ok ? 0 : kNanBits;
     return;
   }
-  // the blocks, pairs and groups that this row sees
-  const int nb = (sq.len + t) / paged_block(D) + 1, np = (nb + kPPair - 1) / kPPair, ng = (nb + kPGroup - 1) / kPGroup;
+  // the blocks, slots and groups that this row sees
+  const int nb = (sq.len + t) / paged_block(D) + 1, ns = (nb + kSlot - 1) / kSlot, ng = (nb + kPGroup - 1) / kPGroup;
   float m[L], l[L], acc[L][E];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
@@ -701,28 +702,39 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int T, int H
     for (int u = 0; u < UN; ++u)
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        const int g = g0 + 4 * u + i;
+        const int g = g0 + kPLanes * u + i;
         if (g >= ng) continue;
-        float gm = -INFINITY, gl = 0.f, go[E] = {};
+        float gm = -INFINITY, gl = 0.f, go[E] = {}, am = -INFINITY, al = 0.f, ao[E] = {};
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-          if (kJoined || g * N + n < np) {
-            const Join j = join(gm, gl, pm[u][i][n], pl[u][i][n]);
+        for (int n = 0; n < N; ++n) {
+          if (g * N + n < ns) {
+            const Join j = join(am, al, pm[u][i][n], pl[u][i][n]);
 #pragma unroll
-            for (int e = 0; e < E; ++e) go[e] = fmaf(po[u][i][n][e], j.part, go[e] * j.before);
+            for (int e = 0; e < E; ++e) ao[e] = fmaf(po[u][i][n][e], j.part, ao[e] * j.before);
           }
+          if ((n + 1) * kSlot % kPQuad == 0) {
+            const Join j = join(gm, gl, am, al);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              go[e] = fmaf(ao[e], j.part, go[e] * j.before);
+              ao[e] = 0.f;
+            }
+            am = -INFINITY;
+            al = 0.f;
+          }
+        }
         const Join j = join(m[i], l[i], gm, gl);
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[i][e] = fmaf(go[e], j.part, acc[i][e] * j.before);
       }
-    g0 += 4 * UN;
+    g0 += kPLanes * UN;
     if (g0 < ng) load(g0);
   }
   const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
-  if constexpr (kSplit == 1) {
+  if constexpr (!kSplit) {
     float rm = -INFINITY, rl = 0.f, ro[E] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kPLanes; ++i) {
       const Join j = join(rm, rl, m[i], l[i]);
 #pragma unroll
       for (int e = 0; e < E; ++e) ro[e] = fmaf(acc[i][e], j.part, ro[e] * j.before);
@@ -738,10 +750,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int T, int H
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[wave][lane + 64 * e] = acc[0][e];
     __syncthreads();
-    for (int d = threadIdx.x; d < D; d += 256) {
+    for (int d = threadIdx.x; d < D; d += 64 * kPLanes) {
       float rm = -INFINITY, rl = 0.f, ro = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < kPLanes; ++w) {
         const Join j = join(rm, rl, ml[w][0], ml[w][1]);
         ro = fmaf(sum[w][d], j.part, ro * j.before);
       }
@@ -752,22 +764,27 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(Pages pg, int T, int H
 
 int paged_blocks(int keys, int D) { return (keys + paged_block(D) - 1) / paged_block(D); }
 
-// Blocks per workgroup: a pair, or a group. Groups move the least (an eighth of the blocks' parts is written and read
-// again, which counts for many rows) and keep loads in flight from block to block, but need enough of them to fill the
-// card, also where sequences end early; sequences of at most one group then also need no merge. Measured, us a call, pairs /
-// groups, 8 kv heads of 128 dims, 4 query heads each, B sequences: one token: 1 x 32768 keys (264 groups) 41.4 / 47.2, 32 of
-// up to 2048 (768, half of them past their end) 31.9 / 37.8, 16 x 8000 (1024) 114 / 107, 64 x 4000 (2048) 211 / 200; of one
-// group, 4 x 1000 13.0 / 22.4, 16 x 500 14.4 / 14.7, 64 x 300 29.6 / 21.3. Eight tokens: 4 x 4000 (128) 24.5 / 29.4,
-// 1 x 32768 48.2 / 49.7, 16 x 2000 (256) 41.5 / 35.5, 64 x 4000 258 / 220.
-int paged_span(int B, int Hkv, int nblk, int rows) {
-  const int64_t all = (int64_t)B * Hkv * ((nblk + kPGroup - 1) / kPGroup);
-  return all >= (nblk <= kPGroup ? 128 : rows <= 16 ? 1024 : 256) ? kPGroup : kPPair;
+// Blocks per workgroup: one, a quad, or a group. Single blocks are the most parallel; the more a workgroup takes, the
+// fewer parts are written and read again (of 32 rows of 128 dims a quarter of a block's own bytes) and the longer its loads
+// stay in flight from block to block, but it takes enough of them to fill the card, also where sequences end early; one
+// part a sequence needs no merge. Measured, us a call by blocks / quads / groups, 4 query heads per kv head, B x keys:
+// one token, 8 heads of 128 dims: 1 x 2048 (136 blocks) 9.4 / 14.2 / 21.9, 4 x 4000 (1024) 19.4 / 19.6 / 26.9, 16 x 2000
+// (2048) 33.1 / 30.9 / 32.2, 32 of up to 2048 (4352) 39.7 / 38.1 / 42.7, 16 x 8000 (8064) 116 / 107 / 105, 64 x 4000
+// (16384) 217 / 201 / 197; in one part, 64 x 300 26.7 / 21.0, 64 x 1000 61 / 56 / 52, 16 x 500 13.7 / 14.1. Eight tokens:
+// 4 x 1000 (256) 14.3 / 18.0 / 23.3, 1 x 8192 (520) 19.4 / 18.2 / 26.8, 16 x 2000 55 / 36 / 35, 4 x 16000 (4032) 84 / 63 /
+// 60. One token, 4 heads of 256 dims: 1 x 8192 (516) 18.0 / 17.3 / 25.2, 8 x 4000 (2048) 35 / 32 / 32, 32 x 2000 (4096)
+// 63 / 58 / 56; 9 of up to 5003, 3 tokens (2880) 32 / 35 / 41.
+int paged_span(int B, int Hkv, int nblk, int rows, int D) {
+  const int64_t heads = (int64_t)B * Hkv, all = heads * nblk;
+  const bool heavy = rows > 16;
+  if (all >= (heavy ? 3000 : D == 256 ? 4096 : 8192) || (nblk <= kPGroup && nblk > kPQuad && heads >= 256)) return kPGroup;
+  return all >= (heavy ? 400 : D == 256 ? 512 : 1536) || (nblk <= kPQuad && heads >= 128) ? kPQuad : 1;
 }
 
 int paged_slots(int nblk, int span) { return (nblk + span - 1) / span; }
 
 size_t paged_workspace(int B, int T, int Hq, int Hkv, int D, int keys) {
-  const int nblk = paged_blocks(keys, D), slots = paged_slots(nblk, paged_span(B, Hkv, nblk, T * (Hq / Hkv)));
+  const int nblk = paged_blocks(keys, D), slots = paged_slots(nblk, paged_span(B, Hkv, nblk, T * (Hq / Hkv), D));
   if (slots == 1) return 0;
   return (size_t)B * Hkv * slots * T * (Hq / Hkv) * (D + 2) * sizeof(float);
 }
@@ -804,7 +821,7 @@ template <int D>
 int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, float* ws,
                            const Out& o, hipStream_t s) {
   const int G = Hq / Hkv, rows = T * G;
-  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows), slots = paged_slots(nblk, span);
+  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows, D), slots = paged_slots(nblk, span);
   float* ml = ws + (size_t)B * Hkv * slots * rows * D;
   const int halves = rows > 32;
   auto go = [&](auto kernel) {
@@ -822,15 +839,17 @@ int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int
   if (const int rc = skinny_check_launch("paged_attention")) return rc;
   if (slots == 1) return SKINNY_OK;
   const int groups = (nblk + kPGroup - 1) / kPGroup;
-  // four waves a row where a wave's groups would be many, or the rows alone would not fill the card
-  const bool split = groups > 8 || (int64_t)B * T * Hq <= 1024;
+  // eight waves a row where the rows alone would not fill the card, and always for blocks
+  const bool split = span == 1 || (int64_t)B * T * Hq <= (groups > 8 ? 1024 : 512);
   auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(256), 0, s, pg, T, Hq, G, Hkv, keys, slots, ws, ml, o);
+    hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(split ? 64 * kPLanes : 256), 0, s, pg, T, Hq, G, Hkv,
+                       keys, slots, ws, ml, o);
   };
-  if (span == kPGroup && split) merge(paged_merge_kernel<D, true, 4>);
-  else if (span == kPGroup) merge(paged_merge_kernel<D, true, 1>);
-  else if (split) merge(paged_merge_kernel<D, false, 4>);
-  else merge(paged_merge_kernel<D, false, 1>);
+  if (span == 1) merge(paged_merge_kernel<D, 1, true>);
+  else if (span == kPQuad && split) merge(paged_merge_kernel<D, kPQuad, true>);
+  else if (span == kPQuad) merge(paged_merge_kernel<D, kPQuad, false>);
+  else if (split) merge(paged_merge_kernel<D, kPGroup, true>);
+  else merge(paged_merge_kernel<D, kPGroup, false>);
   return skinny_check_launch("paged_attention merge");
 }
 
