@@ -283,11 +283,11 @@ __device__ __forceinline__ float quads_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// W tiles of 16 query rows; a call of more rows per kv head than 32 (`halves` 1) takes two workgroups a run, the second
+// W tiles of 16 query rows; a call of more rows per kv head than 32 (kHalves) takes two workgroups a run, the second
 // of which finds K and V in the caches. by_g: 65536 / G rounded up, G = Hq / Hkv. GS: keys of a block that share a page: the page size where that is 16 or 32, else 64.
-template <int D, int W, int GS>
+template <int D, int W, int GS, bool kHalves>
 __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T, int G, int by_g, int Hq,
-                                                               int Hkv, int room, float scale, int span, int slots, int halves,
+                                                               int Hkv, int room, float scale, int span, int slots,
                                                                float* __restrict__ part_o, float* __restrict__ part_ml,
                                                                Out o) {
   constexpr int BLK = paged_block(D), WAVES = paged_waves(D);
@@ -300,8 +300,8 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
   __shared__ u32x4_t p_lds[W][2][ST][64];
   __shared__ __attribute__((aligned(16))) float m_lds[W * 16][WAVES], l_lds[W * 16][WAVES];
   __shared__ __attribute__((aligned(16))) uint16_t q_lds[kKept ? 8 : W * 16 * QP];
-  const int h = blockIdx.y >> halves, b = blockIdx.z;
-  const int row0 = blockIdx.y & halves ? 16 * W : 0;  // of the rows per kv head
+  const int h = kHalves ? blockIdx.y >> 1 : blockIdx.y, b = blockIdx.z;
+  const int row0 = kHalves && (blockIdx.y & 1) ? 16 * W : 0;  // of the rows per kv head
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quad = lane >> 4;
   const int c0 = blockIdx.x * span;
@@ -388,26 +388,26 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
       for (int ks = 0; ks < KS; ++ks) kf[kt][ks] = *reinterpret_cast<const bf16x8_t*>(kr + (k_lane + ks * 32));
     }
   };
-  // V^T rows: dims 16DW wave + 16dt + col, keys 32s + 8quad + 0..7 of the block.
+  // V^T rows: dims 16DW wave + 16dt + col, keys 32s + 8quad + 0..7 of the block. Loaded past the caches' retention where no
+  // other workgroup wants them, a dim tile's steps one after the other, so that the two halves of a line of 64 keys are asked
+  // for together. 64 sequences of 4000 keys of 128 dims with pages of 16 / 64 slots: 193 / 197 us with ordinary loads, 184 /
+  // 190 so, K's loads alike 201 / 202; in 64-dim heads 107 / 108, 90 / 98. With two workgroups a run 328 / 338 as it is, 361 /
+  // 401 past the caches.
   const uint32_t v_lane = col * P + 8 * (GS == 16 ? quad & 1 : quad);
   auto load_v = [&](int c) {
 #pragma unroll
-    for (int s = 0; s < ST; ++s) {
-      auto base = [&](int i) {
-        const int key = 32 * s + 16 * i;
-        return v_head + ((uint64_t)(uint32_t)ids[key / GS] * pg.vt_stride + (GS < 64 ? key & (P - 1) : (c * BLK + key) & (P - 1)));
-      };
-      if constexpr (GS == 16) {
-        const uint16_t *b0 = base(0), *b1 = base(1);
-        const uint16_t* vr = (quad >= 2 ? b1 : b0) + v_lane;
+    for (int dt = 0; dt < DW; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DW; ++dt) vf[s][dt] = *reinterpret_cast<const u32x4_t*>(vr + dt * 16 * P);
-      } else {
+      for (int s = 0; s < ST; ++s) {
+        auto base = [&](int i) {
+          const int key = 32 * s + 16 * i;
+          return v_head + ((uint64_t)(uint32_t)ids[key / GS] * pg.vt_stride + (GS < 64 ? key & (P - 1) : (c * BLK + key) & (P - 1)));
+        };
         const uint16_t* vr = base(0);
-#pragma unroll
-        for (int dt = 0; dt < DW; ++dt) vf[s][dt] = *reinterpret_cast<const u32x4_t*>(vr + (v_lane + dt * 16 * P));
+        if constexpr (GS == 16) vr = quad >= 2 ? base(1) : vr;
+        const u32x4_t* at = reinterpret_cast<const u32x4_t*>(vr + (v_lane + dt * 16 * P));
+        vf[s][dt] = kHalves ? *at : __builtin_nontemporal_load(at);
       }
-    }
   };
 
   bad = settle(c0);
@@ -823,19 +823,20 @@ int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int
   const int G = Hq / Hkv, rows = T * G;
   const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows, D), slots = paged_slots(nblk, span);
   float* ml = ws + (size_t)B * Hkv * slots * rows * D;
-  const int halves = rows > 32;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(slots, Hkv << halves, B), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G, 65535 / G + 1, Hq, Hkv, keys, scale, span, slots,
-                       halves, ws, ml, o);
+    hipLaunchKernelGGL(kernel, dim3(slots, rows > 32 ? 2 * Hkv : Hkv, B), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G,
+                       65535 / G + 1, Hq, Hkv, keys, scale, span, slots, ws, ml, o);
   };
-  auto page = [&](auto w) {
+  auto page = [&](auto w, auto h) {
     constexpr int W = decltype(w)::value;
-    if (pg.log2p == 4) go(paged_block_kernel<D, W, 16>);
-    else if (pg.log2p == 5) go(paged_block_kernel<D, W, 32>);
-    else go(paged_block_kernel<D, W, 64>);
+    constexpr bool kHalves = decltype(h)::value;
+    if (pg.log2p == 4) go(paged_block_kernel<D, W, 16, kHalves>);
+    else if (pg.log2p == 5) go(paged_block_kernel<D, W, 32, kHalves>);
+    else go(paged_block_kernel<D, W, 64, kHalves>);
   };
-  if (rows <= 16) page(std::integral_constant<int, 1>{});
-  else page(std::integral_constant<int, 2>{});
+  if (rows <= 16) page(std::integral_constant<int, 1>{}, std::false_type{});
+  else if (rows <= 32) page(std::integral_constant<int, 2>{}, std::false_type{});
+  else page(std::integral_constant<int, 2>{}, std::true_type{});
   if (const int rc = skinny_check_launch("paged_attention")) return rc;
   if (slots == 1) return SKINNY_OK;
   const int groups = (nblk + kPGroup - 1) / kPGroup;
