@@ -569,17 +569,20 @@ typedef struct {
  * weights: none), rotate-half RoPE over the first rotary_dim dims from a skinny_rope_table_dim table
  * of at least max_pages*page positions; keys and values into their slots, queries to q_out
  * [B*T][Hq][D] (padding rows zero). fp32 inside, rounded once. B and T at most 65535. A page that the
- * call writes must belong to one sequence. */
+ * call writes must stand once in the table (pages that are only read may be shared): values go out in
+ * pieces of eight slots, the slots of no new token with what they held. q_out overlaps no input. */
 int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int T, int Hq, int q_stride, int k_offset, int v_offset,
                             const uint16_t* q_norm, const uint16_t* k_norm, float eps, int rotary_dim,
                             const float* rope_table, int rope_positions, const skinny_paged_kv* kv, uint16_t* q_out,
                             void* stream);
 /* Attention of q [B*T][Hq][D] over the cached and the new tokens (which must be in the pages):
- * token t of sequence b sees positions <= lengths[b] + t. T * Hq / n_kv <= 64. `keys` is the host's
- * bound on lengths[b] + counts[b] (at most max_pages*page); a sequence past it is NaN. With `gate`
- * (row stride ld_gate, head stride gate_stride) the output is multiplied by sigmoid(gate). out
- * [B*T][Hq*D], padding rows zero. A row's bits depend only on its own sequence and position: not on
- * B, T, the page size or the pages' places. The workspace (16-byte aligned, of
+ * token t of sequence b sees positions <= lengths[b] + t. T * Hq / n_kv <= 64, scale > 0. `keys` is
+ * the host's bound on lengths[b] + counts[b] (at most max_pages*page); a sequence past it is NaN. With
+ * `gate` (row stride ld_gate, head stride gate_stride) the output is multiplied by sigmoid(gate). out
+ * [B*T][Hq*D], padding rows zero, overlaps no input. A row's numbers have the same bits whatever B, T,
+ * `keys`, the page size, the pages' places and the other sequences are. A value that a row sees and
+ * that is not finite makes it NaN, and so does a score that is NaN or +inf (-inf is weight 0; nothing
+ * but -inf is NaN); what it does not see changes nothing. The workspace (16-byte aligned, of
  * skinny_paged_attn_workspace_bytes; 0 bytes: NULL will do) carries nothing from call to call; calls
  * that may overlap need their own. */
 size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int keys);

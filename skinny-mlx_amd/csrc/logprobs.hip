@@ -379,7 +379,7 @@ extern "C" int skinny_token_logprobs_bf16(const uint16_t* logits, int rows, int 
   SKINNY_CHECK_ARG(top >= 0 && top <= kMaxTop && top <= V, "token_logprobs: top=%d (at most %d, and V)", top, kMaxTop);
   SKINNY_CHECK_ARG(logits && tokens && workspace && logprob && entropy && (top == 0 || (ids && top_logprob)),
                    "token_logprobs: null pointer");
-  SKINNY_CHECK_ARG(inv_temp > 0.f && inv_temp <= 3.0e38f, "token_logprobs: bad temperature");
+  SKINNY_CHECK_ARG(inv_temp > 0.f && inv_temp <= 1.0e38f, "token_logprobs: bad temperature");
   SKINNY_CHECK_ARG(skinny_aligned(logits, 2) && skinny_aligned(tokens, 4) && skinny_aligned(workspace, 4),
                    "token_logprobs: misaligned buffer");
   const size_t need = skinny_token_logprobs_workspace_bytes(rows, V, top);

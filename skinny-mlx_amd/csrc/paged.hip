@@ -15,6 +15,7 @@
 
 namespace {
 
+constexpr int kPMaxRuns = 65535;  // runs of a sequence: a grid's last index
 constexpr float kPLog2e = 1.4426950408889634f;
 constexpr int kPMaxRows = 64;  // query rows per kv head: T x (Hq / Hkv)
 
@@ -284,7 +285,13 @@ __device__ __forceinline__ float quads_sum(float v) {
 }
 
 // W tiles of 16 query rows; a call of more rows per kv head than 32 (kHalves) takes two workgroups a run, the second
-// of which finds K and V in the caches. by_g: 65536 / G rounded up, G = Hq / Hkv. GS: keys of a block that share a page: the page size where that is 16 or 32, else 64.
+// of which finds K and V in the caches. by_g: 65536 / G rounded up, G = Hq / Hkv. GS: keys of a block that share a page: the
+// page size where that is 16 or 32, else 64.
+//
+// Grid (heads, sequences, runs): the eight dies take workgroups in turn, so neighbours are heads, whose work is alike, and
+// the runs that a sequence turns out not to have come last, of little cost. With the runs first, 32 sequences of 1023
+// keys took, in groups, 44 us a call for a bound of 1032 keys and 61 for one of 4112 (runs of eight: a die each); so 31
+// and 33. 64 of up to 1000: 42 and 38.
 template <int D, int W, int GS, bool kHalves>
 __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T, int G, int by_g, int Hq,
                                                                int Hkv, int room, float scale, int span, int slots,
@@ -300,11 +307,12 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
   __shared__ u32x4_t p_lds[W][2][ST][64];
   __shared__ __attribute__((aligned(16))) float m_lds[W * 16][WAVES], l_lds[W * 16][WAVES];
   __shared__ __attribute__((aligned(16))) uint16_t q_lds[kKept ? 8 : W * 16 * QP];
-  const int h = kHalves ? blockIdx.y >> 1 : blockIdx.y, b = blockIdx.z;
-  const int row0 = kHalves && (blockIdx.y & 1) ? 16 * W : 0;  // of the rows per kv head
+  const bool second = kHalves && (int)blockIdx.x >= Hkv;
+  const int h = second ? blockIdx.x - Hkv : blockIdx.x, b = blockIdx.y, slot = blockIdx.z;
+  const int row0 = second ? 16 * W : 0;  // of the rows per kv head
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int col = lane & 15, quad = lane >> 4;
-  const int c0 = blockIdx.x * span;
+  const int c0 = slot * span;
   // The queries, the first block's pages and the lengths are asked for at once.
   constexpr int QN = kKept ? KS : (W * 16 * (D / 8) + 64 * WAVES - 1) / (64 * WAVES);
   auto token = [&](int r) { return r * by_g >> 16; };  // of row r, which is head r - token * G
@@ -622,7 +630,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
     const int r = row0 + 16 * w + col, d0 = wave * 16 * DW + quad * 4;
     if (r >= rows) continue;
     if (slots > 1) {  // a part, for the merge
-      const size_t at = (((size_t)b * Hkv + h) * slots + blockIdx.x) * (size_t)(T * G) + r;
+      const size_t at = (((size_t)b * Hkv + h) * slots + slot) * (size_t)(T * G) + r;
 #pragma unroll
       for (int dt = 0; dt < DW; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * D + d0 + dt * 16) = go[w][dt];
       if (wave == 0 && quad == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{gm[w], gl[w]};
@@ -768,12 +776,14 @@ int paged_blocks(int keys, int D) { return (keys + paged_block(D) - 1) / paged_b
 // fewer parts are written and read again (of 32 rows of 128 dims a quarter of a block's own bytes) and the longer its loads
 // stay in flight from block to block, but it takes enough of them to fill the card, also where sequences end early; one
 // part a sequence needs no merge. Measured, us a call by blocks / quads / groups, 4 query heads per kv head, B x keys:
-// one token, 8 heads of 128 dims: 1 x 2048 (136 blocks) 9.4 / 14.2 / 21.9, 4 x 4000 (1024) 19.4 / 19.6 / 26.9, 16 x 2000
-// (2048) 33.1 / 30.9 / 32.2, 32 of up to 2048 (4352) 39.7 / 38.1 / 42.7, 16 x 8000 (8064) 116 / 107 / 105, 64 x 4000
-// (16384) 217 / 201 / 197; in one part, 64 x 300 26.7 / 21.0, 64 x 1000 61 / 56 / 52, 16 x 500 13.7 / 14.1. Eight tokens:
-// 4 x 1000 (256) 14.3 / 18.0 / 23.3, 1 x 8192 (520) 19.4 / 18.2 / 26.8, 16 x 2000 55 / 36 / 35, 4 x 16000 (4032) 84 / 63 /
-// 60. One token, 4 heads of 256 dims: 1 x 8192 (516) 18.0 / 17.3 / 25.2, 8 x 4000 (2048) 35 / 32 / 32, 32 x 2000 (4096)
-// 63 / 58 / 56; 9 of up to 5003, 3 tokens (2880) 32 / 35 / 41.
+// one token, 8 heads of 128 dims: 1 x 2048 (136 blocks) 10.0 / 16.1 / 25.3, 1 x 8192 (520) 16.1 / 17.4 / 26.6, 4 x 4000
+// (1024) 20.1 / 19.4 / 28.1, 16 x 2000 (2048) 30.5 / 29.5 / 30.7, 32 of up to 2048 (4352) 41.5 / 38.2 / 46.2, 16 x 8000
+// (8064) 103 / 92 / 91, 64 x 4000 (16384) 238 / 204 / 193; in one part, 64 x 300 30.2 / 21.3, 64 x 1000 58 / 52 / 48, 16 x
+// 500 14.2 / 14.6. Eight tokens: 4 x 1000 (256) 14.9 / 18.7 / 25.3, 1 x 8192 (520) 22.3 / 18.9 / 28.6, 16 x 2000 54 / 36 /
+// 35, 32 of up to 2048 78 / 53 / 53, 4 x 16000 (4032) 85 / 62 / 57. One token, 4 heads of 256 dims: 1 x 8192 (516) 17.1 /
+// 17.3 / 25.5, 8 x 4000 (2016) 30.8 / 29.0 / 28.4, 32 x 2000 (4096) 59 / 52 / 50; 9 of up to 5003, 3 tokens (2880) 37 / 37 /
+// 44. 8 heads of 64 dims: 1 x 8192 11.5 / 13.7 / 20.9, 16 x 2000 19.3 / 18.2 / 22.9, 64 x 4000 92 / 93 / 101, 64 x 8000
+// (32256) 207 / 190 / 189.
 int paged_span(int B, int Hkv, int nblk, int rows, int D) {
   const int64_t heads = (int64_t)B * Hkv, all = heads * nblk;
   const bool heavy = rows > 16;
@@ -824,7 +834,7 @@ int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int
   const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows, D), slots = paged_slots(nblk, span);
   float* ml = ws + (size_t)B * Hkv * slots * rows * D;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(slots, rows > 32 ? 2 * Hkv : Hkv, B), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G,
+    hipLaunchKernelGGL(kernel, dim3(rows > 32 ? 2 * Hkv : Hkv, B, slots), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G,
                        65535 / G + 1, Hq, Hkv, keys, scale, span, slots, ws, ml, o);
   };
   auto page = [&](auto w, auto h) {
@@ -907,6 +917,10 @@ extern "C" int skinny_paged_attention_bf16(const uint16_t* q, int B, int T, int 
                    "paged_attention: gate strides %lld, %d", (long long)ld_gate, gate_stride);
   SKINNY_CHECK_ARG(skinny_aligned(q, 16) && skinny_aligned(out, 16) && skinny_aligned(gate, 2) && skinny_aligned(workspace, 16),
                    "paged_attention: misaligned buffer");
+  const int nblk = paged_blocks(keys, D);
+  SKINNY_CHECK_ARG(paged_slots(nblk, paged_span(B, Hkv, nblk, T * (Hq / Hkv), D)) <= kPMaxRuns,
+                   "paged_attention: keys=%d, at most %d", keys, kPMaxRuns * kPGroup * paged_block(D));
+  SKINNY_CHECK_ARG(scale > 0.f && scale <= 1e38f, "paged_attention: scale=%g must be positive", (double)scale);
   const size_t need = paged_workspace(B, T, Hq, Hkv, D, keys);
   SKINNY_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "paged_attention: workspace of %zu bytes, needs %zu",
                    workspace ? workspace_bytes : (size_t)0, need);

@@ -381,7 +381,8 @@ def paged_store(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_stride:
 
     counts (int32 [B], None: T each) says how many of a sequence's T rows are tokens; the others are padding, stored
     nowhere, their queries zero. A sequence that its row of `pages` cannot hold is not stored and its queries are NaN.
-    lengths are not advanced: that is the caller's, after the step. A page written to must be one sequence's own."""
+    lengths are not advanced: that is the caller's, after the step. A page written to must stand once in `pages`; pages
+    that are only read may be shared."""
     _bf16_2d(qkv, "qkv")
     dev = qkv.get_device()
     kv, b = _paged_kv(dev, lengths, counts, pages, k_pages, vt_pages)
@@ -431,7 +432,8 @@ def paged_attention(q: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor,
     gate: bf16 [B*T, Hq, D], any row and head strides (a view of q_proj's rows); the output is multiplied by its sigmoid.
     keys: the host's bound on lengths[b] + counts[b] (None: what a row of `pages` holds), which sizes the launch; a
     sequence past it comes out NaN. workspace: from paged_attn_workspace (None: allocated for the call). A row's bits
-    depend on its own sequence and position alone: not on the batch, T, the page size or the pages' places."""
+    depend on its own sequence and position alone: not on the batch, T, `keys`, the page size or the pages' places. A value
+    that a row sees and that is not finite makes it NaN, and so does a score that is NaN or +inf."""
     if not (q.is_cuda and q.dtype == BF16 and q.dim() == 3 and q.is_contiguous() and q.numel() > 0):
         raise ValueError("q must be contiguous bf16 [B*T, Hq, D] on the GPU")
     dev = q.get_device()

@@ -185,3 +185,41 @@ def test_wrapper_refuses(dev):
     wide = torch.zeros((1, 524289), dtype=BF16, device=dev)
     with pytest.raises(ValueError, match="V=524289"):
         K.token_logprobs(wide, tok[:1])
+
+
+@pytest.mark.parametrize("v", [151936, 524288])
+@pytest.mark.parametrize("top", [1, 20, 32])
+def test_equal_scores_in_many_slices(dev, v, top):
+    """More candidates of one score than a row's join can list: still the lowest indices first."""
+    rows = torch.stack([torch.full((v,), 2.0), torch.where(torch.arange(v) % 997 == 5, 7.0, -1.0),
+                        torch.where(torch.arange(v) >= v - 9000, 3.0, 0.5)]).to(BF16)
+    tokens = torch.tensor([0, 5, v - 1], dtype=I32)
+    _check(rows, tokens, top, 1.0, K.token_logprobs(rows.to(dev), tokens.to(dev), top), f"{v} {top}")
+
+
+def test_the_most_rows(dev):
+    x = _scores(65535, 40, 13)
+    tokens = torch.arange(65535, dtype=I32) % 40
+    _check(x, tokens, 3, 1.0, K.token_logprobs(x.to(dev), tokens.to(dev), 3))
+
+
+def test_calls_on_two_streams_at_once(dev):
+    x = _scores(16, 100003, 14).to(dev)
+    tokens = torch.arange(16, dtype=I32, device=dev)
+    ref = K.token_logprobs(x, tokens, 5)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(K.token_logprobs(x, tokens, 5))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(o, ref))
+
+
+@pytest.mark.parametrize("T", [1e-3, 0.05, 30.0])
+def test_cold_and_hot_temperatures(dev, T):
+    x = _scores(4, 20001, 15)
+    tokens = torch.tensor([0, 1, 2, 20000], dtype=I32)
+    tokens[0] = int(x[0].float().argmax())
+    _check(x, tokens, 6, T, K.token_logprobs(x.to(dev), tokens.to(dev), 6, T))

@@ -574,3 +574,132 @@ def test_a_batch_decodes_and_scores_as_its_sequences_do(dev):
         ref = own[len(p) - 1:].float()
         got = torch.stack([x[5][i] for x in together]).float()
         assert (got - ref).norm() <= 2e-2 * ref.norm()
+
+
+def _runs(c, b, T, hq, keys):
+    """Blocks per workgroup and whether a merge follows, from the workspace's size."""
+    n = K.paged_attn_workspace(b, T, hq, c.hkv, c.d, keys, c.dev).numel()
+    nblk = -(-keys // (64 if c.d == 256 else 128))
+    slots = n // (b * T * hq * (c.d + 2) * 4)
+    return nblk if slots == 0 else next(s for s in (1, 4, 8) if -(-nblk // s) == slots)
+
+
+@pytest.mark.parametrize("d,G,T,b", [(64, 1, 1, 3), (64, 2, 16, 40), (128, 4, 1, 3), (128, 4, 4, 40), (128, 4, 8, 20), (128, 4, 16, 9),
+                                     (256, 4, 1, 5), (256, 4, 5, 30), (256, 3, 16, 12)])
+def test_bits_do_not_depend_on_how_the_keys_are_cut(dev, d, G, T, b):
+    """The host's bound decides how many blocks a workgroup takes and who joins them; the rows keep their bits, alone too."""
+    hkv = 2
+    hq = hkv * G
+    pattern = [2300, 0, 1025, 513, 64, 1100, 2047 - T, 7, 300, 1536]
+    lengths = [pattern[i % 10] for i in range(b)]
+    counts = [T - (i % 3 if T > 2 else 0) for i in range(b)]
+    c = Cache(dev, d + T, hkv, d, 32, lengths, counts, width=(1 << 18) // 32)
+    q = torch.randn((b * T, hq, d), generator=torch.Generator().manual_seed(20)).to(BF16).to(dev)
+    ln, cn = c.len_t(), _ints(counts, dev)
+    seen, ref = set(), None
+    for keys in (2400, 1 << 14, 1 << 15, 1 << 16, 1 << 18):
+        seen.add(_runs(c, b, T, hq, keys))
+        got = K.paged_attention(q, ln, c.pages, c.k, c.vt, d ** -0.5, counts=cn, keys=keys)
+        ref = got if ref is None else ref
+        assert torch.isfinite(got).all() and torch.equal(_bits(got), _bits(ref)), keys
+    assert 8 in seen and len(seen) > 1
+    for i in sorted({0, 2, b // 2, b - 1}):
+        seen.add(_runs(c, 1, T, hq, 2400))
+        for t in sorted({0, counts[i] - 1}):  # one token at a time, the others before it in the cache
+            one = K.paged_attention(q[i * T + t:i * T + t + 1], ln[i:i + 1] + t, c.pages[i:i + 1], c.k, c.vt, d ** -0.5, keys=2400)
+            assert torch.equal(_bits(one[0]), _bits(ref[i * T + t])), (i, t)
+    assert 1 in seen or 4 in seen
+
+
+@pytest.mark.parametrize("hkv,d,b,keys", [(64, 64, 4, 1000), (32, 256, 8, 500), (32, 128, 4, 400)])
+def test_sequences_of_one_part(dev, hkv, d, b, keys):
+    """Enough heads that a workgroup takes a whole sequence and writes its rows itself."""
+    lengths = [keys - 2, 0, keys // 2, 130, 63, keys - 70, 300, 1][:b]
+    counts = [2, 1, 2, 0, 2, 1, 2, 2][:b]
+    c = Cache(dev, d, hkv, d, 16, lengths, counts)
+    assert _runs(c, b, 2, hkv, keys) > 1 and _runs(c, 1, 2, hkv, keys) == 1
+    q = torch.randn((2 * b, hkv, d), generator=torch.Generator().manual_seed(21)).to(BF16).to(dev)
+    ln, cn = c.len_t(), _ints(counts, dev)
+    got = K.paged_attention(q, ln, c.pages, c.k, c.vt, d ** -0.5, counts=cn, keys=keys).view(b, 2, -1)
+    for i in range(b):
+        one = K.paged_attention(q[2 * i:2 * i + 2], ln[i:i + 1], c.pages[i:i + 1], c.k, c.vt, d ** -0.5, counts=cn[i:i + 1], keys=keys)
+        assert torch.equal(_bits(got[i]), _bits(one)) and (got[i, counts[i]:] == 0).all(), i
+
+
+def test_sequences_that_share_pages(dev):
+    """A prefix held once: the same pages in several rows of the table, each sequence's last page its own."""
+    hq, hkv, d, page = 8, 2, 128, 32
+    c = Cache(dev, 30, hkv, d, page, [200, 200, 200], [1, 1, 1])
+    pages = c.pages.clone()
+    pages[1:, :6] = pages[0, :6]  # 192 tokens of the first sequence
+    k, vt = c.k.clone(), c.vt.clone()
+    for i in (1, 2):
+        for p in range(6):
+            k[c.pages[i, p]], vt[c.pages[i, p]] = c.k[c.pages[0, p]], c.vt[c.pages[0, p]]
+    q = torch.randn((3, hq, d), generator=torch.Generator().manual_seed(22)).to(BF16).to(dev)
+    ref = K.paged_attention(q, c.len_t(), c.pages, k, vt, d ** -0.5)
+    assert torch.equal(_bits(K.paged_attention(q, c.len_t(), pages, c.k, c.vt, d ** -0.5)), _bits(ref))
+
+
+def test_the_most_sequences(dev):
+    """65535 of them, none with a cache: a row's output is its own value."""
+    b, d = 65535, 64
+    k = torch.empty((b, 1, 16, d), dtype=BF16, device=dev)
+    vt = torch.empty((b, 1, d, 16), dtype=BF16, device=dev)
+    ln = torch.zeros(b, dtype=I32, device=dev)
+    pages = torch.arange(b - 1, -1, -1, dtype=I32, device=dev).view(b, 1)
+    rows = torch.randn((b, 4 * d), device=dev, generator=torch.Generator(dev).manual_seed(23)).to(BF16)
+    q = K.paged_store(rows, 2, 1, d, d, 2 * d, 3 * d, None, None, EPS, d, K.rope_table_dim(1e4, d, 16, dev), ln, pages, k, vt)
+    assert torch.equal(_bits(q), _bits(rows[:, :2 * d].reshape(b, 2, d)))  # position 0: cos 1, sin 0
+    got = K.paged_attention(q, ln, pages, k, vt, d ** -0.5).view(b, 2, d)
+    assert torch.equal(_bits(got), _bits(rows[:, None, 3 * d:].expand(-1, 2, -1)))
+
+
+def test_the_most_tokens_at_once(dev):
+    """65535 new tokens stored in one call: the bits of storing them in pieces."""
+    T, d, page = 65535, 64, 16
+    rows = torch.randn((T, 4 * d), device=dev, generator=torch.Generator(dev).manual_seed(24)).to(BF16)
+    w = -(-(T + 5) // page)
+    pages = torch.randperm(w, device=dev, generator=torch.Generator(dev).manual_seed(25)).to(I32).view(1, w)
+    table = K.rope_table_dim(1e6, d, w * page, dev)
+    outs = []
+    for step in (T, 9001):
+        k = torch.zeros((w, 1, page, d), dtype=BF16, device=dev)
+        vt = torch.zeros((w, 1, d, page), dtype=BF16, device=dev)
+        q = [K.paged_store(rows[i:i + step], 2, 1, d, d, 2 * d, 3 * d, None, None, EPS, d, table, _ints([5 + i], dev), pages, k, vt)
+             for i in range(0, T, step)]
+        outs.append((torch.cat(q), k, vt))
+    assert all(torch.equal(_bits(x), _bits(y)) for x, y in zip(*outs))
+
+
+def test_calls_on_another_stream(dev):
+    """Each call runs on the current stream: a store and an attention behind a slow write of their rows on a side stream."""
+    hq, hkv, d = 8, 2, 128
+    c = Cache(dev, 31, hkv, d, 64, [300, 5], [1, 1], fill=False)
+    rows = torch.randn((2, 12 * d), generator=torch.Generator().manual_seed(26)).to(BF16).to(dev)
+    table = K.rope_table_dim(1e6, d, c.width * 64, dev)
+    ln = c.len_t()
+
+    def step(x, k, vt):
+        q = K.paged_store(x, hq, hkv, d, d, 8 * d, 10 * d, None, None, EPS, d, table, ln, c.pages, k, vt)
+        return K.paged_attention(q, ln, c.pages, k, vt, d ** -0.5)
+
+    ref = step(rows, c.k.clone(), c.vt.clone())
+    x, k, vt = torch.zeros_like(rows), c.k.clone(), c.vt.clone()
+    busy = torch.randn((4096, 4096), device=dev)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(8):
+            busy = busy @ busy * 1e-2
+        x.copy_(rows)
+        got = step(x, k, vt)
+    torch.cuda.synchronize()
+    assert torch.equal(_bits(got), _bits(ref))
+
+
+def test_scale_must_be_positive(dev):
+    c = Cache(dev, 32, 1, 64, 16, [3], [1])
+    q = torch.zeros((1, 1, 64), dtype=BF16, device=dev)
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            K.paged_attention(q, c.len_t(), c.pages, c.k, c.vt, scale)

@@ -121,3 +121,19 @@ def test_wrappers_refuse_host_tensors():
         K.paged_attention(torch.zeros((1, 1, 64), dtype=b16), ln, pages, kp, vp, 1.0)
     with pytest.raises(ValueError, match="GPU"):
         K.token_logprobs(torch.zeros((1, 64), dtype=b16), torch.zeros(1, dtype=i32))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("inf"), 2e38])
+def test_paged_attention_refuses_scales(scale):
+    rc = _lib.lib().skinny_paged_attention_bf16(DUMMY, 2, 3, 32, _kv(), 512, scale, None, 0, 0, DUMMY, 1 << 40, DUMMY, None)
+    _expect_einval(rc, "scale=")
+
+
+def test_sequences_past_the_grid_are_refused():
+    kv = _kv(max_pages=1 << 22, ld_pages=1 << 22, page=256, k_stride=8 * 256 * 128, vt_stride=8 * 256 * 128)
+    _expect_einval(_attend(kv, keys=65535 * 8 * 128 + 1, nbytes=1 << 60), "at most 67107840")
+
+
+def test_temperatures_whose_inverse_is_no_number_are_refused():
+    rc = _lib.lib().skinny_token_logprobs_bf16(DUMMY, 4, 1000, 1000, DUMMY, 2e38, 0, DUMMY, 1 << 30, DUMMY, DUMMY, None, None, None)
+    _expect_einval(rc, "temperature")
