@@ -223,3 +223,34 @@ def test_cold_and_hot_temperatures(dev, T):
     tokens = torch.tensor([0, 1, 2, 20000], dtype=I32)
     tokens[0] = int(x[0].float().argmax())
     _check(x, tokens, 6, T, K.token_logprobs(x.to(dev), tokens.to(dev), 6, T))
+
+
+@pytest.mark.parametrize("v", [9000, 40000, 151936])
+@pytest.mark.parametrize("top", [2, 7, 32])
+def test_plateaus_below_and_beside_the_largest(dev, v, top):
+    """Rows whose top-th score is one of many equal ones: few above them, in other places; more of them than can be ranked, in few
+    threads' parts or in many; all of them late in the row."""
+    g = torch.Generator().manual_seed(v + top)
+    x = torch.randn((6, v), generator=g).to(BF16).clamp(-4, 2.5)
+    x[0, 100:1700] = 3.0
+    x[1, 100:1700] = 3.0
+    x[1, [5, 1699, v - 1, v // 2]] = torch.tensor([4.0, 5.0, 4.0, 6.0], dtype=BF16)
+    x[2, ::9] = 3.0
+    x[2, -3:] = 3.5
+    x[3, v - 2000:] = 3.0
+    x[3, 7] = 8.0
+    x[4, :2048] = torch.linspace(3.0, 60.0, 2048).to(BF16)  # many above any thread's, ascending
+    x[5] = float("-inf")
+    x[5, [1, v - 1, v // 3]] = torch.tensor([1.0, 1.0, -2.0], dtype=BF16)
+    tokens = torch.tensor([0, v - 1, 3, 7, 2047, 1], dtype=I32)
+    _check(x, tokens, top, 1.0, K.token_logprobs(x.to(dev), tokens.to(dev), top), f"{v} {top}")
+
+
+def test_few_numbers_among_nan(dev):
+    v = 30000
+    x = torch.full((1, v), float("nan"), dtype=BF16)
+    x[0, [29999, 12000, 4]] = torch.tensor([2.0, float("-inf"), 1.0], dtype=BF16)
+    lp, ent, ids, alt = K.token_logprobs(x.to(dev), torch.zeros(1, dtype=I32, device=dev), 32)
+    rest = [i for i in range(40) if i != 4][:29]
+    assert ids[0].tolist() == [29999, 4, 12000] + rest
+    assert torch.isnan(lp).all() and torch.isnan(ent).all() and torch.isnan(alt).all()
