@@ -780,14 +780,16 @@ int paged_blocks(int keys, int D) { return (keys + paged_block(D) - 1) / paged_b
 // (1024) 20.1 / 19.4 / 28.1, 16 x 2000 (2048) 30.5 / 29.5 / 30.7, 32 of up to 2048 (4352) 41.5 / 38.2 / 46.2, 16 x 8000
 // (8064) 103 / 92 / 91, 64 x 4000 (16384) 238 / 204 / 193; in one part, 64 x 300 30.2 / 21.3, 64 x 1000 58 / 52 / 48, 16 x
 // 500 14.2 / 14.6. Eight tokens: 4 x 1000 (256) 14.9 / 18.7 / 25.3, 1 x 8192 (520) 22.3 / 18.9 / 28.6, 16 x 2000 54 / 36 /
-// 35, 32 of up to 2048 78 / 53 / 53, 4 x 16000 (4032) 85 / 62 / 57. One token, 4 heads of 256 dims: 1 x 8192 (516) 17.1 /
-// 17.3 / 25.5, 8 x 4000 (2016) 30.8 / 29.0 / 28.4, 32 x 2000 (4096) 59 / 52 / 50; 9 of up to 5003, 3 tokens (2880) 37 / 37 /
-// 44. 8 heads of 64 dims: 1 x 8192 11.5 / 13.7 / 20.9, 16 x 2000 19.3 / 18.2 / 22.9, 64 x 4000 92 / 93 / 101, 64 x 8000
-// (32256) 207 / 190 / 189.
+// 35, 12 of up to 4000 (3072) 51 / 34 / 43 and 52 / 41 / 47, 12 x 4000 70 / 51 / 53, 32 of up to 2048 78 / 53 / 53, 48 of
+// up to 2000 (6144) 105 / 66 / 61; six tokens, 256 dims, 16 of up to 4000 (4032) 75 / 55 / 50. One token, 4 heads of 256
+// dims: 1 x 8192 (516) 17.1 / 17.3 / 25.5, 8 x 4000 (2016) 30.8 / 29.0 / 28.4, 32 x 2000 (4096) 59 / 52 / 50; 9 of up to
+// 5003, 3 tokens (2880) 37 / 37 / 44. 8 heads of 64 dims: 1 x 8192 11.5 / 13.7 / 20.9, 16 x 2000 19.3 / 18.2 / 22.9, 64 x
+// 4000 92 / 93 / 101, 64 x 8000 (32256) 207 / 190 / 189.
 int paged_span(int B, int Hkv, int nblk, int rows, int D) {
   const int64_t heads = (int64_t)B * Hkv, all = heads * nblk;
   const bool heavy = rows > 16;
-  if (all >= (heavy ? 3000 : D == 256 ? 4096 : 8192) || (nblk <= kPGroup && nblk > kPQuad && heads >= 256)) return kPGroup;
+  if (all >= (D == 256 ? (heavy ? 3000 : 4096) : heavy ? 4096 : 8192) || (nblk <= kPGroup && nblk > kPQuad && heads >= 256))
+    return kPGroup;
   return all >= (heavy ? 400 : D == 256 ? 512 : 1536) || (nblk <= kPQuad && heads >= 128) ? kPQuad : 1;
 }
 
