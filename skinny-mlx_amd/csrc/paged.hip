@@ -252,9 +252,9 @@ struct Out {
 };
 
 // One output value, divided by the sum of its weights, gated, rounded.
-__device__ __forceinline__ uint16_t finished(float o, float inv, const uint16_t* gate, int d) {
+__device__ __forceinline__ uint16_t finished(float o, float inv, bool gated, uint32_t gate) {
   o *= inv;
-  if (gate) o *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(bf16_bits_to_f32(gate[d]) * -kPLog2e));
+  if (gated) o *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(bf16_bits_to_f32(gate) * -kPLog2e));
   return f32_to_bf16_bits(o);
 }
 
@@ -644,9 +644,11 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
     for (int dt = 0; dt < DW; ++dt) {
       u32x2_t two;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        two[i] = finished(go[w][dt][2 * i], inv, gp, d0 + dt * 16 + 2 * i) |
-                 (uint32_t)finished(go[w][dt][2 * i + 1], inv, gp, d0 + dt * 16 + 2 * i + 1) << 16;
+      for (int i = 0; i < 2; ++i) {
+        const int d = d0 + dt * 16 + 2 * i;
+        two[i] = finished(go[w][dt][2 * i], inv, gp, gp ? gp[d] : 0) |
+                 (uint32_t)finished(go[w][dt][2 * i + 1], inv, gp, gp ? gp[d + 1] : 0) << 16;
+      }
       *reinterpret_cast<u32x2_t*>(o.out + (orow * Hq + head) * D + d0 + dt * 16) = two;
     }
   }
@@ -662,14 +664,17 @@ __global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kerne
   constexpr int E = D / 64, L = kSplit ? 1 : kPLanes;      // lanes of groups that a wave holds
   constexpr int N = kPGroup / kSlot;                       // slots of a group
   constexpr int UN = 8 / (L * N) > 1 ? 8 / (L * N) : 1;    // rounds of groups loaded at once
-  __shared__ float ml[kSplit ? kPLanes : 1][2], sum[kSplit ? kPLanes : 1][kSplit ? D : 1];
+  __shared__ __attribute__((aligned(16))) float sum[kSplit ? kPLanes : 1][kSplit ? D : 1];
+  __shared__ float ml[kSplit ? kPLanes : 1][2];
   const int lane = threadIdx.x & 63, wave = wave_id();
   const int head = kSplit ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave, t = blockIdx.y, b = blockIdx.z;
   if (head >= Hq) return;
   const WorkIndex in = work_index(head, G);  // the kv head, and the head's place in its group
   const size_t step = (size_t)T * G;
   const size_t base = ((size_t)b * Hkv + in.quot) * slots * step + (size_t)t * G + in.rem;
-  float pm[UN][L][N], pl[UN][L][N], po[UN][L][N][E];
+  typedef float dims_t __attribute__((ext_vector_type(E)));  // a lane's: E * lane on
+  float pm[UN][L][N], pl[UN][L][N];
+  dims_t po[UN][L][N];
   auto load = [&](int g0) {
 #pragma unroll
     for (int u = 0; u < UN; ++u)
@@ -681,14 +686,21 @@ __global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kerne
           const float2 two = reinterpret_cast<const float2*>(part_ml)[at];
           pm[u][i][n] = two.x;
           pl[u][i][n] = two.y;
-#pragma unroll
-          for (int e = 0; e < E; ++e) po[u][i][n][e] = part_o[at * D + lane + 64 * e];
+          po[u][i][n] = *reinterpret_cast<const dims_t*>(part_o + at * D + E * lane);
         }
   };
   int g0 = kSplit ? wave : 0;
-  load(g0);  // beside the lengths: slots that this row turns out not to have are not used
-  const Sequence sq = sequence_of(pg, b, T, room);
+  load(g0);  // beside the lengths and the gate: slots that this row turns out not to have are not used
   const size_t orow = (size_t)b * T + t;
+  const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
+  uint32_t gate[E] = {};
+  if (gp) {
+    if constexpr (kSplit) gate[0] = gp[threadIdx.x % D];
+    else
+#pragma unroll
+      for (int e = 0; e < E; ++e) gate[e] = gp[E * lane + e];
+  }
+  const Sequence sq = sequence_of(pg, b, T, room);
   uint16_t* op = o.out + (orow * Hq + head) * D;
   if (!sq.ok || t >= sq.count) {
     if (!kSplit || wave == 0)
@@ -697,13 +709,13 @@ __global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kerne
   }
   // the blocks, slots and groups that this row sees
   const int nb = (sq.len + t) / paged_block(D) + 1, ns = (nb + kSlot - 1) / kSlot, ng = (nb + kPGroup - 1) / kPGroup;
-  float m[L], l[L], acc[L][E];
+  float m[L], l[L];
+  dims_t acc[L];
 #pragma unroll
   for (int i = 0; i < L; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[i][e] = 0.f;
+    acc[i] = dims_t(0.f);
   }
   while (g0 < ng) {
 #pragma unroll
@@ -712,7 +724,8 @@ __global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kerne
       for (int i = 0; i < L; ++i) {
         const int g = g0 + kPLanes * u + i;
         if (g >= ng) continue;
-        float gm = -INFINITY, gl = 0.f, go[E] = {}, am = -INFINITY, al = 0.f, ao[E] = {};
+        float gm = -INFINITY, gl = 0.f, am = -INFINITY, al = 0.f;
+        dims_t go(0.f), ao(0.f);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
           if (g * N + n < ns) {
@@ -738,9 +751,9 @@ __global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kerne
     g0 += kPLanes * UN;
     if (g0 < ng) load(g0);
   }
-  const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs : nullptr;
   if constexpr (!kSplit) {
-    float rm = -INFINITY, rl = 0.f, ro[E] = {};
+    float rm = -INFINITY, rl = 0.f;
+    dims_t ro(0.f);
 #pragma unroll
     for (int i = 0; i < kPLanes; ++i) {
       const Join j = join(rm, rl, m[i], l[i]);
@@ -748,24 +761,26 @@ __global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kerne
       for (int e = 0; e < E; ++e) ro[e] = fmaf(acc[i][e], j.part, ro[e] * j.before);
     }
     const float inv = 1.f / rl;
+    typedef uint16_t out_t __attribute__((ext_vector_type(E)));
+    out_t y;
 #pragma unroll
-    for (int e = 0; e < E; ++e) op[lane + 64 * e] = finished(ro[e], inv, gp, lane + 64 * e);
+    for (int e = 0; e < E; ++e) y[e] = finished(ro[e], inv, gp, gate[e]);
+    *reinterpret_cast<out_t*>(op + E * lane) = y;
   } else {
     if (lane == 0) {
       ml[wave][0] = m[0];
       ml[wave][1] = l[0];
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[wave][lane + 64 * e] = acc[0][e];
+    *reinterpret_cast<dims_t*>(&sum[wave][E * lane]) = acc[0];
     __syncthreads();
-    for (int d = threadIdx.x; d < D; d += 64 * kPLanes) {
+    if (const int d = threadIdx.x; d < D) {
       float rm = -INFINITY, rl = 0.f, ro = 0.f;
 #pragma unroll
       for (int w = 0; w < kPLanes; ++w) {
         const Join j = join(rm, rl, ml[w][0], ml[w][1]);
         ro = fmaf(sum[w][d], j.part, ro * j.before);
       }
-      op[d] = finished(ro, 1.f / rl, gp, d);
+      op[d] = finished(ro, 1.f / rl, gp, gate[0]);
     }
   }
 }
