@@ -343,9 +343,12 @@ def _paged_kv(dev: int, lengths: torch.Tensor, counts, pages: torch.Tensor, k_pa
     n, h, p, d = k_pages.shape
     if not (vt_pages.dtype == BF16 and vt_pages.shape == (n, h, d, p) and vt_pages.get_device() == dev):
         raise ValueError(f"vt_pages must be bf16 [{n}, {h}, {d}, {p}] (V transposed), on the rows' device")
-    ks, vs, pd = k_pages.stride(), vt_pages.stride(), p * d
-    if not ((ks[1:] == (pd, d, 1) or k_pages[0].is_contiguous()) and (vs[1:] == (pd, p, 1) or vt_pages[0].is_contiguous())):
-        raise ValueError("a page must be contiguous")
+    k_stride = vt_stride = h * p * d
+    if not (k_pages.is_contiguous() and vt_pages.is_contiguous()):
+        if not (k_pages[0].is_contiguous() and vt_pages[0].is_contiguous()):
+            raise ValueError("a page must be contiguous")
+        if n > 1:  # the stride of an axis of one entry is never stepped and may be anything
+            k_stride, vt_stride = k_pages.stride(0), vt_pages.stride(0)
     if not (lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.is_contiguous() and lengths.get_device() == dev
             and lengths.numel() > 0):
         raise ValueError("lengths must be contiguous int32 [B] on the rows' device")
@@ -356,13 +359,16 @@ def _paged_kv(dev: int, lengths: torch.Tensor, counts, pages: torch.Tensor, k_pa
     if not (pages.dtype == torch.int32 and pages.dim() == 2 and pages.get_device() == dev):
         raise ValueError(f"pages must be int32 [{b}, max_pages] on the rows' device")
     rows, w = pages.shape
-    ld, step = pages.stride()
-    # the stride of an axis of one entry is never stepped and may be anything
-    if not (rows == b and w > 0 and (w == 1 or step == 1) and (b == 1 or w <= ld < 2 ** 31)):
+    ld = w
+    if not (rows == b and w > 0):
         raise ValueError(f"pages must be int32 [{b}, max_pages] rows")
-    return _lib.PagedKV(lengths.data_ptr(), None if counts is None else counts.data_ptr(), pages.data_ptr(),
-                        w if b == 1 else ld, w, k_pages.data_ptr(), vt_pages.data_ptr(), h * pd if n == 1 else ks[0],
-                        h * pd if n == 1 else vs[0], n, p, h, d), b
+    if not pages.is_contiguous():
+        if b > 1:
+            ld = pages.stride(0)
+        if not ((w == 1 or pages.stride(1) == 1) and w <= ld < 2 ** 31):
+            raise ValueError(f"pages must be int32 [{b}, max_pages] rows")
+    return _lib.PagedKV(lengths.data_ptr(), None if counts is None else counts.data_ptr(), pages.data_ptr(), ld, w,
+                        k_pages.data_ptr(), vt_pages.data_ptr(), k_stride, vt_stride, n, p, h, d), b
 
 
 def _fits(t: torch.Tensor, dtype: torch.dtype, shape: tuple, dev: int) -> bool:
