@@ -320,7 +320,10 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(const uint16_t*
 #pragma unroll
     for (int k = 0; k < kLoads; ++k)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) reach += __popcll(ballot(order_of(e & 1 ? mx[k][e >> 1] >> 16 : mx[k][e >> 1] & 0xffffu) >= next));
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t o = order_of(e & 1 ? mx[k][e >> 1] >> 16 : mx[k][e >> 1] & 0xffffu);
+        reach += __popcll(ballot(o >= next));
+      }
     __syncthreads();
     if (lane == 0) red[wave] = reach;
     __syncthreads();
@@ -407,8 +410,8 @@ extern "C" int skinny_token_logprobs_bf16(const uint16_t* logits, int rows, int 
   hipLaunchKernelGGL(logprobs_slice_kernel, dim3(slices, rows), dim3(kThreads), 0, s, logits, V, ld, inv_temp, heads, maxima);
   if (const int rc = skinny_check_launch("token_logprobs")) return rc;
   auto join = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(rows), dim3(top ? kThreads : 64), 0, s, logits, ld, V, tokens, inv_temp, top, slices, heads, maxima,
-                       logprob, entropy, ids, top_logprob);
+    hipLaunchKernelGGL(kernel, dim3(rows), dim3(top ? kThreads : 64), 0, s, logits, ld, V, tokens, inv_temp, top, slices, heads,
+                       maxima, logprob, entropy, ids, top_logprob);
   };
   if (slices <= 8) join(logprobs_join_kernel<1>);
   else if (slices <= 32) join(logprobs_join_kernel<4>);

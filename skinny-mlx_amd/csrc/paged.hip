@@ -90,7 +90,8 @@ __device__ __forceinline__ void store_heads(const Pages& pg, const StoreRows& ro
   u32x4_t x4 = {0, 0, 0, 0}, w4 = {0, 0, 0, 0};
   const uint16_t* norm = query ? rows.qn : rows.kn;
   if (there) {
-    x4 = *reinterpret_cast<const u32x4_any_t*>(rows.qkv + r * rows.ldq + (query ? head * (size_t)rows.qs : rows.koff + (size_t)(head - Hq) * D) + d0);
+    const size_t at = query ? head * (size_t)rows.qs : rows.koff + (size_t)(head - Hq) * D;
+    x4 = *reinterpret_cast<const u32x4_any_t*>(rows.qkv + r * rows.ldq + at + d0);
     if (norm) w4 = *reinterpret_cast<const u32x4_any_t*>(norm + d0);
   }
   const Sequence sq = sequence_of(pg, b, T, room);
@@ -167,7 +168,8 @@ __device__ __forceinline__ void store_heads(const Pages& pg, const StoreRows& ro
 
 // 64 dims from `dim` on, of the value rows' Hkv * D, of the tokens in a granule's 16 slots: a dim per lane.
 template <int D>
-__device__ __forceinline__ void store_values(const Pages& pg, const StoreRows& rows, int T, int Hkv, int room, int granule, int dim) {
+__device__ __forceinline__ void store_values(const Pages& pg, const StoreRows& rows, int T, int Hkv, int room, int granule,
+                                             int dim) {
   const int lane = threadIdx.x & 63, b = blockIdx.z;
   if (dim >= Hkv * D) return;
   const Sequence sq = sequence_of(pg, b, T, room);
@@ -230,16 +232,16 @@ __global__ __launch_bounds__(256) void paged_store_kernel(Pages pg, StoreRows ro
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Attention. A workgroup takes a run of blocks of keys of one sequence and kv head. In a block each wave scores its share
-// of the keys (S^T = K Q^T, the K rows straight from memory into matrix-core
-// operands); the row maxima and then the weights P go through LDS, and each wave forms its share of the dims over all the block's
-// keys (O^T = V^T P^T). So K and V are read once, by one wave each, and no output is summed across waves. As soon as a
-// block's scores (outputs) are formed, its K (V) registers take the next block's loads, which are in flight through the
-// rest of the block.
+// Attention. A workgroup takes a run of blocks of keys of one sequence and kv head. In a block each wave scores its share of
+// the keys (S^T = K Q^T, the K rows straight from memory into matrix-core operands); the row maxima and then the weights P go
+// through LDS, and each wave forms its share of the dims over all the block's keys (O^T = V^T P^T). So K and V are read once,
+// by one wave each, and no output is summed across waves. As soon as a block's scores (outputs) are formed, its K (V)
+// registers take the next block's loads, which are in flight through the rest of the block.
 //
-// What bounds it is memory, if the instructions of a block (64 KB of K and V for 128 dims) stay few: everything that
-// only a block at the sequence's end, or one with a missing page, needs stands behind one branch, and addresses are
-// formed in scalars once per page.
+// What bounds it is memory, if the instructions of a block (64 KB of K and V for 128 dims) stay few: everything that only a
+// block at the sequence's end, or one with a missing page, needs stands behind one branch, and addresses are formed in
+// scalars once per page. One token of 4 sequences of 65536 keys, 8 heads of 128 dims: 180 us, 5.9 TB/s; of 32 sequences of up
+// to 2048 keys 31 us, 4.5 TB/s.
 //
 // Blocks are joined left to right in quads, quads in groups of kPGroup blocks, groups by the merge. All are cut at fixed
 // positions of the sequence, and keys that a row does not see add exact zeros, so a row's bits depend on its own sequence
@@ -301,10 +303,11 @@ __device__ __forceinline__ float quads_sum(float v) {
 // keys took, in groups, 44 us a call for a bound of 1032 keys and 61 for one of 4112 (runs of eight: a die each); so 31
 // and 33. 64 of up to 1000: 42 and 38.
 template <int D, int W, int GS, bool kHalves>
-__global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T, int G, int by_g, int Hq,
-                                                               int Hkv, int room, float scale, int span, int slots,
-                                                               float* __restrict__ part_o, float* __restrict__ part_ml,
-                                                               Out o) {
+__global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pages pg, const uint16_t* __restrict__ q, int T,
+                                                                             int G, int by_g, int Hq, int Hkv, int room,
+                                                                             float scale, int span, int slots,
+                                                                             float* __restrict__ part_o,
+                                                                             float* __restrict__ part_ml, Out o) {
   constexpr int BLK = paged_block(D), WAVES = paged_waves(D);
   constexpr int KT = BLK / 16 / WAVES, KS = D / 32;           // a wave's 16-key tiles; dim steps of a score
   constexpr int ST = BLK / 32, NG = BLK / GS;                 // a block's 32-key steps and pages
@@ -417,7 +420,8 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
       for (int s = 0; s < ST; ++s) {
         auto base = [&](int i) {
           const int key = 32 * s + 16 * i;
-          return v_head + ((uint64_t)(uint32_t)ids[key / GS] * pg.vt_stride + (GS < 64 ? key & (P - 1) : (c * BLK + key) & (P - 1)));
+          const int in = (GS < 64 ? key : c * BLK + key) & (P - 1);
+          return v_head + ((uint64_t)(uint32_t)ids[key / GS] * pg.vt_stride + in);
         };
         const uint16_t* vr = base(0);
         if constexpr (GS == 16) vr = quad >= 2 ? base(1) : vr;
@@ -663,12 +667,13 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
 }
 
 // The rows' groups joined: group g in order onto lane g % kPLanes, then the lanes in order. A row is one wave's, holding all
-// lanes, or (kSplit) a workgroup's with a wave for each. A slot of the workspace is kSlot blocks: a
-// group, or a quad or a block, joined to its group here as the block kernel would.
+// lanes, or (kSplit) a workgroup's with a wave for each. A slot of the workspace is kSlot blocks: a group, or a quad or a
+// block, joined to its group here as the block kernel would. Bound by latency: a launch and two round trips, 4 to 5.5 us.
 template <int D, int kSlot, bool kSplit>
-__global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kernel(Pages pg, int T, int Hq, int G, int Hkv, int room, int slots,
-                                                          const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                                                          Out o) {
+__global__ __launch_bounds__(kSplit ? 64 * kPLanes : 256) void paged_merge_kernel(Pages pg, int T, int Hq, int G, int Hkv,
+                                                                                  int room, int slots,
+                                                                                  const float* __restrict__ part_o,
+                                                                                  const float* __restrict__ part_ml, Out o) {
   constexpr int E = D / 64, L = kSplit ? 1 : kPLanes;      // lanes of groups that a wave holds
   constexpr int N = kPGroup / kSlot;                       // slots of a group
   constexpr int UN = 8 / (L * N) > 1 ? 8 / (L * N) : 1;    // rounds of groups loaded at once
@@ -803,7 +808,7 @@ int paged_blocks(int keys, int D) { return (keys + paged_block(D) - 1) / paged_b
 // (1024) 20.1 / 19.4 / 28.1, 16 x 2000 (2048) 30.5 / 29.5 / 30.7, 32 of up to 2048 (4352) 41.5 / 38.2 / 46.2, 16 x 8000
 // (8064) 103 / 92 / 91, 64 x 4000 (16384) 238 / 204 / 193; in one part, 64 x 300 30.2 / 21.3, 64 x 1000 58 / 52 / 48, 16 x
 // 500 14.2 / 14.6. Eight tokens: 4 x 1000 (256) 14.9 / 18.7 / 25.3, 1 x 8192 (520) 22.3 / 18.9 / 28.6, 16 x 2000 54 / 36 /
-// 35, 12 of up to 4000 (3072) 51 / 34 / 43 and 52 / 41 / 47, 12 x 4000 70 / 51 / 53, 32 of up to 2048 78 / 53 / 53, 48 of
+// 35, 12 of up to 4000 51 / 34 / 43 and 52 / 41 / 47, 12 x 4000 70 / 51 / 53, 32 of up to 2048 78 / 53 / 53, 48 of
 // up to 2000 (6144) 105 / 66 / 61; six tokens, 256 dims, 16 of up to 4000 (4032) 75 / 55 / 50. One token, 4 heads of 256
 // dims: 1 x 8192 (516) 17.1 / 17.3 / 25.5, 8 x 4000 (2016) 30.8 / 29.0 / 28.4, 32 x 2000 (4096) 59 / 52 / 50; 9 of up to
 // 5003, 3 tokens (2880) 37 / 37 / 44. 8 heads of 64 dims: 1 x 8192 11.5 / 13.7 / 20.9, 16 x 2000 19.3 / 18.2 / 22.9, 64 x
@@ -842,13 +847,13 @@ int check_pages(const skinny_paged_kv* kv, int B, int T, int Hq, Pages& pg, cons
   const int64_t need = (int64_t)kv->n_kv * P * kv->head_dim;
   SKINNY_CHECK_ARG(kv->k_stride >= need && kv->vt_stride >= need && kv->k_stride % 8 == 0 && kv->vt_stride % 8 == 0 &&
                        kv->k_stride <= INT32_MAX && kv->vt_stride <= INT32_MAX,
-                   "%s: page strides %lld, %lld (multiples of 8 below 2^31, at least Hkv*P*D=%lld)", what, (long long)kv->k_stride,
-                   (long long)kv->vt_stride, (long long)need);
+                   "%s: page strides %lld, %lld (multiples of 8 below 2^31, at least Hkv*P*D=%lld)", what,
+                   (long long)kv->k_stride, (long long)kv->vt_stride, (long long)need);
   SKINNY_CHECK_ARG(skinny_aligned(kv->k_pages, 16) && skinny_aligned(kv->vt_pages, 16) && skinny_aligned(kv->lengths, 4) &&
                        skinny_aligned(kv->counts, 4) && skinny_aligned(kv->pages, 4),
                    "%s: misaligned cache", what);
-  pg = Pages{kv->lengths, kv->counts, kv->pages, kv->k_pages, kv->vt_pages, (uint32_t)kv->k_stride, (uint32_t)kv->vt_stride, kv->ld_pages,
-             kv->max_pages, kv->n_pages, __builtin_ctz(P)};
+  pg = Pages{kv->lengths, kv->counts, kv->pages, kv->k_pages, kv->vt_pages, (uint32_t)kv->k_stride, (uint32_t)kv->vt_stride,
+             kv->ld_pages, kv->max_pages, kv->n_pages, __builtin_ctz(P)};
   return SKINNY_OK;
 }
 
@@ -913,8 +918,8 @@ extern "C" int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int 
   const StoreRows rows{qkv, ldq, q_stride, k_offset, v_offset, q_norm, k_norm};
   const hipStream_t s = (hipStream_t)stream;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((groups + (values * (granules_after_first(T) + 1) + T - 1) / T) | 1, T, B), dim3(256), 0, s, pg, rows, T, Hq,
-                       Hkv, eps, rotary_dim, rope_table, room, groups, values, q_out);
+    hipLaunchKernelGGL(kernel, dim3((groups + (values * (granules_after_first(T) + 1) + T - 1) / T) | 1, T, B), dim3(256), 0, s,
+                       pg, rows, T, Hq, Hkv, eps, rotary_dim, rope_table, room, groups, values, q_out);
   };
   if (D == 64) go(paged_store_kernel<64>);
   else if (D == 128) go(paged_store_kernel<128>);
