@@ -389,7 +389,8 @@ def paged_store(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_stride:
     nowhere, their queries zero. A sequence that its row of `pages` cannot hold is not stored and its queries are NaN.
     lengths are not advanced: that is the caller's, after the step. A page written to must stand once in `pages`; pages
     that are only read may be shared."""
-    _bf16_2d(qkv, "qkv")
+    if not (qkv.is_cuda and qkv.dtype == BF16 and qkv.dim() == 2 and qkv.stride(1) == 1):
+        raise ValueError("qkv must be a bf16 2-D GPU tensor")
     dev = qkv.get_device()
     kv, b = _paged_kv(dev, lengths, counts, pages, k_pages, vt_pages)
     rows, cols = qkv.shape
@@ -779,7 +780,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
 
     tokens int32 [rows]; one outside [0, V) has logprob -inf. Alternatives decrease, ties by index, NaN scores last. A
     score of -inf is a token of probability 0; a row with a NaN, a +inf or only -inf scores has NaN for its numbers."""
-    _bf16_2d(logits, "logits")
+    if not (logits.is_cuda and logits.dtype == BF16 and logits.dim() == 2 and logits.stride(1) == 1):
+        raise ValueError("logits must be a bf16 2-D GPU tensor")
     rows, V = logits.shape
     dev = logits.get_device()
     if not _fits(tokens, torch.int32, (rows,), dev):
@@ -793,10 +795,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
         raise ValueError("rows overlap")
     with _on_device(logits):
         L = _lib.lib()
-        lp = logits.new_empty(rows, dtype=torch.float32)
-        ent = logits.new_empty(rows, dtype=torch.float32)
+        lp = torch.empty_like(tokens, dtype=torch.float32)
+        ent = torch.empty_like(lp)
         ids = tokens.new_empty((rows, top))
-        alt = logits.new_empty((rows, top), dtype=torch.float32)
+        alt = torch.empty_like(ids, dtype=torch.float32)
         if rows:
             nbytes = L.skinny_token_logprobs_workspace_bytes(rows, V, top)
             ws = tokens.new_empty(nbytes // 4)
