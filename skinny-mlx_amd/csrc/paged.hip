@@ -261,11 +261,14 @@ struct Out {
   int gs;                // and from head to head
 };
 
-// One output value, divided by the sum of its weights, gated, rounded.
+// One output value, divided by the sum of its weights, gated, rounded. Sums that are not finite end here as one NaN: a value
+// that is not finite leaves an infinity or a NaN, by the sign of its weight's second term, which the joins keep (times a
+// factor that is no 0 or, of 0, as NaN). A compare and a select per value; no block pays for it.
 __device__ __forceinline__ uint16_t finished(float o, float inv, bool gated, uint32_t gate) {
   o *= inv;
+  const bool finite = fabsf(o) < INFINITY;
   if (gated) o *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(bf16_bits_to_f32(gate) * -kPLog2e));
-  return f32_to_bf16_bits(o);
+  return finite ? f32_to_bf16_bits(o) : kNanBits;
 }
 
 // Part (m, l, o) of a row joined to the parts before it: their factor and its own.

@@ -440,7 +440,8 @@ def paged_attention(q: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor,
     keys: the host's bound on lengths[b] + counts[b] (None: what a row of `pages` holds), which sizes the launch; a
     sequence past it comes out NaN. workspace: from paged_attn_workspace (None: allocated for the call). A row's bits
     depend on its own sequence and position alone: not on the batch, T, `keys`, the page size or the pages' places. A value
-    that a row sees and that is not finite makes it NaN, and so does a score that is NaN or +inf."""
+    that a row sees and that is not finite makes the row's output of that dim NaN, and so does a weighted sum past fp32's range;
+    a score that is NaN or +inf makes all of the row NaN."""
     if not (q.is_cuda and q.dtype == BF16 and q.dim() == 3 and q.is_contiguous() and q.numel() > 0):
         raise ValueError("q must be contiguous bf16 [B*T, Hq, D] on the GPU")
     dev = q.get_device()
