@@ -582,8 +582,8 @@ int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int T, int Hq, 
  * [B*T][Hq*D], padding rows zero, overlaps no input. A row's numbers have the same bits whatever B, T,
  * `keys`, the page size, the pages' places and the other sequences are. A value that a row sees and
  * that is not finite makes the row's output of that dim NaN (0x7fc0), with or without a gate, and so
- * does a weighted sum past fp32's range; a score that is NaN or +inf makes all dims NaN (-inf is weight
- * 0; nothing but -inf is NaN); what a row does not see changes nothing. The workspace (16-byte aligned, of
+ * does a weighted sum past fp32's range; a score (times the scale) that is NaN or +inf makes all dims
+ * NaN (-inf is weight 0; nothing but -inf is NaN); what a row does not see changes nothing. The workspace (16-byte aligned, of
  * skinny_paged_attn_workspace_bytes; 0 bytes: NULL will do) carries nothing from call to call; calls
  * that may overlap need their own. */
 size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int keys);

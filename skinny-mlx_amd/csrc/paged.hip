@@ -524,7 +524,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
 #pragma unroll
       for (int v = 1; v < WAVES; ++v) m = fmaxf(m, m_lds[16 * w + col][v]);
       mx[w] = m * sc;
-      const float ref = m == -INFINITY ? 0.f : mx[w];
+      const float ref = mx[w] == -INFINITY ? 0.f : mx[w];  // finite scores too, if the scale takes all of them there
       // P as the sum of two bf16 terms (2^-17 of each weight; one term's 2^-9 would be as large as the output's own
       // rounding).
       float sum = 0.f;

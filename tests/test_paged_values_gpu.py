@@ -92,3 +92,33 @@ def test_infinite_values_of_short_sequences(dev, d, bad):
     want[..., 7] = NAN_BITS
     got = K.paged_attention(q, lens, pages, k, vt, d ** -0.5, keys=n + 1).view(len(hits), hq, d)
     assert torch.equal(_bits(got), want)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("T", [1, 3])
+def test_scores_that_the_scale_takes_to_minus_infinity(dev, d, T):
+    """Finite products of query and key that the scale takes past fp32's range weigh nothing, as ones that are -inf themselves:
+    the same bits, whether whole blocks, joins of blocks or single keys are such, and NaN where nothing else is seen."""
+    hq, hkv, page, n, scale = 8, 2, 32, 1300, 64.0
+    block = 64 if d == 256 else 128
+    low = [range(0, block), range(block, 2 * block), range(0, 4 * block), range(0, 1024), range(1024, n), range(7, n),
+           range(0, n, 3), range(n - n % block, n + T), range(0, n + T)]
+    table, k, vt = _cache(dev, d + T, hkv, d, page, [n + T] * len(low), (1 << 16) // page)
+    pages, lens = torch.tensor(table, device=dev), _ints([n] * len(low), dev)
+    g = torch.Generator().manual_seed(4)
+    q = (torch.rand((len(low) * T, hq, d), generator=g) + 0.5).to(BF16).to(dev)
+    k = k * (2.0 ** -6 * d ** -0.5)             # ordinary scores of a few units
+    finite, infinite = k.clone(), k.clone()
+    for i, these in enumerate(low):
+        p = torch.tensor(list(these))
+        at = torch.from_numpy(table[i].astype(np.int64))[p // page]
+        finite[at.to(dev), :, (p % page).to(dev)] = -(2.0 ** 124) / d  # a product of -2^124, half as much again or less
+        infinite[at.to(dev), :, (p % page).to(dev)] = float("-inf")
+    for keys in (n + T, 1 << 13, 1 << 16):
+        got = K.paged_attention(q, lens, pages, finite, vt, scale, keys=keys).view(len(low), -1)
+        ref = K.paged_attention(q, lens, pages, infinite, vt, scale, keys=keys).view(len(low), -1)
+        assert torch.isfinite(ref[:-1]).all() and torch.isnan(ref[-1]).all(), keys
+        assert torch.equal(_bits(got), _bits(ref)), keys
+        over = K.paged_attention(q, lens, pages, -finite, vt, scale, keys=keys)  # past the other end: a score of +inf
+        assert (_bits(over) == NAN_BITS).all(), keys
+
