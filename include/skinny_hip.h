@@ -585,7 +585,8 @@ int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int T, int Hq, 
  * does a weighted sum past fp32's range; a score (times the scale) that is NaN or +inf makes all dims
  * NaN (-inf is weight 0; nothing but -inf is NaN); what a row does not see changes nothing. The workspace (16-byte aligned, of
  * skinny_paged_attn_workspace_bytes; 0 bytes: NULL will do) carries nothing from call to call; calls
- * that may overlap need their own. */
+ * that may overlap need their own. Its size does not grow with the call's: fewer sequences or keys are
+ * cut finer and can need more bytes, so a program with one workspace takes the largest of its sizes. */
 size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int keys);
 int skinny_paged_attention_bf16(const uint16_t* q, int B, int T, int Hq, const skinny_paged_kv* kv, int keys, float scale,
                                 const uint16_t* gate, int64_t ld_gate, int gate_stride, void* workspace,

@@ -423,7 +423,8 @@ def paged_store(qkv: torch.Tensor, n_q: int, n_kv: int, head_dim: int, q_stride:
 
 def paged_attn_workspace(batch: int, tokens: int, n_q: int, n_kv: int, head_dim: int, keys: int, device) -> torch.Tensor:
     """Workspace of paged_attention for calls of these sizes. It carries nothing from call to call; calls that may overlap,
-    on different streams or in graphs replayed side by side, each need their own."""
+    on different streams or in graphs replayed side by side, each need their own. Fewer sequences or a lower bound are cut
+    finer and can need more bytes: a program with one workspace for several sizes takes the largest of theirs."""
     nbytes = int(_lib.lib().skinny_paged_attn_workspace_bytes(batch, tokens, n_q, n_kv, head_dim, keys))
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
