@@ -815,7 +815,9 @@ int paged_blocks(int keys, int D) { return (keys + paged_block(D) - 1) / paged_b
 // up to 2000 (6144) 105 / 66 / 61; six tokens, 256 dims, 16 of up to 4000 (4032) 75 / 55 / 50. One token, 4 heads of 256
 // dims: 1 x 8192 (516) 17.1 / 17.3 / 25.5, 8 x 4000 (2016) 30.8 / 29.0 / 28.4, 32 x 2000 (4096) 59 / 52 / 50; 9 of up to
 // 5003, 3 tokens (2880) 37 / 37 / 44. 8 heads of 64 dims: 1 x 8192 11.5 / 13.7 / 20.9, 16 x 2000 19.3 / 18.2 / 22.9, 64 x
-// 4000 92 / 93 / 101, 64 x 8000 (32256) 207 / 190 / 189.
+// 4000 92 / 93 / 101, 64 x 8000 (32256) 207 / 190 / 189. 64 dims have no threshold of their own, so that the rule takes groups
+// for the last but one, the slowest of the three there. The blocks are those of the host's bound: short sequences under a
+// large bound are cut as long ones are (32 of up to 2048 keys: 35 us, under a bound 8 times as large 45).
 int paged_span(int B, int Hkv, int nblk, int rows, int D) {
   const int64_t heads = (int64_t)B * Hkv, all = heads * nblk;
   const bool heavy = rows > 16;
