@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define SKINNY_ABI_VERSION 22
+#define SKINNY_ABI_VERSION 23
 
 /* Error codes. */
 #define SKINNY_OK 0
@@ -591,6 +591,43 @@ size_t skinny_paged_attn_workspace_bytes(int B, int T, int Hq, int Hkv, int D, i
 int skinny_paged_attention_bf16(const uint16_t* q, int B, int T, int Hq, const skinny_paged_kv* kv, int keys, float scale,
                                 const uint16_t* gate, int64_t ld_gate, int gate_stride, void* workspace,
                                 size_t workspace_bytes, uint16_t* out, void* stream);
+/* The same attention where all sequences begin with one prefix, whose keys are read once for the batch:
+ * *prefix tokens in the pages prefix_pages[0 .. max_prefix_pages - 1] of the same cache; kv's lengths,
+ * counts and pages are of each sequence's own tokens after it. Row b*T + t sees the prefix and its own
+ * positions <= lengths[b] + t. prefix_keys is the host's bound on *prefix (at most max_prefix_pages *
+ * page); a prefix outside [0, prefix_keys] or with a page that is none makes the rows NaN. Values and
+ * scores that are not finite as above, and the same limits. A row's bits do not depend on the other sequences, but on B, T
+ * and the bounds, which cut the prefix. The workspace is always needed. */
+size_t skinny_paged_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys);
+int skinny_paged_attention_shared_bf16(const uint16_t* q, int B, int T, int Hq, const skinny_paged_kv* kv,
+                                       const int32_t* prefix, const int32_t* prefix_pages, int max_prefix_pages,
+                                       int prefix_keys, int keys, float scale, const uint16_t* gate, int64_t ld_gate,
+                                       int gate_stride, void* workspace, size_t workspace_bytes, uint16_t* out,
+                                       void* stream);
+/* The Gated-DeltaNet mixer of the same batch (counterparts of skinny_gdn_conv_silu and
+ * skinny_gdn_recurrence for one sequence). States lie in a pool, `stride` elements from one to the
+ * next: sequence b begins with state slots[b] (-1: zeros) and the one after its counts[b] tokens goes to
+ * slots_out[b] (NULL: to slots[b]), of a sequence without tokens the state as it was. States that are
+ * only read may be shared, such as the one after a prefix that the sequences have in common; one
+ * that the call writes stands once in slots_out and no other sequence reads it. A sequence with a
+ * state outside the pool or a count outside [0, T] has NaN rows and writes none. Padding rows are zero. */
+typedef struct {
+  const int32_t* slots;      /* [B] */
+  const int32_t* slots_out;  /* [B] or NULL */
+  const int32_t* counts;     /* [B] or NULL: T each */
+  int n_slots;
+  int64_t stride;
+} skinny_state_pool;
+/* x [B*T] rows of C channels (stride ldx), conv_state [n_slots][KW-1][C] bf16, weight [C][KW], KW = 4; out
+ * [B*T] rows (stride ldo). Each sequence's rows and state have skinny_gdn_conv_silu's bits. out overlaps no
+ * input. B and T at most 65535. */
+int skinny_gdn_conv_silu_batch(const uint16_t* x, int64_t ldx, int B, int T, int C, int KW, const skinny_state_pool* pool,
+                               uint16_t* conv_state, const uint16_t* weight, uint16_t* out, int64_t ldo, void* stream);
+/* Rows, gates and heads as skinny_gdn_recurrence takes them; state [n_slots][H][Dv][Dk] fp32 (16-byte aligned, stride
+ * a multiple of 4), y fp32 [B*T][H][Dv]. */
+int skinny_gdn_recurrence_batch(const uint16_t* qkv, int64_t ldq, const uint16_t* b, const uint16_t* a, int64_t ldab,
+                                const float* A_log, const float* dt_bias, int B, int T, const skinny_state_pool* pool,
+                                float* state, float* y, int H, int Hk, int Dk, int Dv, void* stream);
 /* For each bf16 row of scores (V <= 524288, row stride ld), with the distribution softmax(row / T):
  * logprob = ln p(tokens[row]) (-inf for a token outside [0, V)), entropy = -sum p ln p (nats), and
  * the `top` <= 32 most probable tokens (decreasing, ties by index, NaN scores last) with their

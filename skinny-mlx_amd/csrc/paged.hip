@@ -11,13 +11,13 @@
 // call and brings counts[b] of at most T new ones, at positions lengths[b] + t; position p lives in slot
 // p % P of page pages[b][p / P].
 #include <type_traits>
-#include "common.h"
+#include "paged.h"
+
+using namespace paged;
 
 namespace {
 
 constexpr int kPMaxRuns = 65535;  // runs of a sequence: a grid's last index
-constexpr float kPLog2e = 1.4426950408889634f;
-constexpr int kPMaxRows = 64;  // query rows per kv head: T x (Hq / Hkv)
 
 // A block's keys, and the waves that share it: 64 KB of K and V for 128 and 256 dims, a wave's part of which is 64 registers.
 __host__ __device__ constexpr int paged_block(int D) { return D == 256 ? 64 : 128; }
@@ -25,39 +25,6 @@ __host__ __device__ constexpr int paged_waves(int D) { return D == 64 ? 2 : 4; }
 constexpr int kPQuad = 4;      // blocks joined left to right
 constexpr int kPLanes = 8;     // running joins of groups in the merge
 constexpr int kPGroup = 8;     // blocks whose quads are joined left to right
-
-// Memory that this kernel only reads, for uniform addresses: loaded into scalar registers.
-typedef const __attribute__((address_space(4))) int32_t* words_t;
-__device__ __forceinline__ words_t words(const int32_t* p) { return (words_t)(uintptr_t)p; }
-
-struct Pages {
-  const int32_t* lengths;
-  const int32_t* counts;  // null: T each
-  const int32_t* table;   // [B][>= max_pages], row stride ld
-  uint16_t* k;
-  uint16_t* vt;
-  uint32_t k_stride, vt_stride;  // elements from page to page
-  int ld, max_pages, n_pages, log2p;
-};
-
-// A sequence's cached length and new tokens. `ok` is false where they cannot be: a negative length, a count
-// outside [0, T], or more tokens than `room` slots.
-struct Sequence {
-  int len, count;
-  bool ok;
-};
-__device__ __forceinline__ Sequence sequence_of(const Pages& pg, int b, int T, int room) {
-  const int len = words(pg.lengths)[b], count = pg.counts ? words(pg.counts)[b] : T;
-  return {len, count, len >= 0 && count >= 0 && count <= T && count <= room && len <= room - count};
-}
-
-constexpr uint16_t kNanBits = 0x7fc0;
-
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
-}
 
 // ---------------------------------------------------------------------------------------------------------
 // New rows into the cache. A wave takes 64 / (D / 8) query or key heads of a token, eight dims a lane; or 64 value dims of
@@ -247,56 +214,6 @@ __global__ __launch_bounds__(256) void paged_store_kernel(Pages pg, StoreRows ro
 // positions of the sequence, and keys that a row does not see add exact zeros, so a row's bits depend on its own sequence
 // and position alone: not on the batch, on T, on who joins the blocks, or on where the pages lie.
 
-// The first n (0 to 8) of eight consecutive keys' values, the others zero.
-__device__ __forceinline__ u32x4_t first_keys(u32x4_t v, int n) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) v[w] &= n >= 2 * w + 2 ? ~0u : n == 2 * w + 1 ? 0xffffu : 0u;
-  return v;
-}
-
-struct Out {
-  uint16_t* out;
-  const uint16_t* gate;  // null: none
-  int64_t ldg;           // elements from row to row
-  int gs;                // and from head to head
-};
-
-// One output value, divided by the sum of its weights, gated, rounded. Sums that are not finite end here as one NaN: a value
-// that is not finite leaves an infinity or a NaN, by the sign of its weight's second term, which the joins keep (times a
-// factor that is no 0 or, of 0, as NaN). A compare and a select per value; no block pays for it.
-__device__ __forceinline__ uint16_t finished(float o, float inv, bool gated, uint32_t gate) {
-  o *= inv;
-  const bool finite = fabsf(o) < INFINITY;
-  if (gated) o *= __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(bf16_bits_to_f32(gate) * -kPLog2e));
-  return finite ? f32_to_bf16_bits(o) : kNanBits;
-}
-
-// Part (m, l, o) of a row joined to the parts before it: their factor and its own.
-struct Join {
-  float before, part;
-};
-__device__ __forceinline__ Join join(float& m, float& l, float pm, float pl) {
-  const float mm = fmaxf(m, pm), ref = mm == -INFINITY ? 0.f : mm;
-  const Join j{__builtin_amdgcn_exp2f(m - ref), __builtin_amdgcn_exp2f(pm - ref)};
-  m = mm;
-  l = fmaf(pl, j.part, l * j.before);
-  return j;
-}
-
-// The larger of, and the sum over, the four quads' values of a column, in every lane.
-__device__ __forceinline__ float quads_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float quads_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // W tiles of 16 query rows; a call of more rows per kv head than 32 (kHalves) takes two workgroups a run, the second
 // of which finds K and V in the caches. by_g: 65536 / G rounded up, G = Hq / Hkv. GS: keys of a block that share a page: the
 // page size where that is 16 or 32, else 64.
@@ -310,7 +227,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
                                                                              int G, int by_g, int Hq, int Hkv, int room,
                                                                              float scale, int span, int slots,
                                                                              float* __restrict__ part_o,
-                                                                             float* __restrict__ part_ml, Out o) {
+                                                                             float* __restrict__ part_ml, Out o, int first) {
   constexpr int BLK = paged_block(D), WAVES = paged_waves(D);
   constexpr int KT = BLK / 16 / WAVES, KS = D / 32;           // a wave's 16-key tiles; dim steps of a score
   constexpr int ST = BLK / 32, NG = BLK / GS;                 // a block's 32-key steps and pages
@@ -361,9 +278,9 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
   find(c0);
   const Sequence sq = sequence_of(pg, b, T, room);
   if (slots == 1 && row0 == 0) {  // no merge follows: the rows that are no tokens are written here
-    const int first = sq.ok ? sq.count : 0;
-    for (int e = threadIdx.x; e < (T - first) * G * D; e += 64 * WAVES) {
-      const int t = first + e / (G * D);
+    const int live = sq.ok ? sq.count : 0;
+    for (int e = threadIdx.x; e < (T - live) * G * D; e += 64 * WAVES) {
+      const int t = live + e / (G * D);
       o.out[(((size_t)b * T + t) * Hq + h * G) * D + e % (G * D)] = sq.ok ? 0 : kNanBits;
     }
   }
@@ -645,7 +562,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
     const int r = row0 + 16 * w + col, d0 = wave * 16 * DW + quad * 4;
     if (r >= rows) continue;
     if (slots > 1) {  // a part, for the merge
-      const size_t at = (((size_t)b * Hkv + h) * slots + slot) * (size_t)(T * G) + r;
+      const size_t at = (((size_t)b * Hkv + h) * slots + first + slot) * (size_t)(T * G) + r;
 #pragma unroll
       for (int dt = 0; dt < DW; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * D + d0 + dt * 16) = go[w][dt];
       if (wave == 0 && quad == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{gm[w], gl[w]};
@@ -834,43 +751,14 @@ size_t paged_workspace(int B, int T, int Hq, int Hkv, int D, int keys) {
   return (size_t)B * Hkv * slots * T * (Hq / Hkv) * (D + 2) * sizeof(float);
 }
 
-bool head_dim_ok(int D) { return D == 64 || D == 128 || D == 256; }
-
-// What both entry points ask of the cache; sets `pg`.
-int check_pages(const skinny_paged_kv* kv, int B, int T, int Hq, Pages& pg, const char* what) {
-  SKINNY_CHECK_ARG(kv && kv->lengths && kv->pages && kv->k_pages && kv->vt_pages, "%s: null pointer", what);
-  SKINNY_CHECK_ARG(head_dim_ok(kv->head_dim), "%s: head dim %d unsupported (64, 128 or 256)", what, kv->head_dim);
-  SKINNY_CHECK_ARG(kv->n_kv >= 1 && kv->n_kv <= 32767 && Hq >= kv->n_kv && Hq <= 65535 && Hq % kv->n_kv == 0,
-                   "%s: Hq=%d must be a multiple of Hkv=%d", what, Hq, kv->n_kv);
-  SKINNY_CHECK_ARG(B >= 1 && B <= 65535 && T >= 1 && T <= 65535, "%s: B=%d sequences of T=%d tokens (1 to 65535 each)",
-                   what, B, T);
-  const int P = kv->page;
-  SKINNY_CHECK_ARG(P >= 16 && P <= 256 && (P & (P - 1)) == 0, "%s: page=%d slots (a power of two, 16 to 256)", what, P);
-  SKINNY_CHECK_ARG(kv->n_pages >= 1 && kv->max_pages >= 1 && kv->ld_pages >= kv->max_pages &&
-                       (int64_t)kv->max_pages * P <= (1 << 30),
-                   "%s: n_pages=%d, max_pages=%d, ld_pages=%d", what, kv->n_pages, kv->max_pages, kv->ld_pages);
-  const int64_t need = (int64_t)kv->n_kv * P * kv->head_dim;
-  SKINNY_CHECK_ARG(kv->k_stride >= need && kv->vt_stride >= need && kv->k_stride % 8 == 0 && kv->vt_stride % 8 == 0 &&
-                       kv->k_stride <= INT32_MAX && kv->vt_stride <= INT32_MAX,
-                   "%s: page strides %lld, %lld (multiples of 8 below 2^31, at least Hkv*P*D=%lld)", what,
-                   (long long)kv->k_stride, (long long)kv->vt_stride, (long long)need);
-  SKINNY_CHECK_ARG(skinny_aligned(kv->k_pages, 16) && skinny_aligned(kv->vt_pages, 16) && skinny_aligned(kv->lengths, 4) &&
-                       skinny_aligned(kv->counts, 4) && skinny_aligned(kv->pages, 4),
-                   "%s: misaligned cache", what);
-  pg = Pages{kv->lengths, kv->counts, kv->pages, kv->k_pages, kv->vt_pages, (uint32_t)kv->k_stride, (uint32_t)kv->vt_stride,
-             kv->ld_pages, kv->max_pages, kv->n_pages, __builtin_ctz(P)};
-  return SKINNY_OK;
-}
-
+// The blocks of `runs` runs, as parts in the slots from `first` on of `slots`, or (one slot) as outputs.
 template <int D>
-int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, float* ws,
-                           const Out& o, hipStream_t s) {
+int launch_blocks(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, int span, int runs,
+                  int first, int slots, float* part_o, float* part_ml, const Out& o, hipStream_t s) {
   const int G = Hq / Hkv, rows = T * G;
-  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows, D), slots = paged_slots(nblk, span);
-  float* ml = ws + (size_t)B * Hkv * slots * rows * D;
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(rows > 32 ? 2 * Hkv : Hkv, B, slots), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G,
-                       65535 / G + 1, Hq, Hkv, keys, scale, span, slots, ws, ml, o);
+    hipLaunchKernelGGL(kernel, dim3(rows > 32 ? 2 * Hkv : Hkv, B, runs), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G,
+                       65535 / G + 1, Hq, Hkv, keys, scale, span, slots, part_o, part_ml, o, first);
   };
   auto page = [&](auto w, auto h) {
     constexpr int W = decltype(w)::value;
@@ -882,7 +770,16 @@ int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int
   if (rows <= 16) page(std::integral_constant<int, 1>{}, std::false_type{});
   else if (rows <= 32) page(std::integral_constant<int, 2>{}, std::false_type{});
   else page(std::integral_constant<int, 2>{}, std::true_type{});
-  if (const int rc = skinny_check_launch("paged_attention")) return rc;
+  return skinny_check_launch("paged_attention");
+}
+
+template <int D>
+int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, float* ws,
+                           const Out& o, hipStream_t s) {
+  const int G = Hq / Hkv, rows = T * G;
+  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows, D), slots = paged_slots(nblk, span);
+  float* ml = ws + (size_t)B * Hkv * slots * rows * D;
+  if (const int rc = launch_blocks<D>(pg, q, B, T, Hq, Hkv, keys, scale, span, slots, 0, slots, ws, ml, o, s)) return rc;
   if (slots == 1) return SKINNY_OK;
   const int groups = (nblk + kPGroup - 1) / kPGroup;
   // eight waves a row where the rows alone would not fill the card, and always for blocks
@@ -900,6 +797,25 @@ int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int
 }
 
 }  // namespace
+
+namespace paged {
+
+Own own_runs(int B, int T, int Hq, int Hkv, int D, int keys) {
+  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, T * (Hq / Hkv), D);
+  return {span, paged_slots(nblk, span), paged_block(D)};
+}
+
+int own_parts(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int D, int keys, float scale, int first,
+              int slots, float* part_o, float* part_ml, hipStream_t s) {
+  const Own own = own_runs(B, T, Hq, Hkv, D, keys);
+  const Out none{nullptr, nullptr, 0, 0};
+  auto go = [&](auto launch) {
+    return launch(pg, q, B, T, Hq, Hkv, keys, scale, own.span, own.slots, first, slots, part_o, part_ml, none, s);
+  };
+  return D == 64 ? go(launch_blocks<64>) : D == 128 ? go(launch_blocks<128>) : go(launch_blocks<256>);
+}
+
+}  // namespace paged
 
 extern "C" int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int T, int Hq, int q_stride, int k_offset,
                                        int v_offset, const uint16_t* q_norm, const uint16_t* k_norm, float eps,

@@ -1,0 +1,479 @@
+// Attention of sequences that begin with one prefix, in a cache in pages: the prefix's keys and values are read once for
+// the whole batch, whose query rows then make matrix products of them, where paged.hip reads each sequence's own.
+//
+// No reference counterpart: the reference decodes one sequence (skinny_mlx/spec.py:98-156). Arithmetic of a layer as at
+// spec.py:24-29 (causal GQA attention, optionally output * sigmoid(gate)).
+//
+// A row's softmax over [the prefix; its own keys] is joined from parts: runs of the prefix's keys (prefix_kernel here, for all
+// rows), runs of its sequence's own blocks (paged.hip's kernel, unchanged), and a merge.
+#include <type_traits>
+#include "paged.h"
+
+using namespace paged;
+
+namespace {
+
+struct Prefix {
+  const int32_t* length;
+  const int32_t* pages;
+  int max_pages, room;
+};
+
+// The keys that the call may read, -1 where the length cannot be.
+__device__ __forceinline__ int prefix_length(const Prefix& p) {
+  const int n = words(p.length)[0];
+  return n >= 0 && n <= p.room ? n : -1;
+}
+
+// A workgroup of four waves takes 16 * RT * 4 / KW query rows of a kv head (every sequence's, one after the other) and a run of
+// the prefix: 4 / KW groups of 16 * RT rows, in each of which KW waves share a tile's keys. A tile of keys is staged in LDS in
+// the matrix cores' operand order (a lane's 16 bytes after its neighbour's: no bank conflicts) and read by all the row groups;
+// the next tile's loads are in flight meanwhile. Scores are formed transposed, S^T = K Q^T, with the K rows of a 32-key step
+// taken so that a lane holds eight consecutive keys of one query row, which is the operand that O^T = V^T P^T wants: P never
+// leaves its lane.
+//
+// P is rounded to bf16 (2^-9 of a weight) and its sum is taken of the rounded weights, so that the error is of the differences
+// between values only. The running maximum is raised only where a score passes it by 2^8: until then weights up to 2^8
+// are as exact, and the outputs need no rescaling.
+template <int D>
+struct Shape {
+  static constexpr int KS = D / 32;   // dim steps of a score
+  static constexpr int DT = D / 16;   // dim tiles of an output
+};
+
+constexpr float kLag = 8.f;
+
+template <int D, int KW>
+__host__ __device__ constexpr int tile_keys() {
+  return 32 * (KW > 2 ? KW : 2);
+}
+
+template <int D, int RT, int KW>
+__host__ __device__ constexpr int prefix_lds() {
+  const int tiles = 2 * 2 * tile_keys<D, KW>() * D * 2;                         // K and V, two buffers
+  const int join = KW > 1 ? 4 * 16 * RT * (D + 4) * 4 + 4 * 16 * RT * 2 * 4 : 0;  // the waves' outputs, maxima and sums
+  return tiles > join ? tiles : join;
+}
+
+template <int D, int RT, int KW>
+__global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, const uint16_t* __restrict__ q, int rows, int TG,
+                                                        int G, int Hq, int Hkv, float scale, int span, int slots,
+                                                        float* __restrict__ part_o, float* __restrict__ part_ml) {
+  constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, TK = tile_keys<D, KW>();
+  constexpr int ST = TK / 32;        // 32-key steps of a tile
+  constexpr int NF = TK * D / 512;   // 1 KB operands of K, and of V, in a tile
+  constexpr int FW = NF / 4;         // a wave's share of them
+  extern __shared__ u32x4_t lds[];   // [buffer][K operands, V operands][lane]
+  const int h = blockIdx.x, slot = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
+  const int kw = wave % KW, row0 = ((int)blockIdx.y * (4 / KW) + wave / KW) * (16 * RT);
+  const int len = prefix_length(px);
+  const int begin = slot * span, end = min(begin + span, len);
+  if (begin >= end) return;
+  const float sc = scale * kPLog2e;
+  // a flat row's sequence and row of that sequence's T * G
+  auto row_of = [&](int r, int& b, int& in) {
+    b = r / TG;
+    in = r - b * TG;
+  };
+  bf16x8_t qf[RT][KS];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int b, in;
+    row_of(min(row0 + 16 * rt + col, rows - 1), b, in);
+    const int t = in / G;
+    const uint16_t* qp = q + (((size_t)b * (TG / G) + t) * Hq + h * G + in - t * G) * D + quad * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
+  }
+  const int P = 1 << pg.log2p;
+  const uint16_t* k_head = pg.k + (size_t)h * P * D;
+  const uint16_t* v_head = pg.vt + (size_t)h * D * P;
+  u32x4_t kr[FW], vr[FW];
+  // Operand f of a tile's K: step f / (2 KS), half a of its keys, dims 32 ks on. Row r of the half's product is key
+  // 8 (r / 4) + 4a + r % 4 of the step. Of its V: step f / DT, dims 16 dt on.
+  auto page_at = [&](int key, bool& bad) {  // of a key below the tile's end; past the prefix: any page that is one
+    const int id = words(px.pages)[min(key >> pg.log2p, px.max_pages - 1)];
+    const bool ok = (unsigned)id < (unsigned)pg.n_pages;
+    bad = !ok && key < len;
+    return ok ? id : 0;
+  };
+  auto load = [&](int key0) {
+#pragma unroll
+    for (int i = 0; i < FW; ++i) {
+      const int f = wave * FW + i;
+      {
+        const int s = f / (2 * KS), a = f / KS % 2, ks = f % KS;
+        const int step = key0 + 32 * s;
+        bool bad0, bad1;
+        const int p0 = page_at(step, bad0), p1 = page_at(step + 16, bad1);
+        const bool second = col >= 8;
+        const int in = (step + 8 * (col >> 2) + 4 * a + (col & 3)) & (P - 1);
+        const uint16_t* at = k_head + (uint64_t)(uint32_t)(second ? p1 : p0) * pg.k_stride + (uint32_t)(in * D + ks * 32 + quad * 8);
+        u32x4_t v = *reinterpret_cast<const u32x4_t*>(at);
+        if (second ? bad1 : bad0) v = u32x4_t{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+        kr[i] = v;
+      }
+      {
+        const int s = f / DT, dt = f % DT;
+        const int step = key0 + 32 * s;
+        bool bad0, bad1;
+        const int p0 = page_at(step, bad0), p1 = page_at(step + 16, bad1);
+        const bool second = quad >= 2;
+        const int key = step + 8 * quad;
+        const uint16_t* at = v_head + (uint64_t)(uint32_t)(second ? p1 : p0) * pg.vt_stride + (uint32_t)((dt * 16 + col) * P + (key & (P - 1)));
+        vr[i] = first_keys(*reinterpret_cast<const u32x4_t*>(at), (second ? bad1 : bad0) ? 0 : min(max(len - key, 0), 8));
+      }
+    }
+  };
+  auto stage = [&](int buf) {
+    u32x4_t* to = lds + (size_t)buf * 2 * NF * 64;
+#pragma unroll
+    for (int i = 0; i < FW; ++i) {
+      to[(wave * FW + i) * 64 + lane] = kr[i];
+      to[(NF + wave * FW + i) * 64 + lane] = vr[i];
+    }
+  };
+  float m[RT], l[RT];
+  f32x4_t o[RT][DT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  load(begin);
+  stage(0);
+  __syncthreads();
+  for (int key0 = begin, buf = 0; key0 < end; key0 += TK, buf ^= 1) {
+    const bool more = key0 + TK < end;
+    if (more) load(key0 + TK);
+    const u32x4_t* kt = lds + (size_t)buf * 2 * NF * 64 + lane;
+    const u32x4_t* vt = kt + NF * 64;
+#pragma unroll
+    for (int s0 = 0; s0 < ST / KW; ++s0) {
+      const int s = s0 * KW + kw;
+      f32x4_t acc[RT][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, kt[((s * 2 + a) * KS + ks) * 64]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[rt][a] = mfma16x16x32(kf, qf[rt][ks], acc[rt][a]);
+        }
+      const int left = end - (key0 + 32 * s + 8 * quad);  // of the lane's eight keys, those below the run's end
+      if (key0 + 32 * s + 32 > end) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e >= left) acc[rt][e >> 2][e & 3] = -INFINITY;
+      }
+      float top[RT];
+      bool up = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float mx = acc[rt][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, acc[rt][e >> 2][e & 3]);
+        top[rt] = mx * sc;
+        up |= top[rt] > m[rt] + kLag;
+      }
+      if (__any(up)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float nm = fmaxf(m[rt], quads_max(top[rt]));
+          const float f = __builtin_amdgcn_exp2f(m[rt] - (nm == -INFINITY ? 0.f : nm));
+          m[rt] = nm;
+          l[rt] *= f;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[rt][dt][i] *= f;
+        }
+      }
+      bf16x8_t pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float ref = m[rt] == -INFINITY ? 0.f : m[rt];
+        u32x4_t p;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(acc[rt][w >> 1][2 * (w & 1)], sc, -ref));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(acc[rt][w >> 1][2 * (w & 1) + 1], sc, -ref));
+          p[w] = two_bf16(p0, p1);
+          l[rt] += __uint_as_float(p[w] << 16);
+          l[rt] += __uint_as_float(p[w] & 0xffff0000u);
+        }
+        pf[rt] = __builtin_bit_cast(bf16x8_t, p);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, vt[(s * DT + dt) * 64]);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma16x16x32(vf, pf[rt], o[rt][dt]);
+      }
+    }
+    if (more) stage(buf ^ 1);
+    __syncthreads();
+  }
+  auto part_at = [&](int r) {
+    int b, in;
+    row_of(r, b, in);
+    return (((size_t)b * Hkv + h) * slots + slot) * (size_t)TG + in;
+  };
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) l[rt] = quads_sum(l[rt]);
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = row0 + 16 * rt + col;
+      if (r >= rows) continue;
+      const size_t at = part_at(r);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * D + dt * 16 + quad * 4) = o[rt][dt];
+      if (quad == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{m[rt], l[rt]};
+    }
+  } else {
+    // The KW waves of a row group joined in their order.
+    float* sum = reinterpret_cast<float*>(lds);                       // [wave][16 RT][D + 4]
+    float2* ml = reinterpret_cast<float2*>(sum + 4 * 16 * RT * (D + 4));  // [wave][16 RT]
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float* mine = sum + ((size_t)wave * 16 * RT + 16 * rt + col) * (D + 4);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(mine + dt * 16 + quad * 4) = o[rt][dt];
+      if (quad == 0) ml[wave * 16 * RT + 16 * rt + col] = float2{m[rt], l[rt]};
+    }
+    __syncthreads();
+    const int group = wave / KW;
+    for (int i = kw * 64 + lane; i < 16 * RT * (D / 4); i += KW * 64) {
+      const int in = i / (D / 4), d = i % (D / 4) * 4, r = row0 + in;
+      if (r >= rows) continue;
+      float rm = -INFINITY, rl = 0.f;
+      f32x4_t ro = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const int at = (group * KW + w) * 16 * RT + in;
+        const float2 x = ml[at];
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(sum + (size_t)at * (D + 4) + d);
+        const Join j = join(rm, rl, x.x, x.y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ro[e] = fmaf(v[e], j.part, ro[e] * j.before);
+      }
+      const size_t at = part_at(r);
+      *reinterpret_cast<f32x4_t*>(part_o + at * D + d) = ro;
+      if (d == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{rm, rl};
+    }
+  }
+}
+
+// The parts of a row joined: those of the prefix, then those of its own keys, part i by wave i % W of the row's W, the waves in
+// order. Bound by latency for few rows, by the parts' bytes for many.
+template <int D, int W>
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void shared_merge_kernel(Pages pg, Prefix px, int T, int Hq, int G, int Hkv,
+                                                                            int room, int span, int first, int own_keys,
+                                                                            int slots, const float* __restrict__ part_o,
+                                                                            const float* __restrict__ part_ml, Out o) {
+  constexpr int E = D / 64, UN = 8;
+  typedef float dims_t __attribute__((ext_vector_type(E)));
+  typedef uint16_t out_t __attribute__((ext_vector_type(E)));
+  __shared__ __attribute__((aligned(16))) float sum[W][W > 1 ? D : 4];
+  __shared__ float2 ml[W];
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  const int head = W > 1 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave, t = blockIdx.y, b = blockIdx.z;
+  if (head >= Hq) return;
+  const int w = W > 1 ? wave : 0;
+  const Sequence sq = sequence_of(pg, b, T, room);
+  const int len = prefix_length(px);
+  const size_t orow = (size_t)b * T + t;
+  out_t* op = reinterpret_cast<out_t*>(o.out + (orow * Hq + head) * D) + lane;
+  if (!sq.ok || len < 0 || t >= sq.count) {
+    const bool padding = sq.ok && t >= sq.count;
+    if (w == 0) *op = out_t(padding ? (uint16_t)0 : kNanBits);
+    return;
+  }
+  const int np = (len + span - 1) / span, n = np + (sq.len + t) / own_keys + 1;  // parts of the prefix; and of its own keys
+  const size_t step = (size_t)T * G;
+  const size_t base = ((size_t)b * Hkv + head / G) * slots * step + (size_t)t * G + head % G;
+  float rm = -INFINITY, rl = 0.f;
+  dims_t ro(0.f);
+  for (int i0 = w; i0 < n; i0 += W * UN) {
+    float2 x[UN];
+    dims_t v[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int i = min(i0 + u * W, n - 1);
+      const size_t at = base + (size_t)(i < np ? i : first + i - np) * step;
+      x[u] = reinterpret_cast<const float2*>(part_ml)[at];
+      v[u] = *reinterpret_cast<const dims_t*>(part_o + at * D + E * lane);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (i0 + u * W >= n) continue;
+      const Join j = join(rm, rl, x[u].x, x[u].y);
+#pragma unroll
+      for (int e = 0; e < E; ++e) ro[e] = fmaf(v[u][e], j.part, ro[e] * j.before);
+    }
+  }
+  if constexpr (W > 1) {
+    *reinterpret_cast<dims_t*>(&sum[w][E * lane]) = ro;
+    if (lane == 0) ml[w] = float2{rm, rl};
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int i = 1; i < W; ++i) {
+      const dims_t v = *reinterpret_cast<const dims_t*>(&sum[i][E * lane]);
+      const Join j = join(rm, rl, ml[i].x, ml[i].y);
+#pragma unroll
+      for (int e = 0; e < E; ++e) ro[e] = fmaf(v[e], j.part, ro[e] * j.before);
+    }
+  }
+  const uint16_t* gp = o.gate ? o.gate + (int64_t)orow * o.ldg + (int64_t)head * o.gs + E * lane : nullptr;
+  const float inv = 1.f / rl;
+  out_t y;
+#pragma unroll
+  for (int e = 0; e < E; ++e) y[e] = finished(ro[e], inv, gp, gp ? gp[e] : 0);
+  *op = y;
+}
+
+// How the prefix is cut: row tiles a wave, waves that share a tile's keys, keys of a run (`span`) and runs (`slots`).
+struct Cut {
+  int rt, kw, row_blocks, span, slots;
+};
+
+Cut prefix_cut(int rows, int Hkv, int D, int prefix_keys) {
+  Cut c;
+  if (D == 256) {
+    c.rt = rows > 32 ? 2 : 1;
+    c.kw = rows > 64 ? 1 : 2;
+  } else {
+    c.rt = rows > 32 ? 4 : rows > 16 ? 2 : 1;
+    c.kw = rows > 128 ? 1 : rows > 64 ? 2 : 4;
+  }
+  const int block = 16 * c.rt * 4 / c.kw, tile = 32 * (c.kw > 2 ? c.kw : 2);
+  c.row_blocks = (rows + block - 1) / block;
+  const int tiles = (prefix_keys + tile - 1) / tile;
+  int64_t runs = 256 / ((int64_t)Hkv * c.row_blocks);
+  if (runs < 1) runs = 1;
+  c.span = (int)((tiles + runs - 1) / runs) * tile;
+  c.slots = (prefix_keys + c.span - 1) / c.span;
+  return c;
+}
+
+struct Plan {
+  Cut cut;
+  Own own;
+  int slots;
+  size_t parts, bytes;
+};
+
+Plan plan_of(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys) {
+  Plan p;
+  const int G = Hq / Hkv;
+  p.cut = prefix_cut(B * T * G, Hkv, D, prefix_keys);
+  p.own = own_runs(B, T, Hq, Hkv, D, keys);
+  p.slots = p.cut.slots + p.own.slots;
+  p.parts = (size_t)B * Hkv * p.slots * T * G;
+  p.bytes = p.parts * (D + 2) * sizeof(float);
+  return p;
+}
+
+template <int D, int RT, int KW>
+int launch_prefix(const Pages& pg, const Prefix& px, const uint16_t* q, int B, int T, int Hq, int Hkv, float scale, const Plan& p,
+                  float* ws, float* ml, hipStream_t s) {
+  constexpr int bytes = prefix_lds<D, RT, KW>();
+  static_assert(bytes <= 160 * 1024, "a CU's LDS");
+  const int G = Hq / Hkv;
+  if (bytes > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_kernel<D, RT, KW>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return skinny_set_error(SKINNY_ELAUNCH, "paged_attention_shared: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL((prefix_kernel<D, RT, KW>), dim3(Hkv, p.cut.row_blocks, p.cut.slots), dim3(256), bytes, s, pg, px, q,
+                     B * T * G, T * G, G, Hq, Hkv, scale, p.cut.span, p.slots, ws, ml);
+  return skinny_check_launch("paged_attention_shared prefix");
+}
+
+template <int D>
+int launch_shared(const Pages& pg, const Prefix& px, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale,
+                  const Plan& p, float* ws, const Out& o, hipStream_t s) {
+  float* ml = ws + p.parts * D;
+  const Cut& c = p.cut;
+  auto prefix = [&](auto rt, auto kw) {
+    return launch_prefix<D, decltype(rt)::value, decltype(kw)::value>(pg, px, q, B, T, Hq, Hkv, scale, p, ws, ml, s);
+  };
+  using std::integral_constant;
+  int rc;
+  if constexpr (D == 256) {
+    if (c.kw == 1) rc = prefix(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+    else if (c.rt == 2) rc = prefix(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    else rc = prefix(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+  } else {
+    if (c.kw == 1) rc = prefix(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    else if (c.kw == 2) rc = prefix(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else if (c.rt == 4) rc = prefix(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    else if (c.rt == 2) rc = prefix(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+    else rc = prefix(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  }
+  if (rc) return rc;
+  if ((rc = own_parts(pg, q, B, T, Hq, Hkv, D, keys, scale, c.slots, p.slots, ws, ml, s))) return rc;
+  const bool split = (int64_t)B * T * Hq <= 1024;
+  auto merge = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(split ? 512 : 256), 0, s, pg, px, T, Hq, Hq / Hkv, Hkv,
+                       keys, c.span, c.slots, p.own.span * p.own.block, p.slots, ws, ml, o);
+  };
+  if (split) merge(shared_merge_kernel<D, 8>);
+  else merge(shared_merge_kernel<D, 1>);
+  return skinny_check_launch("paged_attention_shared merge");
+}
+
+}  // namespace
+
+extern "C" size_t skinny_paged_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys) {
+  if (B < 1 || B > 65535 || T < 1 || Hkv < 1 || Hq < Hkv || Hq > 65535 || Hq % Hkv || !head_dim_ok(D) || keys < 1 ||
+      prefix_keys < 1 || prefix_keys > (1 << 30) || keys > (1 << 30) || (int64_t)T * (Hq / Hkv) > kPMaxRows)
+    return 0;
+  return plan_of(B, T, Hq, Hkv, D, prefix_keys, keys).bytes;
+}
+
+extern "C" int skinny_paged_attention_shared_bf16(const uint16_t* q, int B, int T, int Hq, const skinny_paged_kv* kv,
+                                                  const int32_t* prefix, const int32_t* prefix_pages, int max_prefix_pages,
+                                                  int prefix_keys, int keys, float scale, const uint16_t* gate, int64_t ld_gate,
+                                                  int gate_stride, void* workspace, size_t workspace_bytes, uint16_t* out,
+                                                  void* stream) {
+  Pages pg;
+  const char* what = "paged_attention_shared";
+  if (const int rc = check_pages(kv, B, T, Hq, pg, what)) return rc;
+  const int D = kv->head_dim, Hkv = kv->n_kv;
+  SKINNY_CHECK_ARG(q && out && prefix && prefix_pages, "%s: null pointer", what);
+  SKINNY_CHECK_ARG((int64_t)T * (Hq / Hkv) <= kPMaxRows, "%s: %lld query rows per kv head, at most %d", what,
+                   (long long)T * (Hq / Hkv), kPMaxRows);
+  SKINNY_CHECK_ARG(keys >= 1 && keys <= kv->max_pages * kv->page, "%s: keys=%d, the pages hold %d", what, keys,
+                   kv->max_pages * kv->page);
+  SKINNY_CHECK_ARG(max_prefix_pages >= 1 && (int64_t)max_prefix_pages * kv->page <= (1 << 30) && prefix_keys >= 1 &&
+                       prefix_keys <= max_prefix_pages * kv->page,
+                   "%s: prefix_keys=%d, %d pages of a prefix", what, prefix_keys, max_prefix_pages);
+  SKINNY_CHECK_ARG(!gate || (gate_stride >= 0 && ld_gate >= 0), "%s: gate strides %lld, %d", what, (long long)ld_gate,
+                   gate_stride);
+  SKINNY_CHECK_ARG(skinny_aligned(q, 16) && skinny_aligned(out, 16) && skinny_aligned(gate, 2) && skinny_aligned(workspace, 16) &&
+                       skinny_aligned(prefix, 4) && skinny_aligned(prefix_pages, 4),
+                   "%s: misaligned buffer", what);
+  SKINNY_CHECK_ARG(scale > 0.f && scale <= 1e38f, "%s: scale=%g must be positive", what, (double)scale);
+  const Plan p = plan_of(B, T, Hq, Hkv, D, prefix_keys, keys);
+  SKINNY_CHECK_ARG(p.own.slots <= 65535 && p.cut.slots <= 65535 && p.cut.row_blocks <= 65535, "%s: keys=%d, prefix_keys=%d",
+                   what, keys, prefix_keys);
+  SKINNY_CHECK_ARG(workspace && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes, needs %zu", what,
+                   workspace ? workspace_bytes : (size_t)0, p.bytes);
+  const Prefix px{prefix, prefix_pages, max_prefix_pages, prefix_keys};
+  const Out o{out, gate, ld_gate, gate_stride};
+  float* ws = static_cast<float*>(workspace);
+  const hipStream_t s = (hipStream_t)stream;
+  if (D == 64) return launch_shared<64>(pg, px, q, B, T, Hq, Hkv, keys, scale, p, ws, o, s);
+  if (D == 128) return launch_shared<128>(pg, px, q, B, T, Hq, Hkv, keys, scale, p, ws, o, s);
+  return launch_shared<256>(pg, px, q, B, T, Hq, Hkv, keys, scale, p, ws, o, s);
+}

@@ -22,7 +22,7 @@ LIB_NAME = "libskinny_hip.so"
 # SKINNY_HIP_LIB names another build of the same library (the host-only sanitizer build the CPU
 # tests load); unset, the in-tree build next to this file.
 LIB_PATH = os.environ.get("SKINNY_HIP_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
@@ -64,6 +64,16 @@ class PagedKV(ctypes.Structure):
 
 
 _paged_p = ctypes.POINTER(PagedKV)
+
+
+class StatePool(ctypes.Structure):
+    """skinny_state_pool of include/skinny_hip.h."""
+
+    _fields_ = [("slots", ctypes.c_void_p), ("slots_out", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("n_slots", ctypes.c_int), ("stride", ctypes.c_int64)]
+
+
+_pool_p = ctypes.POINTER(StatePool)
 
 # name -> (restype, argtypes). Every symbol declared in include/skinny_hip.h is listed.
 SIGNATURES: dict[str, tuple] = {
@@ -193,6 +203,15 @@ SIGNATURES: dict[str, tuple] = {
     "skinny_paged_attn_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "skinny_paged_attention_bf16": (_c_int, [_c_void_p, _c_int, _c_int, _c_int, _paged_p, _c_int, _c_float, _c_void_p,
                                              _c_i64, _c_int, _c_void_p, _c_size_t, _c_void_p, _c_void_p]),
+    "skinny_paged_attn_shared_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "skinny_paged_attention_shared_bf16": (_c_int, [_c_void_p, _c_int, _c_int, _c_int, _paged_p, _c_void_p, _c_void_p, _c_int,
+                                                    _c_int, _c_int, _c_float, _c_void_p, _c_i64, _c_int, _c_void_p,
+                                                    _c_size_t, _c_void_p, _c_void_p]),
+    "skinny_gdn_conv_silu_batch": (_c_int, [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _pool_p, _c_void_p,
+                                            _c_void_p, _c_void_p, _c_i64, _c_void_p]),
+    "skinny_gdn_recurrence_batch": (_c_int, [_c_void_p, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_void_p, _c_int,
+                                             _c_int, _pool_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                                             _c_void_p]),
     "skinny_token_logprobs_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int]),
     "skinny_token_logprobs_bf16": (_c_int, [_c_void_p, _c_int, _c_int, _c_i64, _c_void_p, _c_float, _c_int, _c_void_p,
                                             _c_size_t, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),

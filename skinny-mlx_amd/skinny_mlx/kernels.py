@@ -483,6 +483,75 @@ def paged_attention(q: torch.Tensor, lengths: torch.Tensor, pages: torch.Tensor,
     return o
 
 
+def paged_attn_shared_workspace(batch: int, tokens: int, n_q: int, n_kv: int, head_dim: int, prefix_keys: int, keys: int,
+                                device) -> torch.Tensor:
+    """Workspace of paged_attention_shared for calls of these sizes, with paged_attn_workspace's rules."""
+    nbytes = int(_lib.lib().skinny_paged_attn_shared_workspace_bytes(batch, tokens, n_q, n_kv, head_dim, prefix_keys, keys))
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+
+
+def paged_attention_shared(q: torch.Tensor, prefix: torch.Tensor, prefix_pages: torch.Tensor, lengths: torch.Tensor,
+                           pages: torch.Tensor, k_pages: torch.Tensor, vt_pages: torch.Tensor, scale: float,
+                           counts: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                           prefix_keys: int | None = None, keys: int | None = None, workspace: torch.Tensor | None = None,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attention of sequences that all begin with one prefix, which is read once for the batch
+    (skinny_paged_attention_shared_bf16): prefix int32 [1], the prefix's tokens, its keys and values in the pages
+    prefix_pages (int32 [n]) of the same cache; lengths, counts and pages are of the sequences' own tokens after it, so
+    row b*T + t sees the prefix and its own positions <= lengths[b] + t. The own pages begin with a page's first slot
+    wherever the prefix ends; paged_store takes the RoPE table from the prefix's end on (table[prefix:]).
+
+    prefix_keys: the host's bound on the prefix's tokens (None: what prefix_pages hold). workspace: from
+    paged_attn_shared_workspace (None: allocated for the call). Everything else as in paged_attention; a prefix past its
+    bound, or a page of it that is none, makes the rows NaN. A row's bits do not depend on the other sequences, but on the
+    sizes of the call, which cut the prefix."""
+    if not (q.is_cuda and q.dtype == BF16 and q.dim() == 3 and q.is_contiguous() and q.numel() > 0):
+        raise ValueError("q must be contiguous bf16 [B*T, Hq, D] on the GPU")
+    dev = q.get_device()
+    kv, b = _paged_kv(dev, lengths, counts, pages, k_pages, vt_pages)
+    rows, hq, d = q.shape
+    if d != kv.head_dim:
+        raise ValueError(f"pages of {kv.head_dim}-dim heads, q has {d}")
+    if rows % b:
+        raise ValueError(f"{rows} rows do not divide into {b} sequences")
+    if not _fits(prefix, torch.int32, (1,), dev):
+        raise ValueError("prefix must be int32 [1] on q's device")
+    if not (prefix_pages.dtype == torch.int32 and prefix_pages.dim() == 1 and prefix_pages.is_contiguous()
+            and prefix_pages.numel() > 0 and prefix_pages.get_device() == dev):
+        raise ValueError("prefix_pages must be contiguous int32 [n] on q's device")
+    gate_row = gate_head = 0
+    if gate is not None:
+        if not (gate.dtype == BF16 and gate.shape == (rows, hq, d) and gate.get_device() == dev and gate.stride(2) == 1
+                and gate.stride(1) < 2 ** 31):
+            raise ValueError(f"gate must be bf16 [{rows}, {hq}, {d}] with contiguous dims")
+        gate_row, gate_head, _ = gate.stride()
+    room, front = kv.max_pages * kv.page, prefix_pages.numel() * kv.page
+    if keys is None:
+        keys = room
+    elif not 1 <= keys <= room:
+        raise ValueError(f"keys={keys}: a row of pages holds {room}")
+    if prefix_keys is None:
+        prefix_keys = front
+    elif not 1 <= prefix_keys <= front:
+        raise ValueError(f"prefix_keys={prefix_keys}: prefix_pages hold {front}")
+    if out is not None and not _fits(out, BF16, (rows, hq * d), dev):
+        raise ValueError(f"out must be contiguous bf16 [{rows}, {hq * d}]")
+    if workspace is not None and not (workspace.is_contiguous() and workspace.get_device() == dev):
+        raise ValueError("workspace must be contiguous, on q's device")
+    with _on_device(q):
+        L = _lib.lib()
+        if workspace is None:
+            nbytes = L.skinny_paged_attn_shared_workspace_bytes(b, rows // b, hq, kv.n_kv, d, prefix_keys, keys)
+            workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        nbytes = workspace.numel() * workspace.element_size()
+        o = q.new_empty((rows, hq * d)) if out is None else out
+        _lib.check(L.skinny_paged_attention_shared_bf16(
+            q.data_ptr(), b, rows // b, hq, kv, prefix.data_ptr(), prefix_pages.data_ptr(), prefix_pages.numel(), prefix_keys,
+            keys, scale, _lib.ptr(gate), gate_row, gate_head, workspace.data_ptr(), nbytes, o.data_ptr(),
+            _lib.stream_of(q)), "paged_attention_shared")
+    return o
+
+
 _QKV_ATTN_OK: dict = {}
 
 
@@ -596,6 +665,105 @@ def gdn_recurrence_gated(qkv: torch.Tensor, b: torch.Tensor, a: torch.Tensor, A_
                                                            _lib.stream_of(qkv)),
                "gdn_recurrence_gated")
     return out
+
+
+def _state_pool(dev: int, state: torch.Tensor, slots: torch.Tensor, slots_out, counts) -> tuple["_lib.StatePool", int]:
+    """A pool of states and the sequences' places in it as the C side takes them, and the number of sequences; all on
+    device `dev`."""
+    n = state.shape[0]
+    if not (n > 0 and state.get_device() == dev):
+        raise ValueError("the pool of states must be on the rows' device and hold one at least")
+    stride = state.numel() // n
+    if not state.is_contiguous():
+        if not state[0].is_contiguous():
+            raise ValueError("a state must be contiguous")
+        if n > 1:
+            stride = state.stride(0)
+    if not (slots.dtype == torch.int32 and slots.dim() == 1 and slots.is_contiguous() and slots.get_device() == dev
+            and slots.numel() > 0):
+        raise ValueError("slots must be contiguous int32 [B] on the rows' device")
+    b = slots.numel()
+    if slots_out is not None and not _fits(slots_out, torch.int32, (b,), dev):
+        raise ValueError(f"slots_out must be contiguous int32 [{b}] on the rows' device")
+    if counts is not None and not _fits(counts, torch.int32, (b,), dev):
+        raise ValueError(f"counts must be contiguous int32 [{b}] on the rows' device")
+    return _lib.StatePool(slots.data_ptr(), _lib.ptr(slots_out), _lib.ptr(counts), n, stride), b
+
+
+def gdn_conv_silu_batch(x: torch.Tensor, conv_state: torch.Tensor, weight: torch.Tensor, slots: torch.Tensor,
+                        counts: torch.Tensor | None = None, slots_out: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """gdn_conv_silu of B sequences (skinny_gdn_conv_silu_batch): x bf16 [B*T, C], row b*T + t token t of sequence b;
+    conv_state bf16 [n_slots, KW-1, C], of which sequence b begins with slots[b] (-1: zeros) and leaves the one after its
+    tokens in slots_out[b] (None: in slots[b]) -> bf16 [B*T, C], each sequence's rows and state bitwise gdn_conv_silu's.
+
+    counts (int32 [B], None: T each) says how many of a sequence's T rows are tokens; the others are zero. A state that is
+    only read may be shared; one that is written stands once in slots_out and no other sequence reads it. A sequence with a
+    slot outside the pool or a count outside [0, T] comes out NaN and writes no state."""
+    if not (x.is_cuda and x.dtype == BF16 and x.dim() == 2 and x.stride(1) == 1):
+        raise ValueError("x must be a bf16 2-D GPU tensor")
+    dev = x.get_device()
+    rows, c = x.shape
+    if not (weight.dim() == 2 and _fits(weight, BF16, (c, weight.shape[1]), dev)):
+        raise ValueError(f"weight must be contiguous bf16 [{c}, KW] on x's device")
+    kw = weight.shape[1]
+    if not (conv_state.dtype == BF16 and conv_state.dim() == 3 and conv_state.shape[1:] == (kw - 1, c)):
+        raise ValueError(f"conv_state must be bf16 [n_slots, {kw - 1}, {c}]")
+    pool, b = _state_pool(dev, conv_state, slots, slots_out, counts)
+    if not (rows > 0 and rows % b == 0):
+        raise ValueError(f"{rows} rows do not divide into {b} sequences")
+    ld = c if rows == 1 else x.stride(0)
+    if ld < c:
+        raise ValueError("x rows overlap")
+    if out is not None and not _fits(out, BF16, (rows, c), dev):
+        raise ValueError(f"out must be contiguous bf16 [{rows}, {c}]")
+    with _on_device(x):
+        y = x.new_empty((rows, c)) if out is None else out
+        _lib.check(_lib.lib().skinny_gdn_conv_silu_batch(
+            x.data_ptr(), ld, b, rows // b, c, kw, pool, conv_state.data_ptr(), weight.data_ptr(), y.data_ptr(), c,
+            _lib.stream_of(x)), "gdn_conv_silu_batch")
+    return y
+
+
+def gdn_recurrence_batch(qkv: torch.Tensor, b: torch.Tensor, a: torch.Tensor, A_log: torch.Tensor, dt_bias: torch.Tensor,
+                         state: torch.Tensor, slots: torch.Tensor, n_heads: int, dk: int, dv: int,
+                         counts: torch.Tensor | None = None, slots_out: torch.Tensor | None = None,
+                         n_key_heads: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """gdn_recurrence of B sequences (skinny_gdn_recurrence_batch): qkv, b and a hold B*T rows, row b*T + t token t of
+    sequence b; state fp32 [n_slots, H, Dv, Dk], of which sequence b begins with slots[b] (-1: zeros) and leaves the one
+    after its tokens in slots_out[b] (None: in slots[b]) -> y fp32 [B*T, H, Dv]. counts and slots as for
+    gdn_conv_silu_batch."""
+    if not (qkv.is_cuda and qkv.dtype == BF16 and qkv.dim() == 2 and qkv.stride(1) == 1):
+        raise ValueError("qkv must be a bf16 2-D GPU tensor")
+    dev = qkv.get_device()
+    hk = n_key_heads or n_heads
+    rows, cols = qkv.shape
+    if not (n_heads >= 1 and hk >= 1 and cols >= 2 * hk * dk + n_heads * dv):
+        raise ValueError(f"qkv rows of {cols} hold no {hk} key heads of {dk} and {n_heads} value heads of {dv}")
+    for t, name in ((b, "b"), (a, "a")):
+        if not (t.dtype == BF16 and t.shape == (rows, n_heads) and (t.stride(1) == 1 or n_heads == 1) and t.get_device() == dev):
+            raise ValueError(f"{name} must be bf16 [{rows}, {n_heads}] with contiguous heads, on qkv's device")
+    if rows > 1 and b.stride(0) != a.stride(0):
+        raise ValueError("a and b must share a row stride")
+    for t, name in ((A_log, "A_log"), (dt_bias, "dt_bias")):
+        if not _fits(t, torch.float32, (n_heads,), dev):
+            raise ValueError(f"{name} must be contiguous fp32 [{n_heads}] on qkv's device")
+    if not (state.dtype == torch.float32 and state.dim() == 4 and state.shape[1:] == (n_heads, dv, dk)):
+        raise ValueError(f"state must be fp32 [n_slots, {n_heads}, {dv}, {dk}]")
+    pool, batch = _state_pool(dev, state, slots, slots_out, counts)
+    if not (rows > 0 and rows % batch == 0):
+        raise ValueError(f"{rows} rows do not divide into {batch} sequences")
+    ldq, ldab = (-(-cols // 8) * 8, n_heads) if rows == 1 else (qkv.stride(0), b.stride(0))
+    if ldq < cols or ldab < n_heads:
+        raise ValueError("rows overlap")
+    if out is not None and not _fits(out, torch.float32, (rows, n_heads, dv), dev):
+        raise ValueError(f"out must be contiguous fp32 [{rows}, {n_heads}, {dv}]")
+    with _on_device(qkv):
+        y = torch.empty((rows, n_heads, dv), dtype=torch.float32, device=qkv.device) if out is None else out
+        _lib.check(_lib.lib().skinny_gdn_recurrence_batch(
+            qkv.data_ptr(), ldq, b.data_ptr(), a.data_ptr(), ldab, A_log.data_ptr(), dt_bias.data_ptr(), batch, rows // batch,
+            pool, state.data_ptr(), y.data_ptr(), n_heads, hk, dk, dv, _lib.stream_of(qkv)), "gdn_recurrence_batch")
+    return y
 
 
 def gdn_record_words(n_heads: int) -> int:
