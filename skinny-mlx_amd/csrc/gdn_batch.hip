@@ -252,34 +252,47 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
 // Rows of the products are dealt to tokens, and rows of the state to key dims, as 8 (r / 4) + 4 (tile) + r % 4: then what one
 // product leaves in a lane (eight consecutive tokens, or dims, of one value column) is the operand that the next one takes.
 //
-// All of it is held in 32 bits. K and Q go in as they are, in bf16, their norms applied to the products in 32 bits; S, R, d, T
-// and the products of q and k are taken as the sum of two bf16 terms (2^-16 of each), so a term's 2^-8 is in no result. G is
-// summed in 64 bits: e^(G_i - G_j) of two tokens after a strong decay would otherwise lose what the decay has taken.
+// All of it is held in 32 bits. What a product takes of it is the sum of two fp16 terms, 2^-22 of the value or, for the
+// small ones, 2^-25 of 1: S, R, d, T and the products of q and k by three products of terms (the fourth is 2^-22 of them).
+// For that every value column has a power of two of its own, which keeps the larger of its state and its values near 1; keys and
+// queries are one fp16 term, exact but for what is 2^-17 of their row's length: a row is taken times the power of two below its
+// length's inverse. (With two bf16 terms, 2^-16, the results were off by 5e-6.) Decays are products of the tokens' own,
+// not exponentials of differences, which lose after a strong decay what it has taken.
 //
 // A correction that is not finite (a value, key or gate that is no number; a state that is none) would meet the rows before its
 // token as 0 * NaN: such a chunk's columns are taken token by token instead.
 constexpr int kChunk = 32, kProducers = 4;
-constexpr float kNoDecay = -110.f;  // e^-110 is zero in 32 bits; sums of what is below would only lose digits
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+using ::mfma16x16x32;  // of bf16
+__device__ __forceinline__ f32x4_t mfma16x16x32(f16x8_t a, f16x8_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f16x8_t f16x8(u32x4_t v) { return __builtin_bit_cast(f16x8_t, v); }
 
 constexpr int kPitch = 36;  // floats of a row of L and T
 struct ChunkScalars {
   float beta[kChunk], in[kChunk], out[kChunk], end[kChunk];  // beta; beta |k| e^G; |q| e^G; |k| e^(G_C - G)
-  float decay[kChunk], kn[kChunk], qn[kChunk];               // token by token
+  float decay[kChunk], k[kChunk], q[kChunk];                 // token by token: the factors that make fp16 rows unit vectors
   float total;                                               // e^G_C
   float pad[3];
 };
-struct ChunkOps {          // 1 KB operands: a lane's 16 bytes after its neighbour's
-  u32x4_t k[2][4][64];     // [token tile][dim step]
+struct ChunkOps {        // 1 KB operands: a lane's 16 bytes after its neighbour's
+  u32x4_t k[2][4][64];   // [token tile][dim step]
   u32x4_t q[2][4][64];
-  u32x4_t kt[4][2][64];    // [dim step][half]: rows are key dims
-  u32x4_t t[2][2][64];     // [term][token tile]
+  u32x4_t t[2][2][64];   // [term][token tile]
   u32x4_t a[2][2][64];
   ChunkScalars sc;
 };
 struct ChunkScratch {
   float l[kChunk][kPitch], t[kChunk][kPitch];
-  double g[kChunk];  // log2 of the decays' product
-  float beta[kChunk], decay[kChunk], kn[kChunk], qn[kChunk];
+  float beta[kChunk], decay[kChunk], kk[kChunk], qq[kChunk];
+  float inner[kChunk];         // the product of the decays of a token's eight up to it
+  float since[kChunk], until[kChunk];  // e^G, e^(G_C - G)
+  float k[kChunk], q[kChunk];  // powers of two
+  float kr[kChunk], qr[kChunk];  // the rest of the norms' inverses
 };
 struct ChunkLds {
   ChunkOps ops[2];
@@ -289,6 +302,13 @@ struct ChunkLds {
 // What one wave's lanes exchange through LDS: written before, read after.
 __device__ __forceinline__ void lanes_meet() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
+// The larger of, and the sum over, the four quads' values, in every lane.
+__device__ __forceinline__ float quads_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float quads_sum(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -296,21 +316,37 @@ __device__ __forceinline__ float quads_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Eight values as the sum of two bf16 terms.
+__device__ __forceinline__ uint32_t two_f16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+}
+
+// Eight values as the sum of two fp16 terms. `one` is 1, unknown to the compiler: the rest is then one instruction a value.
 struct Split {
-  bf16x8_t hi, lo;
+  f16x8_t hi, lo;
 };
-__device__ __forceinline__ Split split(const float (&v)[8]) {
-  typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+__device__ __forceinline__ Split split(const float (&v)[8], float one) {
   u32x4_t hi, lo;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    hi[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{v[2 * w], v[2 * w + 1]}, bf16x2_t));
-    const f32x2_t rest = {v[2 * w] - __uint_as_float(hi[w] << 16), v[2 * w + 1] - __uint_as_float(hi[w] & 0xffff0000u)};
-    lo[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, bf16x2_t));
+    uint32_t word = two_f16(v[2 * w], v[2 * w + 1]);
+    asm("" : "+v"(word));  // seen as part of a vector, the compiler subtracts the first word's halves from every pair
+    hi[w] = word;
+    const f16x2_t h = __builtin_bit_cast(f16x2_t, word);
+    lo[w] = two_f16(fmaf(v[2 * w], one, -(float)h.x), fmaf(v[2 * w + 1], one, -(float)h.y));
   }
-  return {__builtin_bit_cast(bf16x8_t, hi), __builtin_bit_cast(bf16x8_t, lo)};
+  return {f16x8(hi), f16x8(lo)};
+}
+
+// Lane i - N of the same eight, or 1.
+template <int N>
+__device__ __forceinline__ float times_before(float v, int lane) {
+  const float u = __int_as_float(__builtin_amdgcn_update_dpp(0x3f800000, __float_as_int(v), 0x110 + N, 0xF, 0xF, false));
+  return v * ((lane & 7) >= N ? u : 1.f);
+}
+template <int N>
+__device__ __forceinline__ float times_after(float v, int lane) {
+  const float u = __int_as_float(__builtin_amdgcn_update_dpp(0x3f800000, __float_as_int(v), 0x100 + N, 0xF, 0xF, false));
+  return v * ((lane & 7) + N < 8 ? u : 1.f);
 }
 
 // The four waves that prepare chunks: wave `p` the chunks p, p + 4, ...
@@ -325,6 +361,8 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   ChunkScratch& my = lds.scratch[p];
   const int tok[2] = {8 * (r >> 2) + (r & 3), 8 * (r >> 2) + 4 + (r & 3)};  // of this lane's row in each token tile
+  float one = 1.f;
+  asm volatile("" : "+v"(one));
   bf16x8_t kf[2][4], qf[2][4];
   Split aq[2];
   uint16_t na = 0, nb = 0;
@@ -346,83 +384,102 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
         na = x.a[g];
         nb = x.b[g];
       } else if (ahead == 2) {
-        float kn[2], qn[2];
+        if (live < kChunk) {  // rows past the end
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float kk = 0.f, qq = 0.f;
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            u32x4_t kw = __builtin_bit_cast(u32x4_t, kf[t][s]), qw = __builtin_bit_cast(u32x4_t, qf[t][s]);
-            if (tok[t] >= live) kw = qw = u32x4_t{0, 0, 0, 0};  // past the end
-            kf[t][s] = __builtin_bit_cast(bf16x8_t, kw);
-            qf[t][s] = __builtin_bit_cast(bf16x8_t, qw);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const float k0 = __uint_as_float(kw[w] << 16), k1 = __uint_as_float(kw[w] & 0xffff0000u);
-              const float q0 = __uint_as_float(qw[w] << 16), q1 = __uint_as_float(qw[w] & 0xffff0000u);
-              kk = fmaf(k0, k0, kk);
-              kk = fmaf(k1, k1, kk);
-              qq = fmaf(q0, q0, qq);
-              qq = fmaf(q1, q1, qq);
-            }
-          }
-          kn[t] = rsqrtf(quads_sum(kk) + 1e-6f);
-          qn[t] = rsqrtf(quads_sum(qq) + 1e-6f) * rsqrtf((float)kDk);
-          if (q == 0) {
-            my.kn[tok[t]] = kn[t];
-            my.qn[tok[t]] = qn[t];
-          }
-        }
-        {  // a lane per token
-          float g = neg_a * softplus(bf16_bits_to_f32(na) + dtb), beta = 1.0f / (1.0f + expf(-bf16_bits_to_f32(nb)));
-          const bool there = lane < live;
-          const float decay = there ? expf(g) : 1.f;
-          g = there ? (g < kNoDecay ? kNoDecay : g) : 0.f;
-          double sum = (double)g * 1.4426950408889634;
-#pragma unroll
-          for (int step = 1; step < kChunk; step *= 2) {
-            const double before = __shfl_up(sum, step, 64);
-            if (lane >= step) sum += before;
-          }
-          if (lane < kChunk) {
-            my.g[lane] = sum;
-            my.beta[lane] = there ? beta : 0.f;
-            my.decay[lane] = decay;
-          }
-        }
-        lanes_meet();
-        double gj[8];
-        float knj[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          gj[e] = my.g[8 * q + e];
-          knj[e] = my.kn[8 * q + e];
-        }
-#pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {  // rows i = tok[ti], columns j = 8q .. 8q + 7
-          f32x4_t kk[2], qk[2];
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            kk[t] = qk[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-              kk[t] = mfma16x16x32(kf[t][s], kf[ti][s], kk[t]);
-              qk[t] = mfma16x16x32(kf[t][s], qf[ti][s], qk[t]);
+              const u32x4_t none = {0, 0, 0, 0};
+              kf[t][s] = __builtin_bit_cast(bf16x8_t, tok[t] < live ? __builtin_bit_cast(u32x4_t, kf[t][s]) : none);
+              qf[t][s] = __builtin_bit_cast(bf16x8_t, tok[t] < live ? __builtin_bit_cast(u32x4_t, qf[t][s]) : none);
+            }
+        }
+        // Rows i = tok[ti] of this lane (its column of the products), columns j = 8q .. 8q + 7.
+        f32x4_t kk[2][2], qk[2][2], qq[2];
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti) {
+          qq[ti] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            kk[ti][t] = qk[ti][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              kk[ti][t] = mfma16x16x32(kf[t][s], kf[ti][s], kk[ti][t]);
+              qk[ti][t] = mfma16x16x32(kf[t][s], qf[ti][s], qk[ti][t]);
+              if (t == ti) qq[ti] = mfma16x16x32(qf[t][s], qf[ti][s], qq[ti]);
             }
           }
-          const double gi = my.g[tok[ti]];
-          const float bk = my.beta[tok[ti]] * kn[ti];
-          float l[8], a[8];
+        }
+        if (q == r >> 2) {  // the squares are the products' diagonals
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int j = 8 * q + e;
-            const float w = knj[e] * __builtin_amdgcn_exp2f((float)(gi - gj[e]));
-            l[e] = j < tok[ti] ? kk[e >> 2][e & 3] * w * bk : 0.f;
-            a[e] = j <= tok[ti] ? qk[e >> 2][e & 3] * w * qn[ti] : 0.f;
+          for (int ti = 0; ti < 2; ++ti) {
+            const int i = r & 3;
+            my.kk[tok[ti]] = i == 0 ? kk[ti][ti][0] : i == 1 ? kk[ti][ti][1] : i == 2 ? kk[ti][ti][2] : kk[ti][ti][3];
+            my.qq[tok[ti]] = i == 0 ? qq[ti][0] : i == 1 ? qq[ti][1] : i == 2 ? qq[ti][2] : qq[ti][3];
           }
-          aq[ti] = split(a);
-          *reinterpret_cast<f32x4_t*>(&my.l[tok[ti]][8 * q]) = f32x4_t{l[0], l[1], l[2], l[3]};
-          *reinterpret_cast<f32x4_t*>(&my.l[tok[ti]][8 * q + 4]) = f32x4_t{l[4], l[5], l[6], l[7]};
+        }
+        // A lane per token: its gates, and the products of decays.
+        const bool there = lane < live;
+        const float decay = there ? expf(neg_a * softplus(bf16_bits_to_f32(na) + dtb)) : 1.f;
+        const float beta = there ? 1.0f / (1.0f + expf(-bf16_bits_to_f32(nb))) : 0.f;
+        const float inner = times_before<4>(times_before<2>(times_before<1>(decay, lane), lane), lane);
+        const float upto = times_after<4>(times_after<2>(times_after<1>(decay, lane), lane), lane);  // from it to its eight's end
+        float after = __int_as_float(__builtin_amdgcn_update_dpp(0x3f800000, __float_as_int(upto), 0x101, 0xF, 0xF, false));
+        if ((lane & 7) == 7) after = 1.f;
+        float block[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) block[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inner), 8 * i + 7));
+        const int own = lane >> 3;
+        const float first = own == 0 ? 1.f : own == 1 ? block[0] : own == 2 ? block[0] * block[1] : block[0] * block[1] * block[2];
+        const float last = own == 0 ? block[1] * block[2] * block[3] : own == 1 ? block[2] * block[3] : own == 2 ? block[3] : 1.f;
+        lanes_meet();
+        if (lane < kChunk) {
+          my.beta[lane] = beta;
+          my.decay[lane] = decay;
+          my.inner[lane] = inner;
+          my.since[lane] = first * inner;
+          my.until[lane] = after * last;
+          // the row's length as a power of two, and what of 1 / sqrt(squares + 1e-6) that leaves
+          auto norm = [&](float ss, float& two, float& rest) {
+            const uint32_t bits = __float_as_uint(rsqrtf(fmaxf(ss, 0x1p-126f))) & 0x7f800000u;
+            two = __uint_as_float(bits);
+            rest = rsqrtf(ss + 1e-6f) * __uint_as_float(0x7f000000u - bits);
+          };
+          float k2, kr, q2, qr;
+          norm(my.kk[lane], k2, kr);
+          norm(my.qq[lane], q2, qr);
+          my.k[lane] = k2;
+          my.kr[lane] = kr;
+          my.q[lane] = q2;
+          my.qr[lane] = qr;
+        }
+        lanes_meet();
+        const int mine = r >> 2;  // the eight that holds both rows
+        const float between = (q < 1 && mine > 1 ? block[1] : 1.f) * (q < 2 && mine > 2 ? block[2] : 1.f);
+        float dj[8], kj[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          dj[e] = my.decay[8 * q + e];
+          kj[e] = my.k[8 * q + e] * my.kr[8 * q + e];
+        }
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti) {
+          const int i = tok[ti], at = mine == q ? i & 7 : -1;
+          const float kn = my.k[i] * my.kr[i], qn = my.q[i] * my.qr[i], bk = my.beta[i] * kn;
+          float l[8], a[8];
+          float w = mine > q ? my.inner[i] * between : 0.f;  // e^(G_i - G_j), from j = 8q + 7 down
+#pragma unroll
+          for (int e = 7; e >= 0; --e) {
+            if (e == at) w = 1.f;
+            const float wk = w * kj[e];
+            l[e] = kk[ti][e >> 2][e & 3] * wk * bk;
+            a[e] = qk[ti][e >> 2][e & 3] * wk * qn;
+            w *= dj[e];
+          }
+          aq[ti] = split(a, one);
+          // (L's diagonal and what is above it are not read)
+          *reinterpret_cast<f32x4_t*>(&my.l[i][8 * q]) = f32x4_t{l[0], l[1], l[2], l[3]};
+          *reinterpret_cast<f32x4_t*>(&my.l[i][8 * q + 4]) = f32x4_t{l[4], l[5], l[6], l[7]};
         }
       } else if (ahead == 1) {
         // T's diagonal blocks of 16 by substitution, a lane per column: row i is e_i less the rows before it times L's. Then the
@@ -474,57 +531,50 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
         ChunkOps& to = lds.ops[c & 1];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+          const float k2 = my.k[tok[t]], q2 = my.q[tok[t]];
+          auto f16 = [&](bf16x8_t v, float two) {
+            const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+            u32x4_t y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = two_f16(__uint_as_float(w[i] << 16) * two, __uint_as_float(w[i] & 0xffff0000u) * two);
+            return y;
+          };
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            to.k[t][s][lane] = __builtin_bit_cast(u32x4_t, kf[t][s]);
-            to.q[t][s][lane] = __builtin_bit_cast(u32x4_t, qf[t][s]);
+            to.k[t][s][lane] = f16(kf[t][s], k2);
+            to.q[t][s][lane] = f16(qf[t][s], q2);
           }
           float row[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) row[e] = tok[t] < 16 && q >= 2 ? 0.f : my.t[tok[t]][8 * q + e];
-          const Split two = split(row);
+          const Split two = split(row, one);
           to.t[0][t][lane] = __builtin_bit_cast(u32x4_t, two.hi);
           to.t[1][t][lane] = __builtin_bit_cast(u32x4_t, two.lo);
           to.a[0][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].hi);
           to.a[1][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].lo);
         }
         if (lane < kChunk) {
-          const float since = __builtin_amdgcn_exp2f((float)my.g[lane]);
-          const float until = __builtin_amdgcn_exp2f((float)(my.g[kChunk - 1] - my.g[lane]));
-          const float beta = my.beta[lane], kn = my.kn[lane], qn = my.qn[lane];
+          const float beta = my.beta[lane], kr = my.kr[lane], qr = my.qr[lane], since = my.since[lane];
           to.sc.beta[lane] = beta;
-          to.sc.in[lane] = beta * kn * since;
-          to.sc.out[lane] = qn * since;
-          to.sc.end[lane] = kn * until;
+          to.sc.in[lane] = beta * kr * since;
+          to.sc.out[lane] = qr * since;
+          to.sc.end[lane] = kr * my.until[lane];
           to.sc.decay[lane] = my.decay[lane];
-          to.sc.kn[lane] = kn;
-          to.sc.qn[lane] = qn;
+          to.sc.k[lane] = kr;
+          to.sc.q[lane] = qr;
           if (lane == kChunk - 1) to.sc.total = since;
         }
-        lanes_meet();
-        // K turned over: row r of (s, half) is dim 32 s + 8 (r / 4) + 4 half + r % 4, its operand tokens 8q .. 8q + 7.
-        const uint16_t* k = reinterpret_cast<const uint16_t*>(&to.k[0][0][0]);
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            u32x4_t v;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              uint32_t two[2];
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int e = 2 * w + i;
-                two[i] = k[(((e >> 2) * 4 + s) * 64 + 4 * q + (e & 3) + 16 * (r >> 2)) * 8 + 4 * half + (r & 3)];
-              }
-              v[w] = two[0] | two[1] << 16;
-            }
-            to.kt[s][half][lane] = v;
-          }
       }
     }
     lds_barrier();
   }
+}
+
+// Column scales: a column's values and state stay between 2^-2 and 2^5 of its power of two, or are brought near 4; powers
+// within 2^-100 .. 2^100.
+constexpr float kLow = 0.25f, kHigh = 32.f;
+__device__ __forceinline__ float power_below(float v) {  // that leaves v at 4 to 8
+  return __uint_as_float((__float_as_uint(fminf(fmaxf(v * 0.25f, 0x1p-100f), 0x1p100f))) & 0x7f800000u);
 }
 
 template <int WC, int NT>
@@ -555,11 +605,15 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
   }
   const int r = lane & 15, q = lane >> 4;
   const int col = wave * 16 * NT + r;  // of the workgroup's; + 16 nt
-  // dims 32 s + 8 q + 4 half + i of column col + 16 nt
+  float one = 1.f;
+  asm volatile("" : "+v"(one));
+  // dims 32 s + 8 q + 4 half + i of column col + 16 nt, times `inv`
   f32x4_t st[NT][4][2];
+  float inv[NT], scale[NT];
   const size_t at = ((size_t)h * kDv + col0 + col) * kDk + q * 8;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < NT; ++nt) {
+    inv[nt] = scale[nt] = 1.f;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -568,6 +622,8 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
         if (run.read >= 0)
           st[nt][s][half] = *reinterpret_cast<const f32x4_t*>(state + run.read * pool.stride + at + (size_t)nt * 16 * kDk + s * 32 + half * 4);
       }
+  }
+  const float qscale = rsqrtf((float)kDk);
   const uint16_t* vrow = rows + (size_t)2 * Hk * kDk + (size_t)h * kDv + col0 + col;
   uint16_t nv[NT][8];
   auto load_v = [&](int c) {
@@ -591,6 +647,37 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[nt][e] = 8 * q + e < live ? bf16_bits_to_f32(nv[nt][e]) : 0.f;
     if (c + 1 < chunks) load_v(c + 1);
+    bool off = false;
+    float top[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float vm = 0.f, sm = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vm = fmaxf(vm, fabsf(v[nt][e]));
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sm = fmaxf(sm, fabsf(st[nt][s][half][i]));
+      top[nt] = quads_max(fmaxf(vm * inv[nt], sm));
+      off |= top[nt] > kHigh || (top[nt] < kLow && top[nt] > 0.f);
+    }
+    if (__any(off)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (!(top[nt] > 0.f && top[nt] < INFINITY)) continue;
+        const float to = power_below(top[nt] * scale[nt]), f = scale[nt] / to;
+        scale[nt] = to;
+        inv[nt] = 1.f / to;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st[nt][s][half][i] *= f;
+      }
+    }
     f32x4_t ks[NT][2], qs[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -603,11 +690,11 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
       for (int nt = 0; nt < NT; ++nt) {
         const f32x4_t a = st[nt][s][0], d = st[nt][s][1];
         const float eight[8] = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
-        two[nt] = split(eight);
+        two[nt] = split(eight, one);
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, ops.k[t][s][lane]), qf = __builtin_bit_cast(bf16x8_t, ops.q[t][s][lane]);
+        const f16x8_t kf = f16x8(ops.k[t][s][lane]), qf = f16x8(ops.q[t][s][lane]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           ks[nt][t] = mfma16x16x32(kf, two[nt].hi, ks[nt][t]);
@@ -625,42 +712,44 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
         to[4 + i] = d[i];
       }
     };
-    float beta[8], in[8];
-    scalars(ops.sc.beta, beta);
-    scalars(ops.sc.in, in);
     f32x4_t d[NT][2];
     bool odd = false;
     {
-      bf16x8_t tf[2][2];
+      float beta[8], in[8];
+      scalars(ops.sc.beta, beta);
+      scalars(ops.sc.in, in);
+      f16x8_t tf[2][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) tf[i][t] = __builtin_bit_cast(bf16x8_t, ops.t[i][t][lane]);
+        for (int t = 0; t < 2; ++t) tf[i][t] = f16x8(ops.t[i][t][lane]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float right[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], v[nt][e], -in[e] * ks[nt][e >> 2][e & 3]);
-        const Split two = split(right);
+        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], v[nt][e] * inv[nt], -in[e] * ks[nt][e >> 2][e & 3]);
+        const Split two = split(right, one);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           d[nt][t] = mfma16x16x32(tf[0][t], two.lo, f32x4_t{0.f, 0.f, 0.f, 0.f});
           d[nt][t] = mfma16x16x32(tf[1][t], two.hi, d[nt][t]);
           d[nt][t] = mfma16x16x32(tf[0][t], two.hi, d[nt][t]);
         }
+        float sum = 0.f;  // NaN where one of them is no number
 #pragma unroll
-        for (int e = 0; e < 8; ++e) odd |= !(fabsf(d[nt][e >> 2][e & 3]) < INFINITY);
+        for (int e = 0; e < 8; ++e) sum = fmaf(d[nt][e >> 2][e & 3], 0.f, sum);
+        odd |= !(sum == 0.f);
       }
     }
     if (!__any(odd)) {
       float out[8], end[8];
       scalars(ops.sc.out, out);
       scalars(ops.sc.end, end);
-      bf16x8_t af[2][2];
+      f16x8_t af[2][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) af[i][t] = __builtin_bit_cast(bf16x8_t, ops.a[i][t][lane]);
+        for (int t = 0; t < 2; ++t) af[i][t] = f16x8(ops.a[i][t][lane]);
       Split ends[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -670,9 +759,10 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
           eight[e] = d[nt][e >> 2][e & 3];
           decayed[e] = eight[e] * end[e];
         }
-        const Split two = split(eight);
-        ends[nt] = split(decayed);
+        const Split two = split(eight, one);
+        ends[nt] = split(decayed, one);
         float* yr = yb + (size_t)(t0 + 8 * q) * ystep + col + 16 * nt;
+        const float whole = qscale * scale[nt];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           f32x4_t acc;
@@ -683,15 +773,27 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
           acc = mfma16x16x32(af[0][t], two.hi, acc);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (8 * q + 4 * t + i < live) yr[(4 * t + i) * ystep] = acc[i];
+            if (8 * q + 4 * t + i < live) yr[(4 * t + i) * ystep] = acc[i] * whole;
         }
       }
       const float total = ops.sc.total;
+      // K turned over, four tokens of a lane's dim at a time: the sixteen lanes of a quad give rows 4q .. 4q + 3 of a tile,
+      // four dims each, and take a dim of the four.
+      const uint32_t turn = ((4 * q + (r >> 2)) + 16 * (r & 3)) * 16;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const bf16x8_t kt = __builtin_bit_cast(bf16x8_t, ops.kt[s][half][lane]);
+          typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+          typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+          typedef __attribute__((ext_vector_type(2))) uint32_t two_t;
+          two_t part[2];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const char* from = reinterpret_cast<const char*>(&ops.k[t][s][0]) + turn + 8 * half;
+            part[t] = __builtin_bit_cast(two_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)from));
+          }
+          const f16x8_t kt = f16x8(u32x4_t{part[0].x, part[0].y, part[1].x, part[1].y});
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -701,30 +803,38 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
           }
         }
     } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st[nt][s][half][i] *= scale[nt];
+        scale[nt] = inv[nt] = 1.f;
+      }
       for (int i = 0; i < live; ++i) {  // token by token
         const int tile = i >> 2 & 1, row = 4 * (i >> 3) + (i & 3) + 16 * q;
-        const float decay = ops.sc.decay[i], kn = ops.sc.kn[i], qn = ops.sc.qn[i], bt = ops.sc.beta[i];
+        const float decay = ops.sc.decay[i], kn = ops.sc.k[i], qn = ops.sc.q[i] * qscale, bt = ops.sc.beta[i];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float sum = 0.f;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const u32x4_t w = ops.k[tile][s][row];
+            const f16x8_t w = f16x8(ops.k[tile][s][row]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              sum = fmaf(bf16_bits_to_f32(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu) * kn, st[nt][s][e >> 2][e & 3], sum);
+            for (int e = 0; e < 8; ++e) sum = fmaf((float)w[e] * kn, st[nt][s][e >> 2][e & 3], sum);
           }
           const float delta = bt * (bf16_bits_to_f32(vrow[(int64_t)(t0 + i) * ldq + nt * 16]) - decay * quads_sum(sum));
           float yv = 0.f;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const u32x4_t w = ops.k[tile][s][row], z = ops.q[tile][s][row];
+            const f16x8_t w = f16x8(ops.k[tile][s][row]), z = f16x8(ops.q[tile][s][row]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float x = fmaf(bf16_bits_to_f32(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu) * kn, delta,
-                                   st[nt][s][e >> 2][e & 3] * decay);
+              const float x = fmaf((float)w[e] * kn, delta, st[nt][s][e >> 2][e & 3] * decay);
               st[nt][s][e >> 2][e & 3] = x;
-              yv = fmaf(bf16_bits_to_f32(e & 1 ? z[e >> 1] >> 16 : z[e >> 1] & 0xffffu) * qn, x, yv);
+              yv = fmaf((float)z[e] * qn, x, yv);
             }
           }
           yv = quads_sum(yv);
@@ -740,7 +850,8 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int half = 0; half < 2; ++half)
-        *reinterpret_cast<f32x4_t*>(state + run.write * pool.stride + at + (size_t)nt * 16 * kDk + s * 32 + half * 4) = st[nt][s][half];
+        *reinterpret_cast<f32x4_t*>(state + run.write * pool.stride + at + (size_t)nt * 16 * kDk + s * 32 + half * 4) =
+            st[nt][s][half] * scale[nt];
 }
 
 template <int WC, int NT>

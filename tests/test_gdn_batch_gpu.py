@@ -72,10 +72,12 @@ def _rule(m, i, state, chunk):
     _bound: the error of a value column, E (2-norm over the key dims), is carried on by the tokens' (I - beta k k^T) and
     decay, none of which lengthens it, and each token adds its own. Token by token (chunk 0) all is fp32: k.S and q.S over
     128 products and the update, 2 * (128 + 16) steps of 2^-24 of |v| + |S|; the unit vectors and gates, another 2 * 140, the
-    exponentials 2 ulp of an argument's worth: 2^-14 in all. In chunks, S, the corrections and the triangular matrices are
-    the sum of two bf16 terms: 2^-16 of each factor, and 2^-16 for the product of the second terms; a correction takes
-    those of the chunk's tokens before it, each of at most 1 times its beta (|v| + |S|), twice (the system's inverse, and
-    its own rounding in 32 substitution steps): so 2^-13 of the sum of beta (|v| + |S|) over the chunk."""
+    exponentials 2 ulp of an argument's worth: 2^-14 in all. In chunks, the state, the corrections and the triangular matrices
+    go into their products as two fp16 terms: 2^-22 of a value, and 2^-25 of a power of two that is at most 4 times the
+    column's largest, so 2^-21.4 of that, 2^-18 of the column's length over 128 dims; the products are summed in fp32, 128 and 32
+    steps of 2^-24, 2^-17 of theirs; a correction takes the errors of the chunk's tokens before it, each of at most 1 times its
+    beta (|v| + |S|), from the system's inverse (32 substitution steps of 2^-24, and its terms) and its own two terms: 2^-16 of
+    the sum of beta (|v| + |S|) over the chunk and of the token's own."""
     n, T = m.counts[i], m.T
     x = m.qkv.view(-1, T, 2 * m.key_heads + m.heads, D)[i, :n].double().cpu()
     rep = m.heads // m.key_heads
@@ -98,11 +100,11 @@ def _rule(m, i, state, chunk):
         size = v[t].abs() + before
         if chunk:
             recent = (0 if t % chunk == 0 else recent) + beta[t, :, None] * size
-            add = 2.0 ** -13 * (recent + size / chunk)
+            add = 2.0 ** -16 * (recent + size)
         else:
             add = 2.0 ** -14 * size
         err = err * decay[t, :, None] + add
-        yerr[t] = q[t].norm(dim=-1)[:, None] * (err + 2.0 ** -14 * s.norm(dim=-1) + add)
+        yerr[t] = q[t].norm(dim=-1)[:, None] * (err + (2.0 ** -16 if chunk else 2.0 ** -14) * s.norm(dim=-1) + add)
     return y, s, yerr, err
 
 
