@@ -288,11 +288,11 @@ struct ChunkOps {        // 1 KB operands: a lane's 16 bytes after its neighbour
 };
 struct ChunkScratch {
   float l[kChunk][kPitch], t[kChunk][kPitch];
-  float beta[kChunk], decay[kChunk], kk[kChunk], qq[kChunk];
+  float beta[kChunk], decay[kChunk];
   float inner[kChunk];         // the product of the decays of a token's eight up to it
   float since[kChunk], until[kChunk];  // e^G, e^(G_C - G)
-  float k[kChunk], q[kChunk];  // powers of two
-  float kr[kChunk], qr[kChunk];  // the rest of the norms' inverses
+  // of k and of q: the squares; a power of two near the length's inverse; what that leaves of 1 / sqrt(squares + 1e-6); that
+  float sq[2][kChunk], two[2][kChunk], rest[2][kChunk], inv[2][kChunk];
 };
 struct ChunkLds {
   ChunkOps ops[2];
@@ -337,6 +337,16 @@ __device__ __forceinline__ Split split(const float (&v)[8], float one) {
   return {f16x8(hi), f16x8(lo)};
 }
 
+// Whether one of the eight is an infinity or NaN.
+__device__ __forceinline__ bool no_numbers(f16x8_t v) {
+  typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
+  const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
+  u16x2_t m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
+  return m.x >= 0x7c00 || m.y >= 0x7c00;
+}
+
 // Lane i - N of the same eight, or 1.
 template <int N>
 __device__ __forceinline__ float times_before(float v, int lane) {
@@ -349,12 +359,35 @@ __device__ __forceinline__ float times_after(float v, int lane) {
   return v * ((lane & 7) + N < 8 ? u : 1.f);
 }
 
-// The four waves that prepare chunks: wave `p` the chunks p, p + 4, ...
+// v, which the compiler then forms again in every turn of a loop: its sums with other offsets, formed before it, take two
+// registers each.
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+__device__ __forceinline__ const uint16_t* at_bytes(const uint16_t* base, uint32_t offset) {
+  return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(base) + offset);
+}
+__device__ __forceinline__ float* at_bytes(float* base, uint32_t offset) {
+  return reinterpret_cast<float*>(reinterpret_cast<char*>(base) + offset);
+}
+
+// Eight floats at a multiple of four.
+__device__ __forceinline__ void eight_of(const float* of, float (&to)[8]) {
+  const f32x4_t a = *reinterpret_cast<const f32x4_t*>(of), b = *reinterpret_cast<const f32x4_t*>(of + 4);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    to[i] = a[i];
+    to[4 + i] = b[i];
+  }
+}
+
+// The four waves that prepare chunks: wave `p` the chunks p, p + 4, ... A chunk's gates are asked for a turn ahead.
 struct Rows {
   const uint16_t* qkv;  // of the sequence's first token
-  int64_t ldq;
+  uint32_t ldq;
   const uint16_t *b, *a;
-  int64_t ldab;
+  uint32_t ldab;
   int h, hk, H, Hk, count;
 };
 __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int p, int chunks, float neg_a, float dtb) {
@@ -363,59 +396,42 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
   const int tok[2] = {8 * (r >> 2) + (r & 3), 8 * (r >> 2) + 4 + (r & 3)};  // of this lane's row in each token tile
   float one = 1.f;
   asm volatile("" : "+v"(one));
-  bf16x8_t kf[2][4], qf[2][4];
-  Split aq[2];
+  uint32_t off[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) off[t] = tok[t] * x.ldq + q * 8;
+  const uint32_t goff = min(lane, kChunk - 1) * x.ldab;
   uint16_t na = 0, nb = 0;
-  for (int n = chunks ? -kProducers : 0; n < chunks; ++n) {
-    const int ahead = (p - n - 1) & 3, c = n + 1 + ahead;  // the chunk, `ahead` periods before its last phase
-    if (c < chunks && c >= 0) {
-      const int t0 = c * kChunk, live = min(kChunk, x.count - t0);
-      if (ahead == 3) {
+  auto load_gates = [&](int c) {
+    if (c >= chunks) return;
+    const int64_t row = (int64_t)c * kChunk;
+    const int live = min(kChunk, x.count - c * kChunk);
+    const uint32_t at = live == kChunk ? goff : (uint32_t)min(lane, live - 1) * x.ldab;
+    na = (x.a + row * x.ldab + x.h)[at];
+    nb = (x.b + row * x.ldab + x.h)[at];
+  };
+  load_gates(p);
+  // Periods: chunk c's last one here is the one before the other waves take it, four before the first chunk's.
+  int left = chunks + kProducers;
+  auto end_period = [&]() {
+    lds_barrier();
+    --left;
+  };
+  for (int i = 0; i < p; ++i) end_period();
+  for (int c = p; c < chunks; c += kProducers) {
+    const int t0 = c * kChunk, live = min(kChunk, x.count - t0);
+    bf16x8_t kf[2][4], qf[2][4];
+    Split aq[2];
+    {
+      {
+        const uint16_t* base = x.qkv + (int64_t)t0 * x.ldq + (size_t)x.hk * kDk;
+        const uint16_t* kbase = base + (size_t)x.Hk * kDk;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const uint16_t* row = x.qkv + (int64_t)(t0 + min(tok[t], live - 1)) * x.ldq + (size_t)x.hk * kDk + q * 8;
+          const uint32_t at = live == kChunk ? off[t] : min(tok[t], live - 1) * x.ldq + q * 8;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            qf[t][s] = *reinterpret_cast<const bf16x8_t*>(row + s * 32);
-            kf[t][s] = *reinterpret_cast<const bf16x8_t*>(row + (size_t)x.Hk * kDk + s * 32);
-          }
-        }
-        const int64_t g = (int64_t)(t0 + min(lane, live - 1)) * x.ldab + x.h;
-        na = x.a[g];
-        nb = x.b[g];
-      } else if (ahead == 2) {
-        if (live < kChunk) {  // rows past the end
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              const u32x4_t none = {0, 0, 0, 0};
-              kf[t][s] = __builtin_bit_cast(bf16x8_t, tok[t] < live ? __builtin_bit_cast(u32x4_t, kf[t][s]) : none);
-              qf[t][s] = __builtin_bit_cast(bf16x8_t, tok[t] < live ? __builtin_bit_cast(u32x4_t, qf[t][s]) : none);
-            }
-        }
-        // Rows i = tok[ti] of this lane (its column of the products), columns j = 8q .. 8q + 7.
-        f32x4_t kk[2][2], qk[2][2], qq[2];
-#pragma unroll
-        for (int ti = 0; ti < 2; ++ti) {
-          qq[ti] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            kk[ti][t] = qk[ti][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              kk[ti][t] = mfma16x16x32(kf[t][s], kf[ti][s], kk[ti][t]);
-              qk[ti][t] = mfma16x16x32(kf[t][s], qf[ti][s], qk[ti][t]);
-              if (t == ti) qq[ti] = mfma16x16x32(qf[t][s], qf[ti][s], qq[ti]);
-            }
-          }
-        }
-        if (q == r >> 2) {  // the squares are the products' diagonals
-#pragma unroll
-          for (int ti = 0; ti < 2; ++ti) {
-            const int i = r & 3;
-            my.kk[tok[ti]] = i == 0 ? kk[ti][ti][0] : i == 1 ? kk[ti][ti][1] : i == 2 ? kk[ti][ti][2] : kk[ti][ti][3];
-            my.qq[tok[ti]] = i == 0 ? qq[ti][0] : i == 1 ? qq[ti][1] : i == 2 ? qq[ti][2] : qq[ti][3];
+            qf[t][s] = *reinterpret_cast<const bf16x8_t*>(base + at + s * 32);
+            kf[t][s] = *reinterpret_cast<const bf16x8_t*>(kbase + at + s * 32);
           }
         }
         // A lane per token: its gates, and the products of decays.
@@ -432,48 +448,79 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
         const int own = lane >> 3;
         const float first = own == 0 ? 1.f : own == 1 ? block[0] : own == 2 ? block[0] * block[1] : block[0] * block[1] * block[2];
         const float last = own == 0 ? block[1] * block[2] * block[3] : own == 1 ? block[2] * block[3] : own == 2 ? block[3] : 1.f;
-        lanes_meet();
         if (lane < kChunk) {
           my.beta[lane] = beta;
           my.decay[lane] = decay;
           my.inner[lane] = inner;
           my.since[lane] = first * inner;
           my.until[lane] = after * last;
-          // the row's length as a power of two, and what of 1 / sqrt(squares + 1e-6) that leaves
-          auto norm = [&](float ss, float& two, float& rest) {
-            const uint32_t bits = __float_as_uint(rsqrtf(fmaxf(ss, 0x1p-126f))) & 0x7f800000u;
-            two = __uint_as_float(bits);
-            rest = rsqrtf(ss + 1e-6f) * __uint_as_float(0x7f000000u - bits);
-          };
-          float k2, kr, q2, qr;
-          norm(my.kk[lane], k2, kr);
-          norm(my.qq[lane], q2, qr);
-          my.k[lane] = k2;
-          my.kr[lane] = kr;
-          my.q[lane] = q2;
-          my.qr[lane] = qr;
+        }
+      }
+      end_period();
+      {
+        if (live < kChunk) {  // rows past the end
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              const u32x4_t none = {0, 0, 0, 0};
+              kf[t][s] = __builtin_bit_cast(bf16x8_t, tok[t] < live ? __builtin_bit_cast(u32x4_t, kf[t][s]) : none);
+              qf[t][s] = __builtin_bit_cast(bf16x8_t, tok[t] < live ? __builtin_bit_cast(u32x4_t, qf[t][s]) : none);
+            }
+        }
+        // Rows i = tok[ti] of this lane (its column of the products), columns j = 8q .. 8q + 7.
+        f32x4_t kk[2][2], qk[2][2], qq[2];
+#pragma unroll
+        for (int ti = 0; ti < 2; ++ti) {
+          qq[ti] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < 2; ++t) kk[ti][t] = qk[ti][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int ti = 0; ti < 2; ++ti) {
+            qq[ti] = mfma16x16x32(qf[ti][s], qf[ti][s], qq[ti]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              kk[ti][t] = mfma16x16x32(kf[t][s], kf[ti][s], kk[ti][t]);
+              qk[ti][t] = mfma16x16x32(kf[t][s], qf[ti][s], qk[ti][t]);
+            }
+          }
+        if (q == r >> 2) {  // the squares are the products' diagonals
+#pragma unroll
+          for (int ti = 0; ti < 2; ++ti) {
+            const int i = r & 3;
+            my.sq[0][tok[ti]] = i == 0 ? kk[ti][ti][0] : i == 1 ? kk[ti][ti][1] : i == 2 ? kk[ti][ti][2] : kk[ti][ti][3];
+            my.sq[1][tok[ti]] = i == 0 ? qq[ti][0] : i == 1 ? qq[ti][1] : i == 2 ? qq[ti][2] : qq[ti][3];
+          }
+        }
+        lanes_meet();
+        {  // a lane per row, keys and queries
+          const float ss = my.sq[0][lane], inv = rsqrtf(ss + 1e-6f);
+          const uint32_t bits = __float_as_uint(rsqrtf(fmaxf(ss, 0x1p-126f))) & 0x7f800000u;
+          my.two[0][lane] = __uint_as_float(bits);
+          my.rest[0][lane] = inv * __uint_as_float(0x7f000000u - bits);
+          my.inv[0][lane] = inv;
         }
         lanes_meet();
         const int mine = r >> 2;  // the eight that holds both rows
-        const float between = (q < 1 && mine > 1 ? block[1] : 1.f) * (q < 2 && mine > 2 ? block[2] : 1.f);
+        const float between = (q < 1 && mine > 1 ? my.inner[15] : 1.f) * (q < 2 && mine > 2 ? my.inner[23] : 1.f);
         float dj[8], kj[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          dj[e] = my.decay[8 * q + e];
-          kj[e] = my.k[8 * q + e] * my.kr[8 * q + e];
-        }
+        eight_of(&my.decay[8 * q], dj);
+        eight_of(&my.inv[0][8 * q], kj);
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti) {
           const int i = tok[ti], at = mine == q ? i & 7 : -1;
-          const float kn = my.k[i] * my.kr[i], qn = my.q[i] * my.qr[i], bk = my.beta[i] * kn;
+          const float qn = my.inv[1][i], bk = my.beta[i] * my.inv[0][i];
           float l[8], a[8];
           float w = mine > q ? my.inner[i] * between : 0.f;  // e^(G_i - G_j), from j = 8q + 7 down
 #pragma unroll
           for (int e = 7; e >= 0; --e) {
-            if (e == at) w = 1.f;
+            w = e == at ? 1.f : w;
             const float wk = w * kj[e];
-            l[e] = kk[ti][e >> 2][e & 3] * wk * bk;
-            a[e] = qk[ti][e >> 2][e & 3] * wk * qn;
+            l[e] = kk[ti][e >> 2][e & 3] * (wk * bk);
+            a[e] = qk[ti][e >> 2][e & 3] * (wk * qn);
             w *= dj[e];
           }
           aq[ti] = split(a, one);
@@ -481,7 +528,9 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
           *reinterpret_cast<f32x4_t*>(&my.l[i][8 * q]) = f32x4_t{l[0], l[1], l[2], l[3]};
           *reinterpret_cast<f32x4_t*>(&my.l[i][8 * q + 4]) = f32x4_t{l[4], l[5], l[6], l[7]};
         }
-      } else if (ahead == 1) {
+      }
+      end_period();
+      {
         // T's diagonal blocks of 16 by substitution, a lane per column: row i is e_i less the rows before it times L's. Then the
         // block below: T21 = -T22 (L21 T11), four rows a quad.
         const int half = q & 1;
@@ -527,16 +576,23 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
         four_rows(my.t, 16 + 4 * q, 16, 16 + r, four);
 #pragma unroll
         for (int e = 0; e < 4; ++e) my.t[16 + 4 * q + e][r] = -four[e];
-      } else {
+      }
+      end_period();
+      {
+        load_gates(c + kProducers);
         ChunkOps& to = lds.ops[c & 1];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float k2 = my.k[tok[t]], q2 = my.q[tok[t]];
+          const float k2 = my.two[0][tok[t]], q2 = my.two[1][tok[t]];
           auto f16 = [&](bf16x8_t v, float two) {
             const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
             u32x4_t y;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = two_f16(__uint_as_float(w[i] << 16) * two, __uint_as_float(w[i] & 0xffff0000u) * two);
+            for (int i = 0; i < 4; ++i) {
+              const _Float16 lo = (_Float16)fmaf(__uint_as_float(w[i] << 16), two, 0.f);
+              const _Float16 hi = (_Float16)fmaf(__uint_as_float(w[i] & 0xffff0000u), two, 0.f);
+              y[i] = __builtin_bit_cast(uint32_t, f16x2_t{lo, hi});
+            }
             return y;
           };
 #pragma unroll
@@ -545,8 +601,9 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
             to.q[t][s][lane] = f16(qf[t][s], q2);
           }
           float row[8];
+          eight_of(&my.t[tok[t]][8 * q], row);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) row[e] = tok[t] < 16 && q >= 2 ? 0.f : my.t[tok[t]][8 * q + e];
+          for (int e = 0; e < 8; ++e) row[e] = tok[t] < 16 && q >= 2 ? 0.f : row[e];
           const Split two = split(row, one);
           to.t[0][t][lane] = __builtin_bit_cast(u32x4_t, two.hi);
           to.t[1][t][lane] = __builtin_bit_cast(u32x4_t, two.lo);
@@ -554,7 +611,7 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
           to.a[1][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].lo);
         }
         if (lane < kChunk) {
-          const float beta = my.beta[lane], kr = my.kr[lane], qr = my.qr[lane], since = my.since[lane];
+          const float beta = my.beta[lane], kr = my.rest[0][lane], qr = my.rest[1][lane], since = my.since[lane];
           to.sc.beta[lane] = beta;
           to.sc.in[lane] = beta * kr * since;
           to.sc.out[lane] = qr * since;
@@ -565,14 +622,17 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
           if (lane == kChunk - 1) to.sc.total = since;
         }
       }
+      end_period();
     }
-    lds_barrier();
   }
+  while (left > 0) end_period();
 }
 
-// Column scales: a column's values and state stay between 2^-2 and 2^5 of its power of two, or are brought near 4; powers
-// within 2^-100 .. 2^100.
+// A column's power of two: its values stay within 2^5 of it, and the larger of values and state between 2^-2 and 2^5 wherever it
+// is looked at, or the power is set anew, so that it is 4 to 8; powers within 2^-100 .. 2^100. A column's length grows by at most
+// beta |v| a token: from one look to the next it stays below 2^5 (sqrt(128) + 128), far inside fp16.
 constexpr float kLow = 0.25f, kHigh = 32.f;
+constexpr int kLook = 4;  // chunks from one look at the state to the next; its values are looked at in each
 __device__ __forceinline__ float power_below(float v) {  // that leaves v at 4 to 8
   return __uint_as_float((__float_as_uint(fminf(fmaxf(v * 0.25f, 0x1p-100f), 0x1p100f))) & 0x7f800000u);
 }
@@ -599,39 +659,70 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
   const int chunks = (run.count + kChunk - 1) / kChunk;
   const uint16_t* rows = qkv + (int64_t)row0 * ldq;
   if (wave >= WC) {
-    const Rows x{rows, ldq, bcol + (int64_t)row0 * ldab, acol + (int64_t)row0 * ldab, ldab, h, h / (H / Hk), H, Hk, run.count};
-    prepare_chunks(x, lds, wave - WC, chunks, -expf(A_log[h]), dt_bias[h]);
+    const Rows x{rows, (uint32_t)ldq, bcol + (int64_t)row0 * ldab, acol + (int64_t)row0 * ldab, (uint32_t)ldab, h, h / (H / Hk), H, Hk, run.count};
+    if (chunks) prepare_chunks(x, lds, wave - WC, chunks, -expf(A_log[h]), dt_bias[h]);
     return;
   }
+  __builtin_amdgcn_s_setprio(1);  // before the preparing waves, which have periods to spare
   const int r = lane & 15, q = lane >> 4;
   const int col = wave * 16 * NT + r;  // of the workgroup's; + 16 nt
   float one = 1.f;
   asm volatile("" : "+v"(one));
   // dims 32 s + 8 q + 4 half + i of column col + 16 nt, times `inv`
   f32x4_t st[NT][4][2];
-  float inv[NT], scale[NT];
+  float inv[NT], scale[NT], top[NT];
   const size_t at = ((size_t)h * kDv + col0 + col) * kDk + q * 8;
+  float* to = state + run.write * pool.stride + at;
+  auto get_state = [&](const float* from) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    inv[nt] = scale[nt] = 1.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      inv[nt] = scale[nt] = 1.f;
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        st[nt][s][half] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        if (run.read >= 0)
-          st[nt][s][half] = *reinterpret_cast<const f32x4_t*>(state + run.read * pool.stride + at + (size_t)nt * 16 * kDk + s * 32 + half * 4);
-      }
+        for (int half = 0; half < 2; ++half) st[nt][s][half] = *reinterpret_cast<const f32x4_t*>(from + nt * 16 * kDk + s * 32 + half * 4);
+    }
+  };
+  auto put_state = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          *reinterpret_cast<f32x4_t*>(to + nt * 16 * kDk + s * 32 + half * 4) = st[nt][s][half] * scale[nt];
+  };
+  if (run.read >= 0) {
+    get_state(state + run.read * pool.stride + at);
+  } else {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      inv[nt] = scale[nt] = 1.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) st[nt][s][half] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
   }
   const float qscale = rsqrtf((float)kDk);
-  const uint16_t* vrow = rows + (size_t)2 * Hk * kDk + (size_t)h * kDv + col0 + col;
+  // A chunk's values and results at 32-bit offsets (bytes) from its first row.
+  const uint16_t* vrow = rows + (size_t)2 * Hk * kDk + (size_t)h * kDv + col0;
+  const uint32_t ld = (uint32_t)ldq * 2, yld = (uint32_t)ystep * 4;
   uint16_t nv[NT][8];
   auto load_v = [&](int c) {
+    const uint16_t* from = vrow + (int64_t)c * kChunk * ldq;
+    const int left = run.count - c * kChunk - 1;
+    if (left >= kChunk - 1) {
+      uint32_t at = here(8 * q * ld + col * 2);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint16_t* from = vrow + (int64_t)min(c * kChunk + 8 * q + e, run.count - 1) * ldq;
+      for (int e = 0; e < 8; ++e, at += ld)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) nv[nt][e] = from[nt * 16];
+        for (int nt = 0; nt < NT; ++nt) nv[nt][e] = *at_bytes(from + nt * 16, at);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) nv[nt][e] = *at_bytes(from + nt * 16, min(8 * q + e, left) * ld + col * 2);
     }
   };
   if (chunks) {
@@ -641,33 +732,35 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
   for (int c = 0; c < chunks; ++c) {
     const ChunkOps& ops = lds.ops[c & 1];
     const int t0 = c * kChunk, live = min(kChunk, run.count - t0);
-    float v[NT][8];
+    const bool full = live == kChunk;
+    if (!full) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[nt][e] = 8 * q + e < live ? bf16_bits_to_f32(nv[nt][e]) : 0.f;
-    if (c + 1 < chunks) load_v(c + 1);
+        for (int e = 0; e < 8; ++e) nv[nt][e] = 8 * q + e < live ? nv[nt][e] : (uint16_t)0;
+    }
     bool off = false;
-    float top[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float vm = 0.f, sm = 0.f;
+      uint32_t m = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) vm = fmaxf(vm, fabsf(v[nt][e]));
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sm = fmaxf(sm, fabsf(st[nt][s][half][i]));
-      top[nt] = quads_max(fmaxf(vm * inv[nt], sm));
-      off |= top[nt] > kHigh || (top[nt] < kLow && top[nt] > 0.f);
+      for (int e = 0; e < 8; ++e) m = max(m, nv[nt][e] & 0x7fffu);
+      top[nt] = bf16_bits_to_f32(m) * inv[nt];  // of this lane's values
+      off |= top[nt] > kHigh;
     }
-    if (__any(off)) {
+    if (c % kLook == 0 || __any(off)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if (!(top[nt] > 0.f && top[nt] < INFINITY)) continue;
-        const float to = power_below(top[nt] * scale[nt]), f = scale[nt] / to;
+        float sm = top[nt];
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sm = fmaxf(sm, fabsf(st[nt][s][half][i]));
+        sm = quads_max(sm);
+        if (!(sm > kHigh || sm < kLow) || !(sm > 0.f && sm < INFINITY)) continue;
+        const float to = power_below(sm * scale[nt]), f = scale[nt] / to;
         scale[nt] = to;
         inv[nt] = 1.f / to;
 #pragma unroll
@@ -704,20 +797,13 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
         }
       }
     }
-    auto scalars = [&](const float* of, float (&to)[8]) {
-      const f32x4_t a = *reinterpret_cast<const f32x4_t*>(of + 8 * q), d = *reinterpret_cast<const f32x4_t*>(of + 8 * q + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        to[i] = a[i];
-        to[4 + i] = d[i];
-      }
-    };
     f32x4_t d[NT][2];
+    Split dd[NT];
     bool odd = false;
     {
       float beta[8], in[8];
-      scalars(ops.sc.beta, beta);
-      scalars(ops.sc.in, in);
+      eight_of(ops.sc.beta + 8 * q, beta);
+      eight_of(ops.sc.in + 8 * q, in);
       f16x8_t tf[2][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -727,7 +813,7 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
       for (int nt = 0; nt < NT; ++nt) {
         float right[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], v[nt][e] * inv[nt], -in[e] * ks[nt][e >> 2][e & 3]);
+        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], bf16_bits_to_f32(nv[nt][e]) * inv[nt], -in[e] * ks[nt][e >> 2][e & 3]);
         const Split two = split(right, one);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -735,45 +821,52 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
           d[nt][t] = mfma16x16x32(tf[1][t], two.hi, d[nt][t]);
           d[nt][t] = mfma16x16x32(tf[0][t], two.hi, d[nt][t]);
         }
-        float sum = 0.f;  // NaN where one of them is no number
+      }
+      if (c + 1 < chunks) load_v(c + 1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(d[nt][e >> 2][e & 3], 0.f, sum);
-        odd |= !(sum == 0.f);
+      for (int nt = 0; nt < NT; ++nt) {
+        float eight[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) eight[e] = d[nt][e >> 2][e & 3];
+        dd[nt] = split(eight, one);
+        odd |= no_numbers(dd[nt].hi);
       }
     }
     if (!__any(odd)) {
       float out[8], end[8];
-      scalars(ops.sc.out, out);
-      scalars(ops.sc.end, end);
+      eight_of(ops.sc.out + 8 * q, out);
+      eight_of(ops.sc.end + 8 * q, end);
       f16x8_t af[2][2];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int t = 0; t < 2; ++t) af[i][t] = f16x8(ops.a[i][t][lane]);
+      float* yr = yb + (size_t)t0 * ystep;
       Split ends[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float eight[8], decayed[8];
+        float decayed[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          eight[e] = d[nt][e >> 2][e & 3];
-          decayed[e] = eight[e] * end[e];
-        }
-        const Split two = split(eight, one);
+        for (int e = 0; e < 8; ++e) decayed[e] = d[nt][e >> 2][e & 3] * end[e];
         ends[nt] = split(decayed, one);
-        float* yr = yb + (size_t)(t0 + 8 * q) * ystep + col + 16 * nt;
         const float whole = qscale * scale[nt];
+        f32x4_t acc[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          f32x4_t acc;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = qs[nt][t][i] * out[4 * t + i];
-          acc = mfma16x16x32(af[0][t], two.lo, acc);
-          acc = mfma16x16x32(af[1][t], two.hi, acc);
-          acc = mfma16x16x32(af[0][t], two.hi, acc);
+          for (int i = 0; i < 4; ++i) acc[t][i] = qs[nt][t][i] * out[4 * t + i];
+          acc[t] = mfma16x16x32(af[0][t], dd[nt].lo, acc[t]);
+          acc[t] = mfma16x16x32(af[1][t], dd[nt].hi, acc[t]);
+          acc[t] = mfma16x16x32(af[0][t], dd[nt].hi, acc[t]);
+        }
+        uint32_t at = here(8 * q * yld + col * 4);
+        if (full) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (8 * q + 4 * t + i < live) yr[(4 * t + i) * ystep] = acc[i] * whole;
+          for (int e = 0; e < 8; ++e, at += yld) *at_bytes(yr + 16 * nt, at) = acc[e >> 2][e & 3] * whole;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e, at += yld)
+            if (8 * q + e < live) *at_bytes(yr + 16 * nt, at) = acc[e >> 2][e & 3] * whole;
         }
       }
       const float total = ops.sc.total;
@@ -803,37 +896,30 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
           }
         }
     } else {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st[nt][s][half][i] *= scale[nt];
-        scale[nt] = inv[nt] = 1.f;
-      }
-      for (int i = 0; i < live; ++i) {  // token by token
+      // Token by token, on the state in memory, where it ends up anyway: this path is rare, and held in registers it would cost
+      // the other one some.
+      put_state();
+      for (int i = 0; i < live; ++i) {
         const int tile = i >> 2 & 1, row = 4 * (i >> 3) + (i & 3) + 16 * q;
         const float decay = ops.sc.decay[i], kn = ops.sc.k[i], qn = ops.sc.q[i] * qscale, bt = ops.sc.beta[i];
-#pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float sum = 0.f;
+          float* mine = to + nt * 16 * kDk;
+          asm volatile("" ::: "memory");  // the state stays where it is
+          float sum = 0.f, yv = 0.f;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const f16x8_t w = f16x8(ops.k[tile][s][row]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf((float)w[e] * kn, st[nt][s][e >> 2][e & 3], sum);
+            for (int e = 0; e < 8; ++e) sum = fmaf((float)w[e] * kn, mine[s * 32 + e], sum);
           }
-          const float delta = bt * (bf16_bits_to_f32(vrow[(int64_t)(t0 + i) * ldq + nt * 16]) - decay * quads_sum(sum));
-          float yv = 0.f;
+          const float delta = bt * (bf16_bits_to_f32(vrow[(int64_t)(t0 + i) * ldq + col + nt * 16]) - decay * quads_sum(sum));
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const f16x8_t w = f16x8(ops.k[tile][s][row]), z = f16x8(ops.q[tile][s][row]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float x = fmaf((float)w[e] * kn, delta, st[nt][s][e >> 2][e & 3] * decay);
-              st[nt][s][e >> 2][e & 3] = x;
+              const float x = fmaf((float)w[e] * kn, delta, mine[s * 32 + e] * decay);
+              mine[s * 32 + e] = x;
               yv = fmaf((float)z[e] * qn, x, yv);
             }
           }
@@ -841,17 +927,12 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
           if (q == 0) yb[(size_t)(t0 + i) * ystep + col + 16 * nt] = yv;
         }
       }
+      asm volatile("" ::: "memory");
+      get_state(to);
     }
     lds_barrier();
   }
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-        *reinterpret_cast<f32x4_t*>(state + run.write * pool.stride + at + (size_t)nt * 16 * kDk + s * 32 + half * 4) =
-            st[nt][s][half] * scale[nt];
+  put_state();
 }
 
 template <int WC, int NT>
@@ -910,6 +991,8 @@ extern "C" int skinny_gdn_recurrence_batch(const uint16_t* qkv, int64_t ldq, con
   SKINNY_CHECK_ARG(H >= 1 && H <= 65535 && Hk >= 1 && H % Hk == 0 && ldq >= (int64_t)2 * Hk * Dk + (int64_t)H * Dv && ldab >= H,
                    "gdn_batch: bad shape H=%d Hk=%d ldq=%lld ldab=%lld", H, Hk, (long long)ldq, (long long)ldab);
   SKINNY_CHECK_ARG(skinny_aligned(qkv, 16) && ldq % 8 == 0, "gdn_batch: qkv rows must be 16-byte aligned");
+  SKINNY_CHECK_ARG(ldq < (1 << 25) && ldab < (1 << 25) && (int64_t)H * Dv < (1 << 25),
+                   "gdn_batch: rows too far apart");
   SKINNY_CHECK_ARG(skinny_aligned(b, 2) && skinny_aligned(a, 2) && skinny_aligned(A_log, 4) && skinny_aligned(dt_bias, 4) &&
                        skinny_aligned(y, 16),
                    "gdn_batch: misaligned buffer");
@@ -920,8 +1003,12 @@ extern "C" int skinny_gdn_recurrence_batch(const uint16_t* qkv, int64_t ldq, con
     auto chunks = [&](auto launch) {
       return launch(p, qkv, ldq, b, a, ldab, A_log, dt_bias, state, y, B, T, H, Hk, (hipStream_t)stream);
     };
+    // As many workgroups to a head as still find a CU each (their registers leave no room for two): us a call for 16, 32, 64 and
+    // 128 columns a workgroup, 1024 tokens of 32 heads: 1 sequence 67 / 68 / 75 / 91, 4 sequences 249 / 134 / 78 / 92, 8: 495 / 271 /
+    // 156 / 118.
     const int64_t heads = (int64_t)B * H;
-    return heads >= 256 ? chunks(launch_chunks<4, 2>) : heads >= 128 ? chunks(launch_chunks<4, 1>) : chunks(launch_chunks<2, 1>);
+    return heads > 128 ? chunks(launch_chunks<4, 2>) : heads > 64 ? chunks(launch_chunks<4, 1>) : heads > 32 ? chunks(launch_chunks<2, 1>)
+                                                                                                             : chunks(launch_chunks<1, 1>);
   }
   auto go = [&](auto kernel, int nc) {
     hipLaunchKernelGGL(kernel, dim3(H, kDv / (kStepGroups * nc), B), dim3(kStepThreads), 0, (hipStream_t)stream, p, qkv, ldq, b, a,
