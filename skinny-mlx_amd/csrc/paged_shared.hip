@@ -43,14 +43,12 @@ struct Shape {
 
 constexpr float kLag = 8.f;
 
-template <int D, int KW>
-__host__ __device__ constexpr int tile_keys() {
-  return 32 * (KW > 2 ? KW : 2);
-}
+// Keys of a tile: 64 KB of K and V for 128 and 256 dims, whose loads are in flight through a tile's products.
+__host__ __device__ constexpr int tile_keys(int D) { return D == 256 ? 64 : 128; }
 
 template <int D, int RT, int KW>
 __host__ __device__ constexpr int prefix_lds() {
-  const int tiles = 2 * 2 * tile_keys<D, KW>() * D * 2;                         // K and V, two buffers
+  const int tiles = 2 * 2 * tile_keys(D) * D * 2;                                 // K and V, two buffers
   const int join = KW > 1 ? 4 * 16 * RT * (D + 4) * 4 + 4 * 16 * RT * 2 * 4 : 0;  // the waves' outputs, maxima and sums
   return tiles > join ? tiles : join;
 }
@@ -59,16 +57,26 @@ template <int D, int RT, int KW>
 __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, const uint16_t* __restrict__ q, int rows, int TG,
                                                         int G, int Hq, int Hkv, float scale, int span, int slots,
                                                         float* __restrict__ part_o, float* __restrict__ part_ml) {
-  constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, TK = tile_keys<D, KW>();
+  constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, TK = tile_keys(D);
   constexpr int ST = TK / 32;        // 32-key steps of a tile
   constexpr int NF = TK * D / 512;   // 1 KB operands of K, and of V, in a tile
-  constexpr int FW = NF / 4;         // a wave's share of them
+  constexpr int FW = NF / 4;         // a wave's share of them, all of one step
   extern __shared__ u32x4_t lds[];   // [buffer][K operands, V operands][lane]
   const int h = blockIdx.x, slot = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
   const int kw = wave % KW, row0 = ((int)blockIdx.y * (4 / KW) + wave / KW) * (16 * RT);
+  // The pages of a wave's step of a tile: its first sixteen keys' and the others'. Asked for a tile before they are used.
+  const words_t table = words(px.pages);
+  const int step = 32 * (wave * ST / 4);  // of the tile
+  int id[2];
+  auto find = [&](int key0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) id[i] = table[min((key0 + step + 16 * i) >> pg.log2p, px.max_pages - 1)];
+  };
+  const int begin = slot * span;
+  find(begin);
   const int len = prefix_length(px);
-  const int begin = slot * span, end = min(begin + span, len);
+  const int end = min(begin + span, len);
   if (begin >= end) return;
   const float sc = scale * kPLog2e;
   // a flat row's sequence and row of that sequence's T * G
@@ -76,6 +84,58 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
     b = r / TG;
     in = r - b * TG;
   };
+  const int P = 1 << pg.log2p;
+  const uint16_t* k_head = pg.k + (size_t)h * P * D;
+  const uint16_t* v_head = pg.vt + (size_t)h * D * P;
+  u32x4_t kr[FW], vr[FW];
+  bool bad = false;  // a page of the run that is none: every row of it is NaN
+  // Operand f of a tile's K: step f / (2 KS), half a of its keys, dims 32 ks on. Row r of the half's product is key
+  // 8 (r / 4) + 4a + r % 4 of the step. Of its V: step f / DT, dims 16 dt on.
+  const uint32_t k_lane = (8 * (col >> 2) + (col & 3)) * D + quad * 8, v_lane = col * P + 8 * quad;
+  int tail = 0;  // of the loaded tile: the lane's V pieces' keys, where some are past the prefix
+  bool edge = false;
+  auto load = [&](int key0) {
+    const int first = key0 + step;
+    uint64_t kp[2], vp[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool ok = (unsigned)id[i] < (unsigned)pg.n_pages;
+      bad |= !ok && first + 16 * i < len;
+      const uint64_t page = ok ? (uint32_t)id[i] : 0u;
+      // keys of a page of 16 begin at its first slot; larger pages hold the whole step
+      const int in = (first & (P - 1)) - (P == 16 ? 16 * i : 0);
+      kp[i] = page * pg.k_stride + (int64_t)in * D;
+      vp[i] = page * pg.vt_stride + (int64_t)in;
+    }
+    const uint16_t* ka = k_head + (col >= 8 ? kp[1] : kp[0]);
+    const uint16_t* va = v_head + (quad >= 2 ? vp[1] : vp[0]);
+#pragma unroll
+    for (int i = 0; i < FW; ++i) {
+      const int f = (wave * FW) % (2 * KS) + i;  // (a multiple of 2 KS if FW is)
+      const int a = FW >= 2 * KS ? i / KS : f / KS, ks = i % KS;
+      kr[i] = *reinterpret_cast<const u32x4_t*>(ka + (k_lane + (uint32_t)(4 * a * D + ks * 32)));
+    }
+#pragma unroll
+    for (int i = 0; i < FW; ++i) {
+      const int dt = FW >= DT ? i : (wave * FW) % DT + i;
+      vr[i] = *reinterpret_cast<const u32x4_t*>(va + (v_lane + (uint32_t)(dt * 16 * P)));
+    }
+    edge = first + 32 > len;
+    tail = min(max(len - first - 8 * quad, 0), 8);
+  };
+  auto stage = [&](int buf) {
+    u32x4_t* to = lds + (size_t)buf * 2 * NF * 64 + wave * FW * 64 + lane;
+    if (edge) {  // slots past the prefix hold anything, and 0 * NaN is NaN
+#pragma unroll
+      for (int i = 0; i < FW; ++i) vr[i] = first_keys(vr[i], tail);
+    }
+#pragma unroll
+    for (int i = 0; i < FW; ++i) {
+      to[i * 64] = kr[i];
+      to[(NF + i) * 64] = vr[i];
+    }
+  };
+  load(begin);
   bf16x8_t qf[RT][KS];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -86,148 +146,128 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
   }
-  const int P = 1 << pg.log2p;
-  const uint16_t* k_head = pg.k + (size_t)h * P * D;
-  const uint16_t* v_head = pg.vt + (size_t)h * D * P;
-  u32x4_t kr[FW], vr[FW];
-  // Operand f of a tile's K: step f / (2 KS), half a of its keys, dims 32 ks on. Row r of the half's product is key
-  // 8 (r / 4) + 4a + r % 4 of the step. Of its V: step f / DT, dims 16 dt on.
-  auto page_at = [&](int key, bool& bad) {  // of a key below the tile's end; past the prefix: any page that is one
-    const int id = words(px.pages)[min(key >> pg.log2p, px.max_pages - 1)];
-    const bool ok = (unsigned)id < (unsigned)pg.n_pages;
-    bad = !ok && key < len;
-    return ok ? id : 0;
-  };
-  auto load = [&](int key0) {
-#pragma unroll
-    for (int i = 0; i < FW; ++i) {
-      const int f = wave * FW + i;
-      {
-        const int s = f / (2 * KS), a = f / KS % 2, ks = f % KS;
-        const int step = key0 + 32 * s;
-        bool bad0, bad1;
-        const int p0 = page_at(step, bad0), p1 = page_at(step + 16, bad1);
-        const bool second = col >= 8;
-        const int in = (step + 8 * (col >> 2) + 4 * a + (col & 3)) & (P - 1);
-        const uint16_t* at = k_head + (uint64_t)(uint32_t)(second ? p1 : p0) * pg.k_stride + (uint32_t)(in * D + ks * 32 + quad * 8);
-        u32x4_t v = *reinterpret_cast<const u32x4_t*>(at);
-        if (second ? bad1 : bad0) v = u32x4_t{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-        kr[i] = v;
-      }
-      {
-        const int s = f / DT, dt = f % DT;
-        const int step = key0 + 32 * s;
-        bool bad0, bad1;
-        const int p0 = page_at(step, bad0), p1 = page_at(step + 16, bad1);
-        const bool second = quad >= 2;
-        const int key = step + 8 * quad;
-        const uint16_t* at = v_head + (uint64_t)(uint32_t)(second ? p1 : p0) * pg.vt_stride + (uint32_t)((dt * 16 + col) * P + (key & (P - 1)));
-        vr[i] = first_keys(*reinterpret_cast<const u32x4_t*>(at), (second ? bad1 : bad0) ? 0 : min(max(len - key, 0), 8));
-      }
-    }
-  };
-  auto stage = [&](int buf) {
-    u32x4_t* to = lds + (size_t)buf * 2 * NF * 64;
-#pragma unroll
-    for (int i = 0; i < FW; ++i) {
-      to[(wave * FW + i) * 64 + lane] = kr[i];
-      to[(NF + wave * FW + i) * 64 + lane] = vr[i];
-    }
-  };
-  float m[RT], l[RT];
-  f32x4_t o[RT][DT];
+  float m[RT];
+  f32x4_t o[RT][DT], sum[RT];  // (sum: of a row's weights, in all four)
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -INFINITY;
-    l[rt] = 0.f;
+    sum[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  load(begin);
+  if (begin + TK < end) find(begin + TK);
   stage(0);
-  __syncthreads();
-  for (int key0 = begin, buf = 0; key0 < end; key0 += TK, buf ^= 1) {
-    const bool more = key0 + TK < end;
-    if (more) load(key0 + TK);
-    const u32x4_t* kt = lds + (size_t)buf * 2 * NF * 64 + lane;
-    const u32x4_t* vt = kt + NF * 64;
+  lds_barrier();
+  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, u32x4_t{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  constexpr int SW = ST / KW;  // a wave's steps of a tile
+  const int steps = (end - begin + TK - 1) / TK * SW;
+  // Scores of step `at`, past the run's end -inf.
+  auto scores = [&](int at, f32x4_t (&acc)[RT][2]) {
+    const int s = at % SW * KW + kw, tile = at / SW;
+    const u32x4_t* kt = lds + (size_t)(tile & 1) * 2 * NF * 64 + s * (2 * KS * 64) + lane;
 #pragma unroll
-    for (int s0 = 0; s0 < ST / KW; ++s0) {
-      const int s = s0 * KW + kw;
-      f32x4_t acc[RT][2];
+    for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int ks = 0; ks < KS; ++ks) {
+        const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, kt[(a * KS + ks) * 64]);
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, kt[((s * 2 + a) * KS + ks) * 64]);
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) acc[rt][a] = mfma16x16x32(kf, qf[rt][ks], acc[rt][a]);
-        }
-      const int left = end - (key0 + 32 * s + 8 * quad);  // of the lane's eight keys, those below the run's end
-      if (key0 + 32 * s + 32 > end) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e >= left) acc[rt][e >> 2][e & 3] = -INFINITY;
+        for (int rt = 0; rt < RT; ++rt) acc[rt][a] = mfma16x16x32(kf, qf[rt][ks], acc[rt][a]);
       }
-      float top[RT];
+    const int left = end - (begin + tile * TK + 32 * s);
+    if (left < 32) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (8 * quad + e >= left) acc[rt][e >> 2][e & 3] = -INFINITY;
+    }
+  };
+  int at = 0, loaded = 0;
+  bool fresh = false;  // the maximum has been raised for this very step
+  for (;;) {
+    // Steps that need no new maximum. (Its raise, which scales the outputs, stands outside this loop: on a branch inside it, the
+    // compiler keeps the outputs in other registers, and moves all of them in every step that does not take it.)
+    while (at < steps) {
+      const int tile = at / SW;
+      const bool more = begin + (tile + 1) * TK < end;
+      if (loaded == tile && more) {
+        load(begin + (tile + 1) * TK);
+        if (begin + (tile + 2) * TK < end) find(begin + (tile + 2) * TK);
+        loaded = tile + 1;
+      }
+      f32x4_t acc[RT][2];
+      scores(at, acc);
+      float t[RT][8];  // over the running maximum, in log2 units
       bool up = false;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float mx = acc[rt][0][0];
+        const float ref = m[rt] == -INFINITY ? 0.f : m[rt];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, acc[rt][e >> 2][e & 3]);
-        top[rt] = mx * sc;
-        up |= top[rt] > m[rt] + kLag;
+        for (int e = 0; e < 8; ++e) t[rt][e] = fmaf(acc[rt][e >> 2][e & 3], sc, -ref);
+        const float top = fmaxf(fmaxf(fmaxf(t[rt][0], t[rt][1]), fmaxf(t[rt][2], t[rt][3])),
+                                fmaxf(fmaxf(t[rt][4], t[rt][5]), fmaxf(t[rt][6], t[rt][7])));
+        up |= top > (m[rt] == -INFINITY ? -INFINITY : kLag);
       }
-      if (__any(up)) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const float nm = fmaxf(m[rt], quads_max(top[rt]));
-          const float f = __builtin_amdgcn_exp2f(m[rt] - (nm == -INFINITY ? 0.f : nm));
-          m[rt] = nm;
-          l[rt] *= f;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[rt][dt][i] *= f;
-        }
-      }
+      if (!fresh && __any(up)) break;
+      fresh = false;
       bf16x8_t pf[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const float ref = m[rt] == -INFINITY ? 0.f : m[rt];
         u32x4_t p;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(acc[rt][w >> 1][2 * (w & 1)], sc, -ref));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(acc[rt][w >> 1][2 * (w & 1) + 1], sc, -ref));
-          p[w] = two_bf16(p0, p1);
-          l[rt] += __uint_as_float(p[w] << 16);
-          l[rt] += __uint_as_float(p[w] & 0xffff0000u);
-        }
+        for (int w = 0; w < 4; ++w)
+          p[w] = two_bf16(__builtin_amdgcn_exp2f(t[rt][2 * w]), __builtin_amdgcn_exp2f(t[rt][2 * w + 1]));
         pf[rt] = __builtin_bit_cast(bf16x8_t, p);
+        sum[rt] = mfma16x16x32(ones, pf[rt], sum[rt]);
       }
+      const u32x4_t* vt = lds + ((size_t)(tile & 1) * 2 + 1) * NF * 64 + (at % SW * KW + kw) * (DT * 64) + lane;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, vt[(s * DT + dt) * 64]);
+        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, vt[dt * 64]);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma16x16x32(vf, pf[rt], o[rt][dt]);
       }
+      if (++at % SW == 0) {
+        if (more) stage((tile + 1) & 1);
+        lds_barrier();
+      }
     }
-    if (more) stage(buf ^ 1);
-    __syncthreads();
+    if (at == steps) break;
+    f32x4_t acc[RT][2];
+    scores(at, acc);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float top = acc[rt][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, acc[rt][e >> 2][e & 3]);
+      const float nm = fmaxf(m[rt], quads_max(top) * sc), f = __builtin_amdgcn_exp2f(m[rt] - (nm == -INFINITY ? 0.f : nm));
+      m[rt] = nm;
+      sum[rt] *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[rt][dt][i] *= f;
+    }
+    fresh = true;
   }
+  // A page that was none, met by any wave.
+  int* flag = reinterpret_cast<int*>(lds);
+  if (threadIdx.x == 0) *flag = 0;
+  lds_barrier();
+  if (bad) *flag = 1;
+  lds_barrier();
+  const bool none = *flag != 0;
+  lds_barrier();
+  float l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) l[rt] = none ? __builtin_nanf("") : sum[rt][0];
   auto part_at = [&](int r) {
     int b, in;
     row_of(r, b, in);
     return (((size_t)b * Hkv + h) * slots + slot) * (size_t)TG + in;
   };
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) l[rt] = quads_sum(l[rt]);
   if constexpr (KW == 1) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -240,11 +280,11 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
     }
   } else {
     // The KW waves of a row group joined in their order.
-    float* sum = reinterpret_cast<float*>(lds);                       // [wave][16 RT][D + 4]
-    float2* ml = reinterpret_cast<float2*>(sum + 4 * 16 * RT * (D + 4));  // [wave][16 RT]
+    float* out = reinterpret_cast<float*>(lds);                       // [wave][16 RT][D + 4]
+    float2* ml = reinterpret_cast<float2*>(out + 4 * 16 * RT * (D + 4));  // [wave][16 RT]
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float* mine = sum + ((size_t)wave * 16 * RT + 16 * rt + col) * (D + 4);
+      float* mine = out + ((size_t)wave * 16 * RT + 16 * rt + col) * (D + 4);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(mine + dt * 16 + quad * 4) = o[rt][dt];
       if (quad == 0) ml[wave * 16 * RT + 16 * rt + col] = float2{m[rt], l[rt]};
@@ -260,7 +300,7 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
       for (int w = 0; w < KW; ++w) {
         const int at = (group * KW + w) * 16 * RT + in;
         const float2 x = ml[at];
-        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(sum + (size_t)at * (D + 4) + d);
+        const f32x4_t v = *reinterpret_cast<const f32x4_t*>(out + (size_t)at * (D + 4) + d);
         const Join j = join(rm, rl, x.x, x.y);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ro[e] = fmaf(v[e], j.part, ro[e] * j.before);
@@ -355,7 +395,7 @@ Cut prefix_cut(int rows, int Hkv, int D, int prefix_keys) {
     c.rt = rows > 32 ? 4 : rows > 16 ? 2 : 1;
     c.kw = rows > 128 ? 1 : rows > 64 ? 2 : 4;
   }
-  const int block = 16 * c.rt * 4 / c.kw, tile = 32 * (c.kw > 2 ? c.kw : 2);
+  const int block = 16 * c.rt * 4 / c.kw, tile = tile_keys(D);
   c.row_blocks = (rows + block - 1) / block;
   const int tiles = (prefix_keys + tile - 1) / tile;
   int64_t runs = 256 / ((int64_t)Hkv * c.row_blocks);
