@@ -46,28 +46,28 @@ constexpr float kLag = 8.f;
 // Keys of a tile: 64 KB of K and V for 128 and 256 dims, whose loads are in flight through a tile's products.
 __host__ __device__ constexpr int tile_keys(int D) { return D == 256 ? 64 : 128; }
 
-template <int D, int RT, int KW>
+template <int D, int RT, int KW, int NW>
 __host__ __device__ constexpr int prefix_lds() {
-  const int tiles = 2 * 2 * tile_keys(D) * D * 2;                                 // K and V, two buffers
-  const int join = KW > 1 ? 4 * 16 * RT * (D + 4) * 4 + 4 * 16 * RT * 2 * 4 : 0;  // the waves' outputs, maxima and sums
+  const int tiles = 2 * 2 * tile_keys(D) * D * 2;                                   // K and V, two buffers
+  const int join = KW > 1 ? NW * 16 * RT * (D + 4) * 4 + NW * 16 * RT * 2 * 4 : 0;  // the waves' outputs, maxima and sums
   return tiles > join ? tiles : join;
 }
 
-template <int D, int RT, int KW>
-__global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, const uint16_t* __restrict__ q, int rows, int TG,
-                                                        int G, int Hq, int Hkv, float scale, int span, int slots,
+template <int D, int RT, int KW, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void prefix_kernel(Pages pg, Prefix px, const uint16_t* __restrict__ q, int rows, int TG,
+                                                        int G, int Hq, int Hkv, float scale, int span,
                                                         float* __restrict__ part_o, float* __restrict__ part_ml) {
   constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, TK = tile_keys(D);
   constexpr int ST = TK / 32;        // 32-key steps of a tile
   constexpr int NF = TK * D / 512;   // 1 KB operands of K, and of V, in a tile
-  constexpr int FW = NF / 4;         // a wave's share of them, all of one step
+  constexpr int FW = NF / NW;        // a wave's share of them, all of one step
   extern __shared__ u32x4_t lds[];   // [buffer][K operands, V operands][lane]
   const int h = blockIdx.x, slot = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int kw = wave % KW, row0 = ((int)blockIdx.y * (4 / KW) + wave / KW) * (16 * RT);
+  const int kw = wave % KW, row0 = ((int)blockIdx.y * (NW / KW) + wave / KW) * (16 * RT);
   // The pages of a wave's step of a tile: its first sixteen keys' and the others'. Asked for a tile before they are used.
   const words_t table = words(px.pages);
-  const int step = 32 * (wave * ST / 4);  // of the tile
+  const int step = 32 * (wave * ST / NW);  // of the tile
   int id[2];
   auto find = [&](int key0) {
 #pragma unroll
@@ -263,17 +263,13 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
   float l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) l[rt] = none ? __builtin_nanf("") : sum[rt][0];
-  auto part_at = [&](int r) {
-    int b, in;
-    row_of(r, b, in);
-    return (((size_t)b * Hkv + h) * slots + slot) * (size_t)TG + in;
-  };
+  const size_t part0 = ((size_t)slot * Hkv + h) * rows;  // parts: [run][kv head][row]
   if constexpr (KW == 1) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const int r = row0 + 16 * rt + col;
       if (r >= rows) continue;
-      const size_t at = part_at(r);
+      const size_t at = part0 + r;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * D + dt * 16 + quad * 4) = o[rt][dt];
       if (quad == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{m[rt], l[rt]};
@@ -281,7 +277,7 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
   } else {
     // The KW waves of a row group joined in their order.
     float* out = reinterpret_cast<float*>(lds);                       // [wave][16 RT][D + 4]
-    float2* ml = reinterpret_cast<float2*>(out + 4 * 16 * RT * (D + 4));  // [wave][16 RT]
+    float2* ml = reinterpret_cast<float2*>(out + NW * 16 * RT * (D + 4));  // [wave][16 RT]
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float* mine = out + ((size_t)wave * 16 * RT + 16 * rt + col) * (D + 4);
@@ -305,7 +301,7 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
 #pragma unroll
         for (int e = 0; e < 4; ++e) ro[e] = fmaf(v[e], j.part, ro[e] * j.before);
       }
-      const size_t at = part_at(r);
+      const size_t at = part0 + r;
       *reinterpret_cast<f32x4_t*>(part_o + at * D + d) = ro;
       if (d == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{rm, rl};
     }
@@ -316,8 +312,8 @@ __global__ __launch_bounds__(256, 1) void prefix_kernel(Pages pg, Prefix px, con
 // order. Bound by latency for few rows, by the parts' bytes for many.
 template <int D, int W>
 __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void shared_merge_kernel(Pages pg, Prefix px, int T, int Hq, int G, int Hkv,
-                                                                            int room, int span, int first, int own_keys,
-                                                                            int slots, const float* __restrict__ part_o,
+                                                                            int room, int span, int own_keys, int slots,
+                                                                            size_t first, const float* __restrict__ part_o,
                                                                             const float* __restrict__ part_ml, Out o) {
   constexpr int E = D / 64, UN = 8;
   typedef float dims_t __attribute__((ext_vector_type(E)));
@@ -338,8 +334,10 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void shared_merge_kernel(Page
     return;
   }
   const int np = (len + span - 1) / span, n = np + (sq.len + t) / own_keys + 1;  // parts of the prefix; and of its own keys
-  const size_t step = (size_t)T * G;
-  const size_t base = ((size_t)b * Hkv + head / G) * slots * step + (size_t)t * G + head % G;
+  // parts of the prefix [run][kv head][row], from `first` on those of the own keys [sequence][kv head][run][row of its T * G]
+  const int h = head / G;
+  const size_t TG = (size_t)T * G, in = (size_t)t * G + head % G;
+  const size_t rows = (size_t)gridDim.z * TG, front = h * rows + b * TG + in, own = first + ((size_t)b * Hkv + h) * slots * TG + in;
   float rm = -INFINITY, rl = 0.f;
   dims_t ro(0.f);
   for (int i0 = w; i0 < n; i0 += W * UN) {
@@ -348,7 +346,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void shared_merge_kernel(Page
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int i = min(i0 + u * W, n - 1);
-      const size_t at = base + (size_t)(i < np ? i : first + i - np) * step;
+      const size_t at = i < np ? front + (size_t)i * Hkv * rows : own + (size_t)(i - np) * TG;
       x[u] = reinterpret_cast<const float2*>(part_ml)[at];
       v[u] = *reinterpret_cast<const dims_t*>(part_o + at * D + E * lane);
     }
@@ -383,19 +381,21 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void shared_merge_kernel(Page
 
 // How the prefix is cut: row tiles a wave, waves that share a tile's keys, keys of a run (`span`) and runs (`slots`).
 struct Cut {
-  int rt, kw, row_blocks, span, slots;
+  int rt, kw, waves, row_blocks, span, slots;
 };
 
 Cut prefix_cut(int rows, int Hkv, int D, int prefix_keys) {
   Cut c;
   if (D == 256) {
+    c.waves = 4;
     c.rt = rows > 32 ? 2 : 1;
     c.kw = rows > 64 ? 1 : 2;
   } else {
-    c.rt = rows > 32 ? 4 : rows > 16 ? 2 : 1;
+    c.waves = rows > 16 ? 8 : 4;
+    c.rt = rows > 32 ? 2 : 1;
     c.kw = rows > 128 ? 1 : rows > 64 ? 2 : 4;
   }
-  const int block = 16 * c.rt * 4 / c.kw, tile = tile_keys(D);
+  const int block = 16 * c.rt * c.waves / c.kw, tile = tile_keys(D);
   c.row_blocks = (rows + block - 1) / block;
   const int tiles = (prefix_keys + tile - 1) / tile;
   int64_t runs = 256 / ((int64_t)Hkv * c.row_blocks);
@@ -408,8 +408,7 @@ Cut prefix_cut(int rows, int Hkv, int D, int prefix_keys) {
 struct Plan {
   Cut cut;
   Own own;
-  int slots;
-  size_t parts, bytes;
+  size_t front, parts, bytes;  // parts of the prefix, and in all
 };
 
 Plan plan_of(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys) {
@@ -417,25 +416,25 @@ Plan plan_of(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys) {
   const int G = Hq / Hkv;
   p.cut = prefix_cut(B * T * G, Hkv, D, prefix_keys);
   p.own = own_runs(B, T, Hq, Hkv, D, keys);
-  p.slots = p.cut.slots + p.own.slots;
-  p.parts = (size_t)B * Hkv * p.slots * T * G;
+  p.front = (size_t)B * Hkv * p.cut.slots * T * G;
+  p.parts = p.front + (size_t)B * Hkv * p.own.slots * T * G;
   p.bytes = p.parts * (D + 2) * sizeof(float);
   return p;
 }
 
-template <int D, int RT, int KW>
+template <int D, int RT, int KW, int NW>
 int launch_prefix(const Pages& pg, const Prefix& px, const uint16_t* q, int B, int T, int Hq, int Hkv, float scale, const Plan& p,
                   float* ws, float* ml, hipStream_t s) {
-  constexpr int bytes = prefix_lds<D, RT, KW>();
+  constexpr int bytes = prefix_lds<D, RT, KW, NW>();
   static_assert(bytes <= 160 * 1024, "a CU's LDS");
   const int G = Hq / Hkv;
   if (bytes > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_kernel<D, RT, KW>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_kernel<D, RT, KW, NW>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return skinny_set_error(SKINNY_ELAUNCH, "paged_attention_shared: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((prefix_kernel<D, RT, KW>), dim3(Hkv, p.cut.row_blocks, p.cut.slots), dim3(256), bytes, s, pg, px, q,
-                     B * T * G, T * G, G, Hq, Hkv, scale, p.cut.span, p.slots, ws, ml);
+  hipLaunchKernelGGL((prefix_kernel<D, RT, KW, NW>), dim3(Hkv, p.cut.row_blocks, p.cut.slots), dim3(64 * NW), bytes, s, pg, px, q,
+                     B * T * G, T * G, G, Hq, Hkv, scale, p.cut.span, ws, ml);
   return skinny_check_launch("paged_attention_shared prefix");
 }
 
@@ -444,28 +443,31 @@ int launch_shared(const Pages& pg, const Prefix& px, const uint16_t* q, int B, i
                   const Plan& p, float* ws, const Out& o, hipStream_t s) {
   float* ml = ws + p.parts * D;
   const Cut& c = p.cut;
-  auto prefix = [&](auto rt, auto kw) {
-    return launch_prefix<D, decltype(rt)::value, decltype(kw)::value>(pg, px, q, B, T, Hq, Hkv, scale, p, ws, ml, s);
+  auto prefix = [&](auto rt, auto kw, auto nw) {
+    return launch_prefix<D, decltype(rt)::value, decltype(kw)::value, decltype(nw)::value>(pg, px, q, B, T, Hq, Hkv, scale, p, ws, ml, s);
   };
-  using std::integral_constant;
+  using one = std::integral_constant<int, 1>;
+  using two = std::integral_constant<int, 2>;
+  using four = std::integral_constant<int, 4>;
+  using eight = std::integral_constant<int, 8>;
   int rc;
   if constexpr (D == 256) {
-    if (c.kw == 1) rc = prefix(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-    else if (c.rt == 2) rc = prefix(integral_constant<int, 2>{}, integral_constant<int, 2>{});
-    else rc = prefix(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+    if (c.kw == 1) rc = prefix(two{}, one{}, four{});
+    else if (c.rt == 2) rc = prefix(two{}, two{}, four{});
+    else rc = prefix(one{}, two{}, four{});
   } else {
-    if (c.kw == 1) rc = prefix(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-    else if (c.kw == 2) rc = prefix(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    else if (c.rt == 4) rc = prefix(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-    else if (c.rt == 2) rc = prefix(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-    else rc = prefix(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    if (c.waves == 4) rc = prefix(one{}, four{}, four{});
+    else if (c.kw == 1) rc = prefix(two{}, one{}, eight{});
+    else if (c.kw == 2) rc = prefix(two{}, two{}, eight{});
+    else if (c.rt == 2) rc = prefix(two{}, four{}, eight{});
+    else rc = prefix(one{}, four{}, eight{});
   }
   if (rc) return rc;
-  if ((rc = own_parts(pg, q, B, T, Hq, Hkv, D, keys, scale, c.slots, p.slots, ws, ml, s))) return rc;
+  if ((rc = own_parts(pg, q, B, T, Hq, Hkv, D, keys, scale, ws + p.front * D, ml + p.front * 2, s))) return rc;
   const bool split = (int64_t)B * T * Hq <= 1024;
   auto merge = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(split ? 512 : 256), 0, s, pg, px, T, Hq, Hq / Hkv, Hkv,
-                       keys, c.span, c.slots, p.own.span * p.own.block, p.slots, ws, ml, o);
+                       keys, c.span, p.own.span * p.own.block, p.own.slots, p.front, ws, ml, o);
   };
   if (split) merge(shared_merge_kernel<D, 8>);
   else merge(shared_merge_kernel<D, 1>);
