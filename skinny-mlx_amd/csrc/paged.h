@@ -120,13 +120,4 @@ inline int check_pages(const skinny_paged_kv* kv, int B, int T, int Hq, Pages& p
   return SKINNY_OK;
 }
 
-// The attention of each sequence's new tokens to its own pages, as parts for a merge (paged.hip): part i of the `slots` of a
-// sequence and kv head is its i-th run of `span` blocks, in paged.hip's order [sequence][kv head][run][row of its T * G].
-struct Own {
-  int span, slots, block;  // blocks of a run; runs; keys of a block
-};
-Own own_runs(int B, int T, int Hq, int Hkv, int D, int keys);
-int own_parts(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int D, int keys, float scale, float* part_o,
-              float* part_ml, hipStream_t s);
-
 }  // namespace paged

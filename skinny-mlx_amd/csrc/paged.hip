@@ -227,7 +227,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
                                                                              int G, int by_g, int Hq, int Hkv, int room,
                                                                              float scale, int span, int slots,
                                                                              float* __restrict__ part_o,
-                                                                             float* __restrict__ part_ml, Out o, bool parts) {
+                                                                             float* __restrict__ part_ml, Out o) {
   constexpr int BLK = paged_block(D), WAVES = paged_waves(D);
   constexpr int KT = BLK / 16 / WAVES, KS = D / 32;           // a wave's 16-key tiles; dim steps of a score
   constexpr int ST = BLK / 32, NG = BLK / GS;                 // a block's 32-key steps and pages
@@ -277,10 +277,10 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
   };
   find(c0);
   const Sequence sq = sequence_of(pg, b, T, room);
-  if (!parts && row0 == 0) {  // no merge follows: the rows that are no tokens are written here
-    const int live = sq.ok ? sq.count : 0;
-    for (int e = threadIdx.x; e < (T - live) * G * D; e += 64 * WAVES) {
-      const int t = live + e / (G * D);
+  if (slots == 1 && row0 == 0) {  // no merge follows: the rows that are no tokens are written here
+    const int first = sq.ok ? sq.count : 0;
+    for (int e = threadIdx.x; e < (T - first) * G * D; e += 64 * WAVES) {
+      const int t = first + e / (G * D);
       o.out[(((size_t)b * T + t) * Hq + h * G) * D + e % (G * D)] = sq.ok ? 0 : kNanBits;
     }
   }
@@ -561,7 +561,7 @@ __global__ __launch_bounds__(64 * paged_waves(D), 2) void paged_block_kernel(Pag
   for (int w = 0; w < W; ++w) {
     const int r = row0 + 16 * w + col, d0 = wave * 16 * DW + quad * 4;
     if (r >= rows) continue;
-    if (parts) {  // for the merge
+    if (slots > 1) {  // a part, for the merge
       const size_t at = (((size_t)b * Hkv + h) * slots + slot) * (size_t)(T * G) + r;
 #pragma unroll
       for (int dt = 0; dt < DW; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * D + d0 + dt * 16) = go[w][dt];
@@ -751,14 +751,15 @@ size_t paged_workspace(int B, int T, int Hq, int Hkv, int D, int keys) {
   return (size_t)B * Hkv * slots * T * (Hq / Hkv) * (D + 2) * sizeof(float);
 }
 
-// The blocks of `slots` runs, as parts or as outputs.
 template <int D>
-int launch_blocks(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, int span, int slots,
-                  bool parts, float* part_o, float* part_ml, const Out& o, hipStream_t s) {
+int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, float* ws,
+                           const Out& o, hipStream_t s) {
   const int G = Hq / Hkv, rows = T * G;
+  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows, D), slots = paged_slots(nblk, span);
+  float* ml = ws + (size_t)B * Hkv * slots * rows * D;
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(rows > 32 ? 2 * Hkv : Hkv, B, slots), dim3(64 * paged_waves(D)), 0, s, pg, q, T, G,
-                       65535 / G + 1, Hq, Hkv, keys, scale, span, slots, part_o, part_ml, o, parts);
+                       65535 / G + 1, Hq, Hkv, keys, scale, span, slots, ws, ml, o);
   };
   auto page = [&](auto w, auto h) {
     constexpr int W = decltype(w)::value;
@@ -770,16 +771,7 @@ int launch_blocks(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int 
   if (rows <= 16) page(std::integral_constant<int, 1>{}, std::false_type{});
   else if (rows <= 32) page(std::integral_constant<int, 2>{}, std::false_type{});
   else page(std::integral_constant<int, 2>{}, std::true_type{});
-  return skinny_check_launch("paged_attention");
-}
-
-template <int D>
-int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int keys, float scale, float* ws,
-                           const Out& o, hipStream_t s) {
-  const int G = Hq / Hkv, rows = T * G;
-  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, rows, D), slots = paged_slots(nblk, span);
-  float* ml = ws + (size_t)B * Hkv * slots * rows * D;
-  if (const int rc = launch_blocks<D>(pg, q, B, T, Hq, Hkv, keys, scale, span, slots, slots > 1, ws, ml, o, s)) return rc;
+  if (const int rc = skinny_check_launch("paged_attention")) return rc;
   if (slots == 1) return SKINNY_OK;
   const int groups = (nblk + kPGroup - 1) / kPGroup;
   // eight waves a row where the rows alone would not fill the card, and always for blocks
@@ -797,25 +789,6 @@ int launch_paged_attention(const Pages& pg, const uint16_t* q, int B, int T, int
 }
 
 }  // namespace
-
-namespace paged {
-
-Own own_runs(int B, int T, int Hq, int Hkv, int D, int keys) {
-  const int nblk = paged_blocks(keys, D), span = paged_span(B, Hkv, nblk, T * (Hq / Hkv), D);
-  return {span, paged_slots(nblk, span), paged_block(D)};
-}
-
-int own_parts(const Pages& pg, const uint16_t* q, int B, int T, int Hq, int Hkv, int D, int keys, float scale, float* part_o,
-              float* part_ml, hipStream_t s) {
-  const Own own = own_runs(B, T, Hq, Hkv, D, keys);
-  const Out none{nullptr, nullptr, 0, 0};
-  auto go = [&](auto launch) {
-    return launch(pg, q, B, T, Hq, Hkv, keys, scale, own.span, own.slots, true, part_o, part_ml, none, s);
-  };
-  return D == 64 ? go(launch_blocks<64>) : D == 128 ? go(launch_blocks<128>) : go(launch_blocks<256>);
-}
-
-}  // namespace paged
 
 extern "C" int skinny_paged_store_bf16(const uint16_t* qkv, int ldq, int B, int T, int Hq, int q_stride, int k_offset,
                                        int v_offset, const uint16_t* q_norm, const uint16_t* k_norm, float eps,

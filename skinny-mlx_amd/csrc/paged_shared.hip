@@ -4,8 +4,9 @@
 // No reference counterpart: the reference decodes one sequence (skinny_mlx/spec.py:98-156). Arithmetic of a layer as at
 // spec.py:24-29 (causal GQA attention, optionally output * sigmoid(gate)).
 //
-// A row's softmax over [the prefix; its own keys] is joined from parts: runs of the prefix's keys (prefix_kernel here, for all
-// rows), runs of its sequence's own blocks (paged.hip's kernel, unchanged), and a merge.
+// A row's softmax over [the prefix; its own keys] is joined from parts: runs of the prefix's keys, formed for all rows by
+// workgroups, and runs of a sequence's own keys, formed for its rows by single waves. Both are workgroups of one launch, so that
+// the first ones' products and the others' loads share the card; a second launch joins them.
 #include <type_traits>
 #include "paged.h"
 
@@ -53,18 +54,24 @@ __host__ __device__ constexpr int prefix_lds() {
   return tiles > join ? tiles : join;
 }
 
+// What both roles are given.
+struct Rows {
+  const uint16_t* q;
+  int B, T, G, Hq, Hkv;
+  float scale;
+  float *part_o, *part_ml;
+};
+
 template <int D, int RT, int KW, int NW>
-__global__ __launch_bounds__(64 * NW, NW / 4) void prefix_kernel(Pages pg, Prefix px, const uint16_t* __restrict__ q, int rows, int TG,
-                                                        int G, int Hq, int Hkv, float scale, int span,
-                                                        float* __restrict__ part_o, float* __restrict__ part_ml) {
+__device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, const Rows& x, int h, int row_block, int slot, int span) {
   constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, TK = tile_keys(D);
   constexpr int ST = TK / 32;        // 32-key steps of a tile
   constexpr int NF = TK * D / 512;   // 1 KB operands of K, and of V, in a tile
   constexpr int FW = NF / NW;        // a wave's share of them, all of one step
   extern __shared__ u32x4_t lds[];   // [buffer][K operands, V operands][lane]
-  const int h = blockIdx.x, slot = blockIdx.z;
+  const int G = x.G, TG = x.T * G, Hq = x.Hq, rows = x.B * TG;
   const int lane = threadIdx.x & 63, wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  const int kw = wave % KW, row0 = ((int)blockIdx.y * (NW / KW) + wave / KW) * (16 * RT);
+  const int kw = wave % KW, row0 = (row_block * (NW / KW) + wave / KW) * (16 * RT);
   // The pages of a wave's step of a tile: its first sixteen keys' and the others'. Asked for a tile before they are used.
   const words_t table = words(px.pages);
   const int step = 32 * (wave * ST / NW);  // of the tile
@@ -78,7 +85,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_kernel(Pages pg, Prefi
   const int len = prefix_length(px);
   const int end = min(begin + span, len);
   if (begin >= end) return;
-  const float sc = scale * kPLog2e;
+  const float sc = x.scale * kPLog2e;
   // a flat row's sequence and row of that sequence's T * G
   auto row_of = [&](int r, int& b, int& in) {
     b = r / TG;
@@ -142,7 +149,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_kernel(Pages pg, Prefi
     int b, in;
     row_of(min(row0 + 16 * rt + col, rows - 1), b, in);
     const int t = in / G;
-    const uint16_t* qp = q + (((size_t)b * (TG / G) + t) * Hq + h * G + in - t * G) * D + quad * 8;
+    const uint16_t* qp = x.q + (((size_t)b * x.T + t) * Hq + h * G + in - t * G) * D + quad * 8;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
   }
@@ -263,7 +270,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_kernel(Pages pg, Prefi
   float l[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) l[rt] = none ? __builtin_nanf("") : sum[rt][0];
-  const size_t part0 = ((size_t)slot * Hkv + h) * rows;  // parts: [run][kv head][row]
+  const size_t part0 = ((size_t)slot * x.Hkv + h) * rows;  // parts: [run][kv head][row]
   if constexpr (KW == 1) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -271,8 +278,8 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_kernel(Pages pg, Prefi
       if (r >= rows) continue;
       const size_t at = part0 + r;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(part_o + at * D + dt * 16 + quad * 4) = o[rt][dt];
-      if (quad == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{m[rt], l[rt]};
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(x.part_o + at * D + dt * 16 + quad * 4) = o[rt][dt];
+      if (quad == 0) reinterpret_cast<float2*>(x.part_ml)[at] = float2{m[rt], l[rt]};
     }
   } else {
     // The KW waves of a row group joined in their order.
@@ -295,16 +302,189 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void prefix_kernel(Pages pg, Prefi
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         const int at = (group * KW + w) * 16 * RT + in;
-        const float2 x = ml[at];
+        const float2 one = ml[at];
         const f32x4_t v = *reinterpret_cast<const f32x4_t*>(out + (size_t)at * (D + 4) + d);
-        const Join j = join(rm, rl, x.x, x.y);
+        const Join j = join(rm, rl, one.x, one.y);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ro[e] = fmaf(v[e], j.part, ro[e] * j.before);
       }
       const size_t at = part0 + r;
-      *reinterpret_cast<f32x4_t*>(part_o + at * D + d) = ro;
-      if (d == 0) reinterpret_cast<float2*>(part_ml)[at] = float2{rm, rl};
+      *reinterpret_cast<f32x4_t*>(x.part_o + at * D + d) = ro;
+      if (d == 0) reinterpret_cast<float2*>(x.part_ml)[at] = float2{rm, rl};
     }
+  }
+}
+
+// A wave takes a run of a sequence's own keys for 16 of its query rows of a kv head, 32 keys a step, K and V straight from memory
+// in the matrix cores' operand order; as soon as a step's scores (outputs) are formed, its K (V) registers take the next one's
+// loads. Bound by memory. P is the sum of two bf16 terms here, as in paged.hip: products are not what it waits for.
+template <int D>
+__device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, int h, int tile, int run, int runs, int run_keys, int room) {
+  constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT;
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  const int begin = run * run_keys;
+  const words_t table = words(pg.table + (size_t)b * pg.ld);
+  int id[2];  // the pages of a step's first sixteen keys and of the others
+  auto find = [&](int key0) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) id[i] = table[min((key0 + 16 * i) >> pg.log2p, pg.max_pages - 1)];
+  };
+  find(begin);
+  const Sequence sq = sequence_of(pg, b, x.T, room);
+  const int total = sq.len + sq.count, rows = sq.count * x.G;
+  if (!sq.ok || begin >= total || 16 * tile >= rows) return;
+  const int end = min(begin + run_keys, total);
+  const int r = 16 * tile + col, t = r / x.G;
+  const int last = r < rows ? sq.len + t : -1;  // the last key that this lane's row sees
+  bf16x8_t qf[KS];
+  {
+    const int in = min(r, rows - 1), token = in / x.G;
+    const uint16_t* qp = x.q + (((size_t)b * x.T + token) * x.Hq + h * x.G + in - token * x.G) * D + quad * 8;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
+  }
+  const int P = 1 << pg.log2p;
+  const uint16_t* k_head = pg.k + (size_t)h * P * D;
+  const uint16_t* v_head = pg.vt + (size_t)h * D * P;
+  const uint32_t k_lane = (8 * (col >> 2) + (col & 3)) * D + quad * 8, v_lane = col * P + 8 * quad;
+  bf16x8_t kf[2][KS];
+  u32x4_t vf[DT];
+  auto there = [&](int i) { return (unsigned)id[i] < (unsigned)pg.n_pages; };
+  auto slot_of = [&](int key0, int i) { return (key0 & (P - 1)) - (P == 16 ? 16 * i : 0); };
+  auto load_k = [&](int key0) {
+    uint64_t at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) at[i] = (there(i) ? (uint32_t)id[i] : 0u) * (uint64_t)pg.k_stride + (int64_t)slot_of(key0, i) * D;
+    const uint16_t* p = k_head + (col >= 8 ? at[1] : at[0]);
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[a][ks] = *reinterpret_cast<const bf16x8_t*>(p + (k_lane + (uint32_t)(4 * a * D + ks * 32)));
+  };
+  auto load_v = [&](int key0) {
+    uint64_t at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) at[i] = (there(i) ? (uint32_t)id[i] : 0u) * (uint64_t)pg.vt_stride + (int64_t)slot_of(key0, i);
+    const uint16_t* p = v_head + (quad >= 2 ? at[1] : at[0]);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) vf[dt] = *reinterpret_cast<const u32x4_t*>(p + (v_lane + (uint32_t)(dt * 16 * P)));
+  };
+  uint32_t bad = 0, bad_next = 0;  // halves of the step on a page that is none
+  auto missing = [&](int key0) { return (!there(0) && key0 < total ? 1u : 0u) | (!there(1) && key0 + 16 < total ? 2u : 0u); };
+  load_k(begin);
+  load_v(begin);
+  bad = missing(begin);
+  if (begin + 32 < end) find(begin + 32);
+  const float sc = x.scale * kPLog2e;
+  float m = -INFINITY, l = 0.f;
+  f32x4_t o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int key0 = begin; key0 < end; key0 += 32) {
+    const bool more = key0 + 32 < end;
+    const bool edge = key0 + 32 > sq.len + 1 || bad;  // some row does not see, or may not read, some key
+    f32x4_t acc[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      acc[a] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) acc[a] = mfma16x16x32(kf[a][ks], qf[ks], acc[a]);
+    }
+    if (more) {
+      bad_next = missing(key0 + 32);
+      load_k(key0 + 32);
+    }
+    float s[8];  // of keys 8 quad + e
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = acc[e >> 2][e & 3];
+    if (edge) {
+      const bool none = bad >> (quad >> 1) & 1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = key0 + 8 * quad + e > last ? -INFINITY : none ? __builtin_nanf("") : s[e];
+    }
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e]);
+    const float nm = fmaxf(m, quads_max(top) * sc), ref = nm == -INFINITY ? 0.f : nm, f = __builtin_amdgcn_exp2f(m - ref);
+    m = nm;
+    l *= f;
+    u32x4_t hi, lo;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * w], sc, -ref)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * w + 1], sc, -ref));
+      l += p0;
+      l += p1;
+      hi[w] = two_bf16(p0, p1);
+      lo[w] = two_bf16(p0 - __uint_as_float(hi[w] << 16), p1 - __uint_as_float(hi[w] & 0xffff0000u));
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[dt][i] *= f;
+    if (edge) {
+      // Slots past the sequence hold anything: zeroed, for 0 * NaN is NaN. So are new tokens' values that are no numbers, which no
+      // earlier row may meet: the outputs that see one become NaN instead, by a product of the odd values' and the seen keys' ones.
+      const int n = (bad >> (quad >> 1)) & 1 ? 0 : min(max(total - (key0 + 8 * quad), 0), 8);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vf[dt] = first_keys(vf[dt], n);
+      if (sq.count > 1 && any_not_finite(vf)) {
+        const u32x4_t one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        const bf16x8_t seen = __builtin_bit_cast(bf16x8_t, first_keys(one, min(max(last + 1 - (key0 + 8 * quad), 0), 8)));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          u32x4_t odd;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const uint32_t no = ((vf[dt][v] & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u;  // exponents of all ones
+            vf[dt][v] &= ~(no * 0xffffu);
+            odd[v] = no * 0x3f80u;
+          }
+          const f32x4_t met = mfma16x16x32(__builtin_bit_cast(bf16x8_t, odd), seen, f32x4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[dt][i] = met[i] > 0.f ? __builtin_nanf("") : o[dt][i];
+        }
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      o[dt] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, vf[dt]), __builtin_bit_cast(bf16x8_t, hi), o[dt]);
+      o[dt] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, vf[dt]), __builtin_bit_cast(bf16x8_t, lo), o[dt]);
+    }
+    if (more) {
+      load_v(key0 + 32);
+      if (key0 + 64 < end) find(key0 + 64);
+    }
+    bad = bad_next;
+  }
+  l = quads_sum(l);
+  if (r >= rows) return;
+  // parts: [sequence][kv head][run][row of its T * G]
+  const size_t at = (((size_t)b * x.Hkv + h) * runs + run) * (size_t)(x.T * x.G) + r;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(x.part_o + at * D + dt * 16 + quad * 4) = o[dt];
+  if (quad == 0) reinterpret_cast<float2*>(x.part_ml)[at] = float2{m, l};
+}
+
+// The prefix's workgroups first (a run's heads one after the other: the eight dies take workgroups in turn), then the own keys'
+// waves, the runs that a sequence turns out not to have last.
+template <int D, int RT, int KW, int NW>
+__global__ __launch_bounds__(64 * NW, NW / 4) void shared_parts_kernel(Pages pg, Prefix px, Rows x, int row_blocks, int span, int front,
+                                                                       int tiles, int runs, int run_keys, int room, float* own_o,
+                                                                       float* own_ml) {
+  const int i = blockIdx.x;
+  if (i < front) {
+    prefix_run<D, RT, KW, NW>(pg, px, x, i % x.Hkv, i / x.Hkv % row_blocks, i / x.Hkv / row_blocks, span);
+  } else {
+    uint32_t unit = __builtin_amdgcn_readfirstlane((uint32_t)(i - front) * NW + wave_id());
+    const uint32_t tile = unit % tiles;
+    unit /= tiles;
+    const uint32_t h = unit % x.Hkv;
+    unit /= x.Hkv;
+    const uint32_t b = unit % x.B, run = unit / x.B;
+    if ((int)run >= runs) return;
+    x.part_o = own_o;
+    x.part_ml = own_ml;
+    own_run<D>(pg, x, b, h, tile, run, runs, run_keys, room);
   }
 }
 
@@ -405,37 +585,57 @@ Cut prefix_cut(int rows, int Hkv, int D, int prefix_keys) {
   return c;
 }
 
+// A sequence's own keys: 16-row tiles of its rows, keys of a run, runs; enough waves to fill the card with loads (eight of 16 KB a
+// CU), and no shorter than four steps.
+struct Own {
+  int tiles, keys, runs;
+};
+
+Own own_cut(int B, int T, int G, int Hkv, int keys) {
+  Own o;
+  o.tiles = (T * G + 15) / 16;
+  const int64_t all = (int64_t)B * Hkv * o.tiles;
+  int64_t run = (all * keys / 2048 + 31) / 32 * 32;
+  if (run < 128) run = 128;
+  if (run > keys) run = (keys + 31) / 32 * 32;
+  o.keys = (int)run;
+  o.runs = (keys + o.keys - 1) / o.keys;
+  return o;
+}
+
 struct Plan {
   Cut cut;
   Own own;
-  size_t front, parts, bytes;  // parts of the prefix, and in all
+  int64_t prefix_groups, groups;  // workgroups
+  size_t front, parts, bytes;     // parts of the prefix, and in all
 };
 
 Plan plan_of(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys) {
   Plan p;
   const int G = Hq / Hkv;
   p.cut = prefix_cut(B * T * G, Hkv, D, prefix_keys);
-  p.own = own_runs(B, T, Hq, Hkv, D, keys);
+  p.own = own_cut(B, T, G, Hkv, keys);
+  p.prefix_groups = (int64_t)Hkv * p.cut.row_blocks * p.cut.slots;
+  p.groups = p.prefix_groups + ((int64_t)B * Hkv * p.own.tiles * p.own.runs + p.cut.waves - 1) / p.cut.waves;
   p.front = (size_t)B * Hkv * p.cut.slots * T * G;
-  p.parts = p.front + (size_t)B * Hkv * p.own.slots * T * G;
+  p.parts = p.front + (size_t)B * Hkv * p.own.runs * T * G;
   p.bytes = p.parts * (D + 2) * sizeof(float);
   return p;
 }
 
 template <int D, int RT, int KW, int NW>
-int launch_prefix(const Pages& pg, const Prefix& px, const uint16_t* q, int B, int T, int Hq, int Hkv, float scale, const Plan& p,
-                  float* ws, float* ml, hipStream_t s) {
+int launch_parts(const Pages& pg, const Prefix& px, const Rows& x, int keys, const Plan& p, hipStream_t s) {
   constexpr int bytes = prefix_lds<D, RT, KW, NW>();
   static_assert(bytes <= 160 * 1024, "a CU's LDS");
-  const int G = Hq / Hkv;
   if (bytes > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(prefix_kernel<D, RT, KW, NW>),
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_parts_kernel<D, RT, KW, NW>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return skinny_set_error(SKINNY_ELAUNCH, "paged_attention_shared: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
   }
-  hipLaunchKernelGGL((prefix_kernel<D, RT, KW, NW>), dim3(Hkv, p.cut.row_blocks, p.cut.slots), dim3(64 * NW), bytes, s, pg, px, q,
-                     B * T * G, T * G, G, Hq, Hkv, scale, p.cut.span, ws, ml);
-  return skinny_check_launch("paged_attention_shared prefix");
+  hipLaunchKernelGGL((shared_parts_kernel<D, RT, KW, NW>), dim3((uint32_t)p.groups), dim3(64 * NW), bytes, s, pg, px, x,
+                     p.cut.row_blocks, p.cut.span, (int)p.prefix_groups, p.own.tiles, p.own.runs, p.own.keys, keys,
+                     x.part_o + p.front * D, x.part_ml + p.front * 2);
+  return skinny_check_launch("paged_attention_shared parts");
 }
 
 template <int D>
@@ -443,8 +643,9 @@ int launch_shared(const Pages& pg, const Prefix& px, const uint16_t* q, int B, i
                   const Plan& p, float* ws, const Out& o, hipStream_t s) {
   float* ml = ws + p.parts * D;
   const Cut& c = p.cut;
-  auto prefix = [&](auto rt, auto kw, auto nw) {
-    return launch_prefix<D, decltype(rt)::value, decltype(kw)::value, decltype(nw)::value>(pg, px, q, B, T, Hq, Hkv, scale, p, ws, ml, s);
+  const Rows x{q, B, T, Hq / Hkv, Hq, Hkv, scale, ws, ml};
+  auto parts = [&](auto rt, auto kw, auto nw) {
+    return launch_parts<D, decltype(rt)::value, decltype(kw)::value, decltype(nw)::value>(pg, px, x, keys, p, s);
   };
   using one = std::integral_constant<int, 1>;
   using two = std::integral_constant<int, 2>;
@@ -452,22 +653,21 @@ int launch_shared(const Pages& pg, const Prefix& px, const uint16_t* q, int B, i
   using eight = std::integral_constant<int, 8>;
   int rc;
   if constexpr (D == 256) {
-    if (c.kw == 1) rc = prefix(two{}, one{}, four{});
-    else if (c.rt == 2) rc = prefix(two{}, two{}, four{});
-    else rc = prefix(one{}, two{}, four{});
+    if (c.kw == 1) rc = parts(two{}, one{}, four{});
+    else if (c.rt == 2) rc = parts(two{}, two{}, four{});
+    else rc = parts(one{}, two{}, four{});
   } else {
-    if (c.waves == 4) rc = prefix(one{}, four{}, four{});
-    else if (c.kw == 1) rc = prefix(two{}, one{}, eight{});
-    else if (c.kw == 2) rc = prefix(two{}, two{}, eight{});
-    else if (c.rt == 2) rc = prefix(two{}, four{}, eight{});
-    else rc = prefix(one{}, four{}, eight{});
+    if (c.waves == 4) rc = parts(one{}, four{}, four{});
+    else if (c.kw == 1) rc = parts(two{}, one{}, eight{});
+    else if (c.kw == 2) rc = parts(two{}, two{}, eight{});
+    else if (c.rt == 2) rc = parts(two{}, four{}, eight{});
+    else rc = parts(one{}, four{}, eight{});
   }
   if (rc) return rc;
-  if ((rc = own_parts(pg, q, B, T, Hq, Hkv, D, keys, scale, ws + p.front * D, ml + p.front * 2, s))) return rc;
   const bool split = (int64_t)B * T * Hq <= 1024;
   auto merge = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(split ? 512 : 256), 0, s, pg, px, T, Hq, Hq / Hkv, Hkv,
-                       keys, c.span, p.own.span * p.own.block, p.own.slots, p.front, ws, ml, o);
+                       keys, c.span, p.own.keys, p.own.runs, p.front, ws, ml, o);
   };
   if (split) merge(shared_merge_kernel<D, 8>);
   else merge(shared_merge_kernel<D, 1>);
@@ -507,8 +707,7 @@ extern "C" int skinny_paged_attention_shared_bf16(const uint16_t* q, int B, int 
                    "%s: misaligned buffer", what);
   SKINNY_CHECK_ARG(scale > 0.f && scale <= 1e38f, "%s: scale=%g must be positive", what, (double)scale);
   const Plan p = plan_of(B, T, Hq, Hkv, D, prefix_keys, keys);
-  SKINNY_CHECK_ARG(p.own.slots <= 65535 && p.cut.slots <= 65535 && p.cut.row_blocks <= 65535, "%s: keys=%d, prefix_keys=%d",
-                   what, keys, prefix_keys);
+  SKINNY_CHECK_ARG(p.groups <= 0x7fffffff / 8, "%s: keys=%d, prefix_keys=%d of B=%d sequences", what, keys, prefix_keys, B);
   SKINNY_CHECK_ARG(workspace && workspace_bytes >= p.bytes, "%s: workspace of %zu bytes, needs %zu", what,
                    workspace ? workspace_bytes : (size_t)0, p.bytes);
   const Prefix px{prefix, prefix_pages, max_prefix_pages, prefix_keys};
