@@ -8,6 +8,7 @@
 // workgroups, and runs of a sequence's own keys, formed for its rows by single waves. Both are workgroups of one launch, so that
 // the first ones' products and the others' loads share the card; a second launch joins them.
 #include <type_traits>
+#include <cmath>
 #include "paged.h"
 
 using namespace paged;
@@ -26,10 +27,11 @@ __device__ __forceinline__ int prefix_length(const Prefix& p) {
   return n >= 0 && n <= p.room ? n : -1;
 }
 
-// A workgroup of four waves takes 16 * RT * 4 / KW query rows of a kv head (every sequence's, one after the other) and a run of
-// the prefix: 4 / KW groups of 16 * RT rows, in each of which KW waves share a tile's keys. A tile of keys is staged in LDS in
-// the matrix cores' operand order (a lane's 16 bytes after its neighbour's: no bank conflicts) and read by all the row groups;
-// the next tile's loads are in flight meanwhile. Scores are formed transposed, S^T = K Q^T, with the K rows of a 32-key step
+// A workgroup of NW waves takes 16 * RT * NW / KW query rows of a kv head (every sequence's, one after the other) and a run of
+// the prefix: NW / KW groups of 16 * RT rows, in each of which KW waves share a tile's keys. A tile of keys is staged in LDS as
+// the matrix cores' operands and read by all the row groups; the next tile's loads are in flight meanwhile. Four lanes in a row
+// load 64 bytes of a K (V) row at once (a row a lane: 96.8 us where this takes 93.7, 64 sequences of 500 behind 32768 tokens) and
+// put them where the lanes that want them read without bank conflicts: the 16 rows of an operand's quad q in order row ^ 4q. Scores are formed transposed, S^T = K Q^T, with the K rows of a 32-key step
 // taken so that a lane holds eight consecutive keys of one query row, which is the operand that O^T = V^T P^T wants: P never
 // leaves its lane.
 //
@@ -98,7 +100,9 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
   bool bad = false;  // a page of the run that is none: every row of it is NaN
   // Operand f of a tile's K: step f / (2 KS), half a of its keys, dims 32 ks on. Row r of the half's product is key
   // 8 (r / 4) + 4a + r % 4 of the step. Of its V: step f / DT, dims 16 dt on.
-  const uint32_t k_lane = (8 * (col >> 2) + (col & 3)) * D + quad * 8, v_lane = col * P + 8 * quad;
+  const int lrow = lane >> 2, lquad = lane & 3;
+  const uint32_t k_lane = (8 * (lrow >> 2) + (lrow & 3)) * D + lquad * 8, v_lane = lrow * P + 8 * lquad;
+  const int put = lquad * 16 + (lrow ^ 4 * lquad), get = quad * 16 + (col ^ 4 * quad);
   int tail = 0;  // of the loaded tile: the lane's V pieces' keys, where some are past the prefix
   bool edge = false;
   auto load = [&](int key0) {
@@ -114,12 +118,12 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
       kp[i] = page * pg.k_stride + (int64_t)in * D;
       vp[i] = page * pg.vt_stride + (int64_t)in;
     }
-    const uint16_t* ka = k_head + (col >= 8 ? kp[1] : kp[0]);
-    const uint16_t* va = v_head + (quad >= 2 ? vp[1] : vp[0]);
+    const uint16_t* ka = k_head + (lrow >= 8 ? kp[1] : kp[0]);
+    const uint16_t* va = v_head + (lquad >= 2 ? vp[1] : vp[0]);
 #pragma unroll
     for (int i = 0; i < FW; ++i) {
       const int f = (wave * FW) % (2 * KS) + i;  // (a multiple of 2 KS if FW is)
-      const int a = FW >= 2 * KS ? i / KS : f / KS, ks = i % KS;
+      const int a = FW >= 2 * KS ? i / KS : f / KS, ks = FW >= KS ? i % KS : f % KS;
       kr[i] = *reinterpret_cast<const u32x4_t*>(ka + (k_lane + (uint32_t)(4 * a * D + ks * 32)));
     }
 #pragma unroll
@@ -128,10 +132,10 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
       vr[i] = *reinterpret_cast<const u32x4_t*>(va + (v_lane + (uint32_t)(dt * 16 * P)));
     }
     edge = first + 32 > len;
-    tail = min(max(len - first - 8 * quad, 0), 8);
+    tail = min(max(len - first - 8 * lquad, 0), 8);
   };
   auto stage = [&](int buf) {
-    u32x4_t* to = lds + (size_t)buf * 2 * NF * 64 + wave * FW * 64 + lane;
+    u32x4_t* to = lds + (size_t)buf * 2 * NF * 64 + wave * FW * 64 + put;
     if (edge) {  // slots past the prefix hold anything, and 0 * NaN is NaN
 #pragma unroll
       for (int i = 0; i < FW; ++i) vr[i] = first_keys(vr[i], tail);
@@ -171,7 +175,7 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
   // Scores of step `at`, past the run's end -inf.
   auto scores = [&](int at, f32x4_t (&acc)[RT][2]) {
     const int s = at % SW * KW + kw, tile = at / SW;
-    const u32x4_t* kt = lds + (size_t)(tile & 1) * 2 * NF * 64 + s * (2 * KS * 64) + lane;
+    const u32x4_t* kt = lds + (size_t)(tile & 1) * 2 * NF * 64 + s * (2 * KS * 64) + get;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) acc[rt][0] = acc[rt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -229,7 +233,7 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
         pf[rt] = __builtin_bit_cast(bf16x8_t, p);
         sum[rt] = mfma16x16x32(ones, pf[rt], sum[rt]);
       }
-      const u32x4_t* vt = lds + ((size_t)(tile & 1) * 2 + 1) * NF * 64 + (at % SW * KW + kw) * (DT * 64) + lane;
+      const u32x4_t* vt = lds + ((size_t)(tile & 1) * 2 + 1) * NF * 64 + (at % SW * KW + kw) * (DT * 64) + get;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, vt[dt * 64]);
@@ -315,12 +319,13 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
   }
 }
 
-// A wave takes a run of a sequence's own keys for 16 of its query rows of a kv head, 32 keys a step, K and V straight from memory
-// in the matrix cores' operand order; as soon as a step's scores (outputs) are formed, its K (V) registers take the next one's
-// loads. Bound by memory. P is the sum of two bf16 terms here, as in paged.hip: products are not what it waits for.
+// A wave takes a run of a sequence's own keys for 16 of its query rows of a kv head, 32 keys a step. Four lanes in
+// a row load 64 bytes of a K (V) row at once, and the wave turns them into the matrix cores' operands through LDS of its own; as
+// soon as a step's K (V) is there, its registers take the next one's loads. Bound by memory: 64 sequences of 1000 tokens, 262 MB, in
+// 52 us. (Loaded as operands, a row a lane, 54; and 16 rows of 256 dims are left no registers.) P is the sum of two bf16 terms here, as in paged.hip: products are not what it waits for.
 template <int D>
 __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, int h, int tile, int run, int runs, int run_keys, int room) {
-  constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT;
+  constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, CH = DT < 8 ? DT : 8;  // (CH: operands staged at a time)
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   const int begin = run * run_keys;
   const words_t table = words(pg.table + (size_t)b * pg.ld);
@@ -336,38 +341,53 @@ __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, i
   const int end = min(begin + run_keys, total);
   const int r = 16 * tile + col, t = r / x.G;
   const int last = r < rows ? sq.len + t : -1;  // the last key that this lane's row sees
-  bf16x8_t qf[KS];
+  extern __shared__ u32x4_t lds[];  // D = 256: the wave's queries, which no register is left for
+  constexpr bool kFar = D == 256;
+  const uint32_t area = wave_id() * (kFar ? CH + KS : CH) * 64;
+  uint32_t mine = area + CH * 64 + lane;
+  bf16x8_t qf[kFar ? 1 : KS];
   {
     const int in = min(r, rows - 1), token = in / x.G;
     const uint16_t* qp = x.q + (((size_t)b * x.T + token) * x.Hq + h * x.G + in - token * x.G) * D + quad * 8;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
+    for (int ks = 0; ks < KS; ++ks) {
+      if (kFar) lds[mine + ks * 64] = *reinterpret_cast<const u32x4_t*>(qp + ks * 32);
+      else qf[ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
+    }
   }
   const int P = 1 << pg.log2p;
   const uint16_t* k_head = pg.k + (size_t)h * P * D;
   const uint16_t* v_head = pg.vt + (size_t)h * D * P;
-  const uint32_t k_lane = (8 * (col >> 2) + (col & 3)) * D + quad * 8, v_lane = col * P + 8 * quad;
-  bf16x8_t kf[2][KS];
-  u32x4_t vf[DT];
+  const int lrow = lane >> 2, lquad = lane & 3;  // of an operand, as it is loaded
+  const uint32_t k_lane = (8 * (lrow >> 2) + (lrow & 3)) * D + lquad * 8, v_lane = lrow * P + 8 * lquad;
+  const uint32_t put = area + lquad * 16 + (lrow ^ 4 * lquad), get = area + quad * 16 + (col ^ 4 * quad);
+  u32x4_t kr[DT], vr[DT];
+  // Operands c CH on of the step's K or V to LDS (an area of 16 D words a wave at most), where every lane's reads before are done: a wave's go in their order.
+  auto stage = [&](const u32x4_t (&of)[DT], int c) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < CH; ++i) lds[put + i * 64] = of[c * CH + i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
   auto there = [&](int i) { return (unsigned)id[i] < (unsigned)pg.n_pages; };
   auto slot_of = [&](int key0, int i) { return (key0 & (P - 1)) - (P == 16 ? 16 * i : 0); };
   auto load_k = [&](int key0) {
     uint64_t at[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) at[i] = (there(i) ? (uint32_t)id[i] : 0u) * (uint64_t)pg.k_stride + (int64_t)slot_of(key0, i) * D;
-    const uint16_t* p = k_head + (col >= 8 ? at[1] : at[0]);
+    const uint16_t* p = k_head + (lrow >= 8 ? at[1] : at[0]);
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[a][ks] = *reinterpret_cast<const bf16x8_t*>(p + (k_lane + (uint32_t)(4 * a * D + ks * 32)));
+      for (int ks = 0; ks < KS; ++ks) kr[a * KS + ks] = *reinterpret_cast<const u32x4_t*>(p + (k_lane + (uint32_t)(4 * a * D + ks * 32)));
   };
   auto load_v = [&](int key0) {
     uint64_t at[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) at[i] = (there(i) ? (uint32_t)id[i] : 0u) * (uint64_t)pg.vt_stride + (int64_t)slot_of(key0, i);
-    const uint16_t* p = v_head + (quad >= 2 ? at[1] : at[0]);
+    const uint16_t* p = v_head + (lquad >= 2 ? at[1] : at[0]);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) vf[dt] = *reinterpret_cast<const u32x4_t*>(p + (v_lane + (uint32_t)(dt * 16 * P)));
+    for (int dt = 0; dt < DT; ++dt) vr[dt] = *reinterpret_cast<const u32x4_t*>(p + (v_lane + (uint32_t)(dt * 16 * P)));
   };
   uint32_t bad = 0, bad_next = 0;  // halves of the step on a page that is none
   auto missing = [&](int key0) { return (!there(0) && key0 < total ? 1u : 0u) | (!there(1) && key0 + 16 < total ? 2u : 0u); };
@@ -383,12 +403,17 @@ __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, i
   for (int key0 = begin; key0 < end; key0 += 32) {
     const bool more = key0 + 32 < end;
     const bool edge = key0 + 32 > sq.len + 1 || bad;  // some row does not see, or may not read, some key
-    f32x4_t acc[2];
+    f32x4_t acc[2] = {};
+    if (kFar) asm volatile("" : "+v"(mine));  // (read anew in every step)
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      acc[a] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < DT / CH; ++c) {
+      stage(kr, c);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) acc[a] = mfma16x16x32(kf[a][ks], qf[ks], acc[a]);
+      for (int i = 0; i < CH; ++i) {
+        const int a = (c * CH + i) / KS, ks = (c * CH + i) % KS;
+        const bf16x8_t one = kFar ? __builtin_bit_cast(bf16x8_t, lds[mine + ks * 64]) : qf[kFar ? 0 : ks];
+        acc[a] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, lds[get + i * 64]), one, acc[a]);
+      }
     }
     if (more) {
       bad_next = missing(key0 + 32);
@@ -421,34 +446,42 @@ __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, i
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[dt][i] *= f;
+    bool odd = false;
     if (edge) {
       // Slots past the sequence hold anything: zeroed, for 0 * NaN is NaN. So are new tokens' values that are no numbers, which no
       // earlier row may meet: the outputs that see one become NaN instead, by a product of the odd values' and the seen keys' ones.
-      const int n = (bad >> (quad >> 1)) & 1 ? 0 : min(max(total - (key0 + 8 * quad), 0), 8);
+      const int n = (bad >> (lquad >> 1)) & 1 ? 0 : min(max(total - (key0 + 8 * lquad), 0), 8);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) vf[dt] = first_keys(vf[dt], n);
-      if (sq.count > 1 && any_not_finite(vf)) {
+      for (int dt = 0; dt < DT; ++dt) vr[dt] = first_keys(vr[dt], n);
+      odd = sq.count > 1 && any_not_finite(vr);
+    }
+#pragma unroll
+    for (int c = 0; c < DT / CH; ++c) {
+      stage(vr, c);
+      if (odd) {
         const u32x4_t one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
         const bf16x8_t seen = __builtin_bit_cast(bf16x8_t, first_keys(one, min(max(last + 1 - (key0 + 8 * quad), 0), 8)));
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          u32x4_t odd;
+        for (int i = 0; i < CH; ++i) {
+          u32x4_t v = lds[get + i * 64], is;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const uint32_t no = ((vf[dt][v] & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u;  // exponents of all ones
-            vf[dt][v] &= ~(no * 0xffffu);
-            odd[v] = no * 0x3f80u;
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t no = ((v[w] & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u;  // exponents of all ones
+            v[w] &= ~(no * 0xffffu);
+            is[w] = no * 0x3f80u;
           }
-          const f32x4_t met = mfma16x16x32(__builtin_bit_cast(bf16x8_t, odd), seen, f32x4_t{0.f, 0.f, 0.f, 0.f});
+          lds[get + i * 64] = v;
+          const f32x4_t met = mfma16x16x32(__builtin_bit_cast(bf16x8_t, is), seen, f32x4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[dt][i] = met[i] > 0.f ? __builtin_nanf("") : o[dt][i];
+          for (int e = 0; e < 4; ++e) o[c * CH + i][e] = met[e] > 0.f ? __builtin_nanf("") : o[c * CH + i][e];
         }
       }
-    }
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      o[dt] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, vf[dt]), __builtin_bit_cast(bf16x8_t, hi), o[dt]);
-      o[dt] = mfma16x16x32(__builtin_bit_cast(bf16x8_t, vf[dt]), __builtin_bit_cast(bf16x8_t, lo), o[dt]);
+      for (int i = 0; i < CH; ++i) {
+        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, lds[get + i * 64]);
+        o[c * CH + i] = mfma16x16x32(vf, __builtin_bit_cast(bf16x8_t, hi), o[c * CH + i]);
+        o[c * CH + i] = mfma16x16x32(vf, __builtin_bit_cast(bf16x8_t, lo), o[c * CH + i]);
+      }
     }
     if (more) {
       load_v(key0 + 32);
@@ -491,7 +524,7 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void shared_parts_kernel(Pages pg,
 // The parts of a row joined: those of the prefix, then those of its own keys, part i by wave i % W of the row's W, the waves in
 // order. Bound by latency for few rows, by the parts' bytes for many.
 template <int D, int W>
-__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void shared_merge_kernel(Pages pg, Prefix px, int T, int Hq, int G, int Hkv,
+__global__ __launch_bounds__(256) void shared_merge_kernel(Pages pg, Prefix px, int T, int Hq, int G, int Hkv,
                                                                             int room, int span, int own_keys, int slots,
                                                                             size_t first, const float* __restrict__ part_o,
                                                                             const float* __restrict__ part_ml, Out o) {
@@ -559,53 +592,77 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void shared_merge_kernel(Page
   *op = y;
 }
 
-// How the prefix is cut: row tiles a wave, waves that share a tile's keys, keys of a run (`span`) and runs (`slots`).
+// How a call is cut. The prefix: row tiles a wave, waves that share a tile's keys, keys of a run (`span`) and runs (`slots`). A
+// sequence's own keys: 16-row tiles of its rows, keys of a run, runs.
 struct Cut {
   int rt, kw, waves, row_blocks, span, slots;
+  int tiles, own_keys, own_runs;
 };
 
-Cut prefix_cut(int rows, int Hkv, int D, int prefix_keys) {
-  Cut c;
+// The form of the prefix's kernel by the query rows of a kv head.
+void set_form(Cut& c, int rows, int D) {
   if (D == 256) {
-    c.waves = 4;
-    c.rt = rows > 32 ? 2 : 1;
+    c.waves = rows > 32 ? 8 : 4;
+    c.rt = 1;
     c.kw = rows > 64 ? 1 : 2;
   } else {
     c.waves = rows > 16 ? 8 : 4;
     c.rt = rows > 32 ? 2 : 1;
     c.kw = rows > 128 ? 1 : rows > 64 ? 2 : 4;
   }
-  const int block = 16 * c.rt * c.waves / c.kw, tile = tile_keys(D);
-  c.row_blocks = (rows + block - 1) / block;
-  const int tiles = (prefix_keys + tile - 1) / tile;
-  int64_t runs = 256 / ((int64_t)Hkv * c.row_blocks);
-  if (runs < 1) runs = 1;
-  c.span = (int)((tiles + runs - 1) / runs) * tile;
-  c.slots = (prefix_keys + c.span - 1) / c.span;
-  return c;
 }
 
-// A sequence's own keys: 16-row tiles of its rows, keys of a run, runs; enough waves to fill the card with loads (eight of 16 KB a
-// CU), and no shorter than four steps.
-struct Own {
-  int tiles, keys, runs;
-};
-
-Own own_cut(int B, int T, int G, int Hkv, int keys) {
-  Own o;
-  o.tiles = (T * G + 15) / 16;
-  const int64_t all = (int64_t)B * Hkv * o.tiles;
-  int64_t run = (all * keys / 2048 + 31) / 32 * 32;
-  if (run < 128) run = 128;
-  if (run > keys) run = (keys + 31) / 32 * 32;
-  o.keys = (int)run;
-  o.runs = (keys + o.keys - 1) / o.keys;
-  return o;
+// The runs. A CU holds one workgroup, so the card is shared out: so many workgroups to the prefix that those left over are done
+// with the own keys in the same time, by what a CU was measured to do. It reads 35 bytes a ns, and forms 256 x 128 scores and
+// outputs of 128 dims in 4 us; a workgroup of either kind begins and ends in 6 and 3 us. Own runs have 64 keys at least, and the
+// prefix half the card: `keys` may be a loose bound. (All of the card to the prefix first, and then to runs of 128 own keys: 32
+// sequences of 500 behind 4099 tokens 36 -> 28 us, 16 of 300 behind 16384 39 -> 28, 128 of 300 behind 16384 97 -> 83.)
+Cut cut_of(int B, int T, int G, int Hkv, int D, int prefix_keys, int keys) {
+  Cut c;
+  const int rows = B * T * G, tile = tile_keys(D);
+  set_form(c, rows, D);
+  const int block = 16 * c.rt * c.waves / c.kw;
+  c.row_blocks = (rows + block - 1) / block;
+  c.tiles = (T * G + 15) / 16;
+  const int tiles = (prefix_keys + tile - 1) / tile, front = Hkv * c.row_blocks, most = 256 / front > 1 ? 256 / front : 1;
+  const float read = 4.f * tile * D / 35, form = (float)block * tile * (D + 128) * 4.8e-4f, a_tile = read > form ? read : form;
+  const float a_step = c.waves * (4.f * 32 * D) / 35, a_part = 8.f * Hkv * rows * D / 4900;
+  const float late = 35 / 19.f;  // what a step takes longer with all CUs at it
+  const int64_t all = (int64_t)B * Hkv * c.tiles;
+  float best = INFINITY;
+  for (int eighths = 4; eighths <= 8; ++eighths) {
+    const int runs = most * eighths / 8 > 1 ? most * eighths / 8 : 1;
+    const int span = (tiles + runs - 1) / runs, slots = (tiles + span - 1) / span;
+    const int64_t groups = (int64_t)front * slots;
+    const float first = (6000 + span * a_tile) * ((groups + 255) / 256);
+    const int64_t left = groups < 256 ? 256 - groups : 0;
+    for (int n = 1;; n += (n + 1) / 2) {
+      int run = ((keys + n - 1) / n + 31) / 32 * 32;
+      const int own_runs = (keys + run - 1) / run;
+      const int64_t own = (all * own_runs + c.waves - 1) / c.waves;
+      const float one = 3000 + run / 32 * a_step;
+      // rounds of own workgroups in the CUs left over while the prefix's are at work, and then in all
+      const int64_t beside = (int64_t)(first / one) * left;
+      float time = first;
+      if (own <= left) time = first > one ? first : one;
+      else if (own > beside) time = first + (own - beside + 255) / 256 * (3000 + run / 32 * a_step * late);
+      time += (slots + own_runs) * a_part;
+      if (time < best) {
+        best = time;
+        c.span = span * tile;
+        c.slots = slots;
+        c.own_keys = run;
+        c.own_runs = own_runs;
+      }
+      if (run == 32 || own > 4096) break;
+    }
+    if (runs == most) break;
+  }
+  return c;
 }
 
 struct Plan {
   Cut cut;
-  Own own;
   int64_t prefix_groups, groups;  // workgroups
   size_t front, parts, bytes;     // parts of the prefix, and in all
 };
@@ -613,12 +670,11 @@ struct Plan {
 Plan plan_of(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys) {
   Plan p;
   const int G = Hq / Hkv;
-  p.cut = prefix_cut(B * T * G, Hkv, D, prefix_keys);
-  p.own = own_cut(B, T, G, Hkv, keys);
+  p.cut = cut_of(B, T, G, Hkv, D, prefix_keys, keys);
   p.prefix_groups = (int64_t)Hkv * p.cut.row_blocks * p.cut.slots;
-  p.groups = p.prefix_groups + ((int64_t)B * Hkv * p.own.tiles * p.own.runs + p.cut.waves - 1) / p.cut.waves;
+  p.groups = p.prefix_groups + ((int64_t)B * Hkv * p.cut.tiles * p.cut.own_runs + p.cut.waves - 1) / p.cut.waves;
   p.front = (size_t)B * Hkv * p.cut.slots * T * G;
-  p.parts = p.front + (size_t)B * Hkv * p.own.runs * T * G;
+  p.parts = p.front + (size_t)B * Hkv * p.cut.own_runs * T * G;
   p.bytes = p.parts * (D + 2) * sizeof(float);
   return p;
 }
@@ -627,13 +683,14 @@ template <int D, int RT, int KW, int NW>
 int launch_parts(const Pages& pg, const Prefix& px, const Rows& x, int keys, const Plan& p, hipStream_t s) {
   constexpr int bytes = prefix_lds<D, RT, KW, NW>();
   static_assert(bytes <= 160 * 1024, "a CU's LDS");
+  static_assert(bytes >= NW * 16 * D * 4, "a wave's area of its own");
   if (bytes > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(shared_parts_kernel<D, RT, KW, NW>),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return skinny_set_error(SKINNY_ELAUNCH, "paged_attention_shared: %d bytes of LDS: %s", bytes, hipGetErrorString(e));
   }
   hipLaunchKernelGGL((shared_parts_kernel<D, RT, KW, NW>), dim3((uint32_t)p.groups), dim3(64 * NW), bytes, s, pg, px, x,
-                     p.cut.row_blocks, p.cut.span, (int)p.prefix_groups, p.own.tiles, p.own.runs, p.own.keys, keys,
+                     p.cut.row_blocks, p.cut.span, (int)p.prefix_groups, p.cut.tiles, p.cut.own_runs, p.cut.own_keys, keys,
                      x.part_o + p.front * D, x.part_ml + p.front * 2);
   return skinny_check_launch("paged_attention_shared parts");
 }
@@ -653,8 +710,8 @@ int launch_shared(const Pages& pg, const Prefix& px, const uint16_t* q, int B, i
   using eight = std::integral_constant<int, 8>;
   int rc;
   if constexpr (D == 256) {
-    if (c.kw == 1) rc = parts(two{}, one{}, four{});
-    else if (c.rt == 2) rc = parts(two{}, two{}, four{});
+    if (c.kw == 1) rc = parts(one{}, one{}, eight{});
+    else if (c.waves == 8) rc = parts(one{}, two{}, eight{});
     else rc = parts(one{}, two{}, four{});
   } else {
     if (c.waves == 4) rc = parts(one{}, four{}, four{});
@@ -664,12 +721,14 @@ int launch_shared(const Pages& pg, const Prefix& px, const uint16_t* q, int B, i
     else rc = parts(one{}, four{}, eight{});
   }
   if (rc) return rc;
+  // Four waves a row while the rows are few (32 heads of 4 sequences behind 20000 tokens 36.8 -> 34.8 us a call, of 128 behind 16384
+  // 94.2 -> 99.0; eight waves 36.7 and 108).
   const bool split = (int64_t)B * T * Hq <= 1024;
   auto merge = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(split ? 512 : 256), 0, s, pg, px, T, Hq, Hq / Hkv, Hkv,
-                       keys, c.span, p.own.keys, p.own.runs, p.front, ws, ml, o);
+    hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(256), 0, s, pg, px, T, Hq, Hq / Hkv, Hkv,
+                       keys, c.span, c.own_keys, c.own_runs, p.front, ws, ml, o);
   };
-  if (split) merge(shared_merge_kernel<D, 8>);
+  if (split) merge(shared_merge_kernel<D, 4>);
   else merge(shared_merge_kernel<D, 1>);
   return skinny_check_launch("paged_attention_shared merge");
 }

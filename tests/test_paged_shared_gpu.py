@@ -216,6 +216,42 @@ def test_values_that_are_no_numbers(dev):
     assert torch.isnan(y[1, 0, :, 3]).all() and torch.equal(_bits(y[0]), _bits(clean[0]))
 
 
+@pytest.mark.parametrize("hq,hkv,d,page", [(8, 2, 128, 32), (16, 4, 256, 16), (4, 4, 64, 64), (4, 1, 128, 256)])
+def test_new_tokens_that_are_no_numbers(dev, hq, hkv, d, page):
+    """A new token's value or key that is not finite reaches its own row and the later ones; the rows before it, and the other
+    sequences, keep their bits. At every place of a step of 32 keys."""
+    T, lengths = 5, [0, 27, 61, 300, 1023]
+    s = Shared(dev, 14, hq, hkv, d, page, 150, lengths, T)
+    clean = _bits(s.run().view(5, T, hq, d))
+    rep = hq // hkv
+    for i, n in enumerate(lengths):
+        for at, bad in ((1, NAN), (T - 1, float("inf")), (3, -float("inf"))):
+            where = int(s.pages[i, (n + at) // page]), (n + at) % page
+            vt = s.vt.clone()
+            vt[where[0], 0, 7, where[1]] = bad
+            y = s.run(vt=vt).view(5, T, hq, d)
+            hit = torch.zeros((5, T, hq, d), dtype=torch.bool, device=dev)
+            hit[i, at:, :rep, 7] = True
+            assert not torch.isfinite(y[hit]).any() and torch.equal(_bits(y)[~hit], clean[~hit])
+            k = s.k.clone()
+            k[where[0], hkv - 1, where[1], 3] = NAN
+            y = s.run(k=k).view(5, T, hq, d)
+            hit[:] = False
+            hit[i, at:, hq - rep:] = True
+            assert torch.isnan(y[hit]).all() and torch.equal(_bits(y)[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 1, 128), (16, 4, 256), (2, 2, 64)])
+def test_own_keys_of_many_runs(dev, hq, hkv, d):
+    """Own caches far longer than the prefix, their ends at and beside a run's, with a bound on the keys that is far too loose."""
+    lengths = [5000, 63, 64, 2047, 2048, 0]
+    s = Shared(dev, 15, hq, hkv, d, 64, 40, lengths, 2, counts=[2, 2, 1, 1, 2, 0])
+    s.check(s.run())
+    wide = torch.full((6, 4096), -7, dtype=I32, device=dev)
+    wide[:, :s.pages.shape[1]] = s.pages
+    s.check(s.run(pages=wide))
+
+
 def test_what_cannot_be_is_nan_and_reads_nothing(dev):
     s = Shared(dev, 8, 8, 2, 128, 32, 300, [5, 40, 9], 2)
     clean = s.run()
