@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) void conv_silu_batch_kernel(Pool pool, const u
 
 // ---------------------------------------------------------------------------------------------------------
 // The rule token by token: 16 lanes hold a value column (8 key dims each), a group of lanes NC columns, so a workgroup
-// 16 * NC of a head's 128. All of the state's loads are issued at once. The token's update is gdn.hip's, its sums in the
+// 16 * NC of a head's 128; 16 tokens at most. All of the state's loads are issued at once. The token's update is gdn.hip's, its sums in the
 // same order: y and the state have the bits of skinny_gdn_recurrence on each sequence alone.
 constexpr int kStepThreads = 256, kStepGroups = kStepThreads / kPart;
 
@@ -187,55 +187,51 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
   }
   const int hk = h / (H / Hk);
   const float neg_a = -expf(A_log[h]), dtb = dt_bias[h], qscale = rsqrtf((float)kDk);
-  for (int t0 = 0; t0 < r.count; t0 += kTokBlock) {
-    const int mb = min(kTokBlock, r.count - t0);
-    if (t0 > 0) __syncthreads();
-    if (g < mb) {  // a lane group per token: its q and k, normalised
-      const uint16_t* row = qkv + (int64_t)(row0 + t0 + g) * ldq + (size_t)hk * kDk + p * 8;
-      const u32x4_t qw = *reinterpret_cast<const u32x4_t*>(row);
-      const u32x4_t kw = *reinterpret_cast<const u32x4_t*>(row + (size_t)Hk * kDk);
-      float q[8], k[8], qq = 0.f, kk = 0.f;
+  if (g < r.count) {  // a lane group per token: its q and k, normalised
+    const uint16_t* row = qkv + (int64_t)(row0 + g) * ldq + (size_t)hk * kDk + p * 8;
+    const u32x4_t qw = *reinterpret_cast<const u32x4_t*>(row);
+    const u32x4_t kw = *reinterpret_cast<const u32x4_t*>(row + (size_t)Hk * kDk);
+    float q[8], k[8], qq = 0.f, kk = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        q[e] = bf16_bits_to_f32((e & 1) ? (qw[e >> 1] >> 16) : (qw[e >> 1] & 0xffffu));
-        k[e] = bf16_bits_to_f32((e & 1) ? (kw[e >> 1] >> 16) : (kw[e >> 1] & 0xffffu));
-        qq = fmaf(q[e], q[e], qq);
-        kk = fmaf(k[e], k[e], kk);
-      }
-      const float qn = rsqrtf(sum16(qq) + 1e-6f) * qscale, kn = rsqrtf(sum16(kk) + 1e-6f);
-      f32x4_t* qd = reinterpret_cast<f32x4_t*>(&qk_lds[g][0][p * 8]);
-      f32x4_t* kd = reinterpret_cast<f32x4_t*>(&qk_lds[g][1][p * 8]);
-      qd[0] = f32x4_t{q[0] * qn, q[1] * qn, q[2] * qn, q[3] * qn};
-      qd[1] = f32x4_t{q[4] * qn, q[5] * qn, q[6] * qn, q[7] * qn};
-      kd[0] = f32x4_t{k[0] * kn, k[1] * kn, k[2] * kn, k[3] * kn};
-      kd[1] = f32x4_t{k[4] * kn, k[5] * kn, k[6] * kn, k[7] * kn};
-      if (p < 2) {
-        const float x = bf16_bits_to_f32((p ? bcol : acol)[(int64_t)(row0 + t0 + g) * ldab + h]);
-        gate_lds[g][p] = p ? 1.0f / (1.0f + expf(-x)) : expf(neg_a * softplus(x + dtb));
-      }
+    for (int e = 0; e < 8; ++e) {
+      q[e] = bf16_bits_to_f32((e & 1) ? (qw[e >> 1] >> 16) : (qw[e >> 1] & 0xffffu));
+      k[e] = bf16_bits_to_f32((e & 1) ? (kw[e >> 1] >> 16) : (kw[e >> 1] & 0xffffu));
+      qq = fmaf(q[e], q[e], qq);
+      kk = fmaf(k[e], k[e], kk);
     }
-    for (int i = tid; i < mb * COLS; i += kStepThreads)
-      v_lds[i / COLS][i % COLS] =
-          bf16_bits_to_f32(qkv[(int64_t)(row0 + t0 + i / COLS) * ldq + (size_t)2 * Hk * kDk + (size_t)h * kDv + col0 + i % COLS]);
-    __syncthreads();
-    for (int i = 0; i < mb; ++i) {
-      float q[8], k[8];
-      const f32x4_t* qp = reinterpret_cast<const f32x4_t*>(&qk_lds[i][0][p * 8]);
-      const f32x4_t* kp = reinterpret_cast<const f32x4_t*>(&qk_lds[i][1][p * 8]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        q[e] = qp[e >> 2][e & 3];
-        k[e] = kp[e >> 2][e & 3];
-      }
-      const float decay = gate_lds[i][0], beta = gate_lds[i][1];
-      float yv = 0.f;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const float one = gdn_token(s[c], k, q, v_lds[i][g * NC + c], decay, beta);
-        if (p == c) yv = one;
-      }
-      if (p < NC) yb[(t0 + i) * ystep + g * NC + p] = yv;
+    const float qn = rsqrtf(sum16(qq) + 1e-6f) * qscale, kn = rsqrtf(sum16(kk) + 1e-6f);
+    f32x4_t* qd = reinterpret_cast<f32x4_t*>(&qk_lds[g][0][p * 8]);
+    f32x4_t* kd = reinterpret_cast<f32x4_t*>(&qk_lds[g][1][p * 8]);
+    qd[0] = f32x4_t{q[0] * qn, q[1] * qn, q[2] * qn, q[3] * qn};
+    qd[1] = f32x4_t{q[4] * qn, q[5] * qn, q[6] * qn, q[7] * qn};
+    kd[0] = f32x4_t{k[0] * kn, k[1] * kn, k[2] * kn, k[3] * kn};
+    kd[1] = f32x4_t{k[4] * kn, k[5] * kn, k[6] * kn, k[7] * kn};
+    if (p < 2) {
+      const float x = bf16_bits_to_f32((p ? bcol : acol)[(int64_t)(row0 + g) * ldab + h]);
+      gate_lds[g][p] = p ? 1.0f / (1.0f + expf(-x)) : expf(neg_a * softplus(x + dtb));
     }
+  }
+  for (int i = tid; i < r.count * COLS; i += kStepThreads)
+    v_lds[i / COLS][i % COLS] =
+        bf16_bits_to_f32(qkv[(int64_t)(row0 + i / COLS) * ldq + (size_t)2 * Hk * kDk + (size_t)h * kDv + col0 + i % COLS]);
+  __syncthreads();
+  for (int i = 0; i < r.count; ++i) {
+    float q[8], k[8];
+    const f32x4_t* qp = reinterpret_cast<const f32x4_t*>(&qk_lds[i][0][p * 8]);
+    const f32x4_t* kp = reinterpret_cast<const f32x4_t*>(&qk_lds[i][1][p * 8]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[e] = qp[e >> 2][e & 3];
+      k[e] = kp[e >> 2][e & 3];
+    }
+    const float decay = gate_lds[i][0], beta = gate_lds[i][1];
+    float yv = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float one = gdn_token(s[c], k, q, v_lds[i][g * NC + c], decay, beta);
+      if (p == c) yv = one;
+    }
+    if (p < NC) yb[i * ystep + g * NC + p] = yv;
   }
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -253,10 +249,11 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
 // So the state is met in matrix products, once a chunk, and a token costs no chain of its own.
 //
 // A workgroup has WC waves for value columns (16 * NT each, whose states stay in their registers from the first chunk to the
-// last) and four that prepare chunks. A preparing wave takes every fourth chunk, through four periods between the workgroup's
-// barriers: its loads; the products of keys and queries, gates and L; T by substitution; everything into LDS in the matrix
-// cores' operand order, for the period after. So one chunk is ready each period, K and Q are read once a workgroup, and no
-// wave waits on memory.
+// last) and NP that prepare chunks. A preparing wave takes every NPth chunk, through NP periods between the workgroup's barriers:
+// its loads; the products of keys and queries, gates and L; T by substitution; everything into LDS in the matrix cores' operand
+// order, for the period after. So one chunk is ready each period, K and Q are read once a workgroup, and no wave waits on memory.
+// NP is 4, or 6 where a period's longest piece of preparing, 4500 cycles, would be longer than what a wave of 16 columns does in
+// it, 3300: then the last two are in halves (2039 tokens of 16 heads 120 -> 101 us).
 //
 // Rows of the products are dealt to tokens, and rows of the state to key dims, as 8 (r / 4) + 4 (tile) + r % 4: then what one
 // product leaves in a lane (eight consecutive tokens, or dims, of one value column) is the operand that the next one takes.
@@ -270,7 +267,7 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
 //
 // A correction that is not finite (a value, key or gate that is no number; a state that is none) would meet the rows before its
 // token as 0 * NaN: such a chunk's columns are taken token by token instead.
-constexpr int kChunk = 32, kProducers = 4;
+constexpr int kChunk = 32;
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
@@ -303,9 +300,10 @@ struct ChunkScratch {
   // of k and of q: the squares; a power of two near the length's inverse; what that leaves of 1 / sqrt(squares + 1e-6); that
   float sq[2][kChunk], two[2][kChunk], rest[2][kChunk], inv[2][kChunk];
 };
+template <int NP>
 struct ChunkLds {
   ChunkOps ops[2];
-  ChunkScratch scratch[kProducers];
+  ChunkScratch scratch[NP];
 };
 
 // What one wave's lanes exchange through LDS: written before, read after.
@@ -368,19 +366,16 @@ __device__ __forceinline__ float times_after(float v, int lane) {
   return v * ((lane & 7) + N < 8 ? u : 1.f);
 }
 
+// Waits for loads and stores (vmcnt(0)). At the end of a rare path: where it meets the usual one, the compiler would have that one
+// wait for all that either may have in flight (16 prompts of up to 1501 tokens 271 -> 253 us).
+__device__ __forceinline__ void nothing_in_flight() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // v, which the compiler then forms again in every turn of a loop: its sums with other offsets, formed before it, take two
 // registers each.
 __device__ __forceinline__ uint32_t here(uint32_t v) {
   asm volatile("" : "+v"(v));
   return v;
 }
-__device__ __forceinline__ const uint16_t* at_bytes(const uint16_t* base, uint32_t offset) {
-  return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(base) + offset);
-}
-__device__ __forceinline__ float* at_bytes(float* base, uint32_t offset) {
-  return reinterpret_cast<float*>(reinterpret_cast<char*>(base) + offset);
-}
-
 // Eight floats at a multiple of four.
 __device__ __forceinline__ void eight_of(const float* of, float (&to)[8]) {
   const f32x4_t a = *reinterpret_cast<const f32x4_t*>(of), b = *reinterpret_cast<const f32x4_t*>(of + 4);
@@ -391,7 +386,7 @@ __device__ __forceinline__ void eight_of(const float* of, float (&to)[8]) {
   }
 }
 
-// The four waves that prepare chunks: wave `p` the chunks p, p + 4, ... A chunk's gates are asked for a turn ahead.
+// The waves that prepare chunks: wave `p` the chunks p, p + NP, ... A chunk's gates are asked for a turn ahead.
 struct Rows {
   const uint16_t* qkv;  // of the sequence's first token
   uint32_t ldq;
@@ -399,7 +394,8 @@ struct Rows {
   uint32_t ldab;
   int h, hk, H, Hk, count;
 };
-__device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int p, int chunks, float neg_a, float dtb) {
+template <int NP>
+__device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds, int p, int chunks, float neg_a, float dtb) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   ChunkScratch& my = lds.scratch[p];
   const int tok[2] = {8 * (r >> 2) + (r & 3), 8 * (r >> 2) + 4 + (r & 3)};  // of this lane's row in each token tile
@@ -419,14 +415,17 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
     nb = (x.b + row * x.ldab + x.h)[at];
   };
   load_gates(p);
-  // Periods: chunk c's last one here is the one before the other waves take it, four before the first chunk's.
-  int left = chunks + kProducers;
+  // Periods: chunk c's last one here is the one before the other waves take it, NP before the first chunk's.
+  int left = chunks + NP;
   auto end_period = [&]() {
     lds_barrier();
     --left;
   };
+  auto half_period = [&]() {
+    if (NP == 6) end_period();
+  };
   for (int i = 0; i < p; ++i) end_period();
-  for (int c = p; c < chunks; c += kProducers) {
+  for (int c = p; c < chunks; c += NP) {
     const int t0 = c * kChunk, live = min(kChunk, x.count - t0);
     bf16x8_t kf[2][4], qf[2][4];
     Split aq[2];
@@ -561,6 +560,7 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
           for (int i = 0; i < 16; ++i) my.t[16 * half + i][16 * half + r] = t[i];
         }
         lanes_meet();
+        half_period();
         auto four_rows = [&](const float (*m)[kPitch], int row, int mcol, int vcol, float (&sum)[4]) {
           float v[16];
 #pragma unroll
@@ -588,8 +588,10 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
       }
       end_period();
       {
-        load_gates(c + kProducers);
+        load_gates(c + NP);
         ChunkOps& to = lds.ops[c & 1];
+        u32x4_t kh[2][4], qh[2][4];
+        Split two[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float k2 = my.two[0][tok[t]], q2 = my.two[1][tok[t]];
@@ -606,16 +608,25 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
           };
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            to.k[t][s][lane] = f16(kf[t][s], k2);
-            to.q[t][s][lane] = f16(qf[t][s], q2);
+            kh[t][s] = f16(kf[t][s], k2);
+            qh[t][s] = f16(qf[t][s], q2);
           }
           float row[8];
           eight_of(&my.t[tok[t]][8 * q], row);
 #pragma unroll
           for (int e = 0; e < 8; ++e) row[e] = tok[t] < 16 && q >= 2 ? 0.f : row[e];
-          const Split two = split(row, one);
-          to.t[0][t][lane] = __builtin_bit_cast(u32x4_t, two.hi);
-          to.t[1][t][lane] = __builtin_bit_cast(u32x4_t, two.lo);
+          two[t] = split(row, one);
+        }
+        half_period();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            to.k[t][s][lane] = kh[t][s];
+            to.q[t][s][lane] = qh[t][s];
+          }
+          to.t[0][t][lane] = __builtin_bit_cast(u32x4_t, two[t].hi);
+          to.t[1][t][lane] = __builtin_bit_cast(u32x4_t, two[t].lo);
           to.a[0][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].hi);
           to.a[1][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].lo);
         }
@@ -641,19 +652,20 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds& lds, int
 // is looked at, or the power is set anew, so that it is 4 to 8; powers within 2^-100 .. 2^100. A column's length grows by at most
 // beta |v| a token: from one look to the next it stays below 2^5 (sqrt(128) + 128), far inside fp16.
 constexpr float kLow = 0.25f, kHigh = 32.f;
+constexpr int kBuffer = 0x00020000;  // a raw buffer's words
 constexpr int kLook = 4;  // chunks from one look at the state to the next; its values are looked at in each
 __device__ __forceinline__ float power_below(float v) {  // that leaves v at 4 to 8
   return __uint_as_float((__float_as_uint(fminf(fmaxf(v * 0.25f, 0x1p-100f), 0x1p100f))) & 0x7f800000u);
 }
 
-template <int WC, int NT>
-__global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kernel(
+template <int WC, int NT, int NP>
+__global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
     Pool pool, const uint16_t* __restrict__ qkv, int64_t ldq, const uint16_t* __restrict__ bcol, const uint16_t* __restrict__ acol,
     int64_t ldab, const float* __restrict__ A_log, const float* __restrict__ dt_bias, float* state, float* __restrict__ y, int T,
     int H, int Hk) {
-  constexpr int COLS = 16 * WC * NT, THREADS = 64 * (WC + kProducers);
+  constexpr int COLS = 16 * WC * NT, THREADS = 64 * (WC + NP);
   extern __shared__ u32x4_t chunk_lds[];
-  ChunkLds& lds = *reinterpret_cast<ChunkLds*>(chunk_lds);
+  ChunkLds<NP>& lds = *reinterpret_cast<ChunkLds<NP>*>(chunk_lds);
   const int h = blockIdx.x, b = blockIdx.z, tid = threadIdx.x, wave = wave_id(), lane = tid & 63;
   const int col0 = (int)blockIdx.y * COLS;
   const Run run = run_of(pool, b, T);
@@ -672,7 +684,7 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
     if (chunks) prepare_chunks(x, lds, wave - WC, chunks, -expf(A_log[h]), dt_bias[h]);
     return;
   }
-  __builtin_amdgcn_s_setprio(1);  // before the preparing waves, which have periods to spare
+  __builtin_amdgcn_s_setprio(1);  // before the preparing waves, which have time to spare: 1 to 2 %
   const int r = lane & 15, q = lane >> 4;
   const int col = wave * 16 * NT + r;  // of the workgroup's; + 16 nt
   float one = 1.f;
@@ -714,40 +726,29 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
     }
   }
   const float qscale = rsqrtf((float)kDk);
-  // A chunk's values and results at 32-bit offsets (bytes) from its first row.
+  // A chunk's values and results as buffers from its first row to the sequence's end, at 32-bit offsets (bytes): loads past it are
+  // zero, stores nothing. So no path through a chunk but the rare one below has a branch around either, and the compiler knows at
+  // each wait how many are behind it.
   const uint16_t* vrow = rows + (size_t)2 * Hk * kDk + (size_t)h * kDv + col0;
   const uint32_t ld = (uint32_t)ldq * 2, yld = (uint32_t)ystep * 4;
   uint16_t nv[NT][8];
   auto load_v = [&](int c) {
-    const uint16_t* from = vrow + (int64_t)c * kChunk * ldq;
-    const int left = run.count - c * kChunk - 1;
-    if (left >= kChunk - 1) {
-      uint32_t at = here(8 * q * ld + col * 2);
+    const int left = min(kChunk, run.count - c * kChunk);
+    const auto from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vrow + (int64_t)c * kChunk * ldq), 0, left * ld, kBuffer);
+    uint32_t at = here(8 * q * ld + col * 2);
 #pragma unroll
-      for (int e = 0; e < 8; ++e, at += ld)
+    for (int e = 0; e < 8; ++e, at += ld)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) nv[nt][e] = *at_bytes(from + nt * 16, at);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) nv[nt][e] = *at_bytes(from + nt * 16, min(8 * q + e, left) * ld + col * 2);
-    }
+      for (int nt = 0; nt < NT; ++nt) nv[nt][e] = __builtin_amdgcn_raw_buffer_load_b16(from, at + nt * 32, 0, 0);
   };
   if (chunks) {
     load_v(0);
-    for (int i = 0; i < kProducers; ++i) lds_barrier();  // the first chunk's four periods
+    for (int i = 0; i < NP; ++i) lds_barrier();  // the first chunk's periods
+    nothing_in_flight();
   }
   for (int c = 0; c < chunks; ++c) {
     const ChunkOps& ops = lds.ops[c & 1];
     const int t0 = c * kChunk, live = min(kChunk, run.count - t0);
-    const bool full = live == kChunk;
-    if (!full) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) nv[nt][e] = 8 * q + e < live ? nv[nt][e] : (uint16_t)0;
-    }
     bool off = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -850,7 +851,7 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int t = 0; t < 2; ++t) af[i][t] = f16x8(ops.a[i][t][lane]);
-      float* yr = yb + (size_t)t0 * ystep;
+      const auto yr = __builtin_amdgcn_make_buffer_rsrc(yb + (size_t)t0 * ystep, 0, live * yld, kBuffer);
       Split ends[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -869,14 +870,9 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
           acc[t] = mfma16x16x32(af[0][t], dd[nt].hi, acc[t]);
         }
         uint32_t at = here(8 * q * yld + col * 4);
-        if (full) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e, at += yld) *at_bytes(yr + 16 * nt, at) = acc[e >> 2][e & 3] * whole;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e, at += yld)
-            if (8 * q + e < live) *at_bytes(yr + 16 * nt, at) = acc[e >> 2][e & 3] * whole;
-        }
+        for (int e = 0; e < 8; ++e, at += yld)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[e >> 2][e & 3] * whole), yr, at + nt * 64, 0, 0);
       }
       const float total = ops.sc.total;
       // K turned over, four tokens of a lane's dim at a time: the sixteen lanes of a quad give rows 4q .. 4q + 3 of a tile,
@@ -938,21 +934,22 @@ __global__ __launch_bounds__(64 * (WC + kProducers)) void gdn_batch_chunks_kerne
       }
       asm volatile("" ::: "memory");
       get_state(to);
+      nothing_in_flight();
     }
     lds_barrier();
   }
   put_state();
 }
 
-template <int WC, int NT>
+template <int WC, int NT, int NP>
 int launch_chunks(const Pool& p, const uint16_t* qkv, int64_t ldq, const uint16_t* b, const uint16_t* a, int64_t ldab,
                   const float* A_log, const float* dt_bias, float* state, float* y, int B, int T, int H, int Hk, hipStream_t s) {
-  static_assert(sizeof(ChunkLds) <= 160 * 1024, "a CU's LDS");
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(gdn_batch_chunks_kernel<WC, NT>),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChunkLds));
-  if (e != hipSuccess) return skinny_set_error(SKINNY_ELAUNCH, "gdn_batch: %zu bytes of LDS: %s", sizeof(ChunkLds), hipGetErrorString(e));
-  hipLaunchKernelGGL((gdn_batch_chunks_kernel<WC, NT>), dim3(H, kDv / (16 * WC * NT), B), dim3(64 * (WC + kProducers)),
-                     sizeof(ChunkLds), s, p, qkv, ldq, b, a, ldab, A_log, dt_bias, state, y, T, H, Hk);
+  static_assert(sizeof(ChunkLds<NP>) <= 160 * 1024, "a CU's LDS");
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(gdn_batch_chunks_kernel<WC, NT, NP>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ChunkLds<NP>));
+  if (e != hipSuccess) return skinny_set_error(SKINNY_ELAUNCH, "gdn_batch: %zu bytes of LDS: %s", sizeof(ChunkLds<NP>), hipGetErrorString(e));
+  hipLaunchKernelGGL((gdn_batch_chunks_kernel<WC, NT, NP>), dim3(H, kDv / (16 * WC * NT), B), dim3(64 * (WC + NP)),
+                     sizeof(ChunkLds<NP>), s, p, qkv, ldq, b, a, ldab, A_log, dt_bias, state, y, T, H, Hk);
   return skinny_check_launch("gdn_batch chunks");
 }
 
@@ -1013,17 +1010,19 @@ extern "C" int skinny_gdn_recurrence_batch(const uint16_t* qkv, int64_t ldq, con
       return launch(p, qkv, ldq, b, a, ldab, A_log, dt_bias, state, y, B, T, H, Hk, (hipStream_t)stream);
     };
     // As many workgroups to a head as still find a CU each (their registers leave no room for two): us a call for 16, 32, 64 and
-    // 128 columns a workgroup, 1024 tokens of 32 heads: 1 sequence 67 / 68 / 75 / 91, 4 sequences 249 / 134 / 78 / 92, 8: 495 / 271 /
-    // 156 / 118.
+    // 128 columns a workgroup, 1024 tokens of 32 heads: 1 sequence 57.7 / 58.6 / 71.8 / 91.0, 4 sequences 217 / 116 / 74.7 / 90.2, 8:
+    // 435 / 230 / 149 / 108.
     const int64_t heads = (int64_t)B * H;
-    return heads > 128 ? chunks(launch_chunks<4, 2>) : heads > 64 ? chunks(launch_chunks<4, 1>) : heads > 32 ? chunks(launch_chunks<2, 1>)
-                                                                                                             : chunks(launch_chunks<1, 1>);
+    return heads > 128 ? chunks(launch_chunks<4, 2, 4>) : heads > 64 ? chunks(launch_chunks<4, 1, 4>) : heads > 32 ? chunks(launch_chunks<2, 1, 6>)
+                                                                                                             : chunks(launch_chunks<1, 1, 6>);
   }
   auto go = [&](auto kernel, int nc) {
     hipLaunchKernelGGL(kernel, dim3(H, kDv / (kStepGroups * nc), B), dim3(kStepThreads), 0, (hipStream_t)stream, p, qkv, ldq, b, a,
                        ldab, A_log, dt_bias, state, y, T, H, Hk);
   };
-  if ((int64_t)B * H >= 512) go(gdn_batch_steps_kernel<8>, 8);
-  else go(gdn_batch_steps_kernel<1>, 1);
+  // Columns a lane group, 1 / 2 / 4 / 8, us a call of 32 heads: 16 sequences of 8 tokens 21.9 / 22.1 / 23.9 / 27.6, 64 of 16 109 / 104
+  // / 105 / 111; 64 of one token 51.9 / 50.1 / 48.2 / 52.0, 64 of four 57.6 / 51.5 / 51.1 / 56.9.
+  if (T <= 4 && (int64_t)B * H >= 1024) go(gdn_batch_steps_kernel<4>, 4);
+  else go(gdn_batch_steps_kernel<2>, 2);
   return skinny_check_launch("gdn_batch");
 }

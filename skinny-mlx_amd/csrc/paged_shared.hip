@@ -599,7 +599,14 @@ struct Cut {
   int tiles, own_keys, own_runs;
 };
 
-// The form of the prefix's kernel by the query rows of a kv head.
+// The form of the prefix's kernel by the query rows of a kv head: few rows want the tile's keys dealt to many waves, many rows few
+// reads of a tile. Behind 20000 tokens, us a call, (waves, row tiles, waves that share the keys):
+//   8 heads of 128 dims:   (4, 1, 4) (8, 1, 4) (8, 2, 4) (8, 2, 2) (8, 2, 1)     4 heads of 256:  (4, 1, 2) (8, 1, 2) (8, 1, 1)
+//            16 rows          22.3      22.8      24.7      30.7      39.7                           26.4      29.0      32.0
+//            32               27.9      22.9      26.1      32.0      40.4                           27.3      30.1      34.8
+//            64               42.8      30.1      27.9      32.9      41.4                           37.3      32.5      37.1
+//           128               68.9      47.1      37.2      35.3      44.2                           52.9      44.5      43.2
+//           256              122.7      74.5      54.5      49.4      49.5                           89.3      65.1      60.5
 void set_form(Cut& c, int rows, int D) {
   if (D == 256) {
     c.waves = rows > 32 ? 8 : 4;
