@@ -39,8 +39,8 @@ constexpr uint16_t kNanBits = 0x7fc0;
 // The conv: a thread per V channels and block of kTokBlock tokens. A token's taps are input rows, or for the first three
 // the state's, so the blocks need nothing of each other; the first one reads the state and writes the one after the call.
 // Taps oldest first and the exact exponential and division, as gdn.hip's conv: the same bits. For prompts memory and the vector
-// units take about as long: 16 sequences of 1000 tokens, 8192 channels, 159 us (3.3 TB/s) with four channels a thread, 176 with
-// eight, whose fewer waves load and compute in step; 155 with two, but 23 against 12 for 500 tokens of one sequence.
+// units take about as long: 16 sequences of 1000 tokens, 8192 channels, 121 us (4.3 TB/s) with two channels a thread, 135 with
+// four and 150 with eight, whose fewer waves load and compute in step.
 constexpr int kConvWidth = 4;
 
 template <int V>
@@ -73,6 +73,17 @@ struct Chans {
   __device__ __forceinline__ float value(int e) const { return bf16_bits_to_f32(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu); }
 };
 
+// v, which the compiler then keeps: it would form it from its 16 bits again for every product.
+__device__ __forceinline__ float kept(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+__device__ __forceinline__ uint32_t two_bf16(float a, float b) {
+  typedef __attribute__((ext_vector_type(2))) float two_t;
+  typedef __attribute__((ext_vector_type(2))) __bf16 two_bf16_t;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(two_t{a, b}, two_bf16_t));
+}
+
 template <int V>
 __global__ __launch_bounds__(256) void conv_silu_batch_kernel(Pool pool, const uint16_t* __restrict__ x, int64_t ldx, int T, int C,
                                                               uint16_t* state, const uint16_t* __restrict__ weight,
@@ -97,30 +108,38 @@ __global__ __launch_bounds__(256) void conv_silu_batch_kernel(Pool pool, const u
 #pragma unroll
     for (int j = 0; j < H; ++j) line[j].load(x + (int64_t)(t0 - H + j) * ldx);
   }
-  Chans<V> taps[kConvWidth];  // channel by channel: tap j of channel e is value e * kConvWidth + j
+  Chans<V> words[kConvWidth];  // channel by channel: tap j of channel e is value e * kConvWidth + j
 #pragma unroll
-  for (int i = 0; i < kConvWidth; ++i) taps[i].load(weight + (size_t)c * kConvWidth + i * V);
+  for (int i = 0; i < kConvWidth; ++i) words[i].load(weight + (size_t)c * kConvWidth + i * V);
 #pragma unroll
   for (int i = 0; i < kTokBlock; ++i)
     if (i < live) line[H + i].load(x + (int64_t)(t0 + i) * ldx);
+  float taps[kConvWidth][V], seen[kConvWidth][V];  // (seen: of the last four tokens, token i's in i % 4)
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+#pragma unroll
+    for (int j = 0; j < kConvWidth; ++j) taps[j][e] = kept(words[(e * kConvWidth + j) / V].value((e * kConvWidth + j) % V));
+#pragma unroll
+    for (int j = 0; j < H; ++j) seen[j][e] = line[j].value(e);
+  }
 #pragma unroll
   for (int i = 0; i < kTokBlock; ++i) {
     if (i >= rows) continue;
     Chans<V> y;
     if (i < live) {
-      uint16_t half[V];
+      float one[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
+        seen[(H + i) % kConvWidth][e] = kept(line[H + i].value(e));
         float acc = 0.f;
 #pragma unroll
-        for (int j = 0; j < kConvWidth; ++j)
-          acc = fmaf(taps[(e * kConvWidth + j) / V].value((e * kConvWidth + j) % V), line[i + j].value(e), acc);
-        half[e] = f32_to_bf16_bits(acc / (1.0f + expf(-acc)));
+        for (int j = 0; j < kConvWidth; ++j) acc = fmaf(taps[j][e], seen[(i + j) % kConvWidth][e], acc);
+        one[e] = acc / (1.0f + expf(-acc));
       }
-      if constexpr (V == 1) y.w[0] = half[0];
+      if constexpr (V == 1) y.w[0] = f32_to_bf16_bits(one[0]);
       else
 #pragma unroll
-        for (int e = 0; e < V / 2; ++e) y.w[e] = half[2 * e] | (uint32_t)half[2 * e + 1] << 16;
+        for (int e = 0; e < V / 2; ++e) y.w[e] = two_bf16(one[2 * e], one[2 * e + 1]);
     } else {
       y.fill(r.ok ? 0u : kNanBits);
     }
@@ -134,7 +153,9 @@ __global__ __launch_bounds__(256) void conv_silu_batch_kernel(Pool pool, const u
     Chans<V> v;
     const int at = r.count + j;
     if (at >= H) v.load(x + (int64_t)(at - H) * ldx);
-    else v = at == 0 ? line[0] : at == 1 ? line[1] : line[2];
+    else
+#pragma unroll
+      for (int i = 0; i < (V + 1) / 2; ++i) v.w[i] = at == 0 ? line[0].w[i] : at == 1 ? line[1].w[i] : line[2].w[i];
     v.store(to + (int64_t)j * C);
   }
 }
@@ -983,7 +1004,7 @@ extern "C" int skinny_gdn_conv_silu_batch(const uint16_t* x, int64_t ldx, int B,
     hipLaunchKernelGGL(kernel, dim3((n + 255) / 256, (T + kTokBlock - 1) / kTokBlock, B), dim3(256), 0, (hipStream_t)stream, p, x,
                        ldx, T, C, conv_state, weight, out, ldo);
   };
-  if (C % 4 == 0) go(conv_silu_batch_kernel<4>, 4);
+  if (C % 2 == 0) go(conv_silu_batch_kernel<2>, 2);
   else go(conv_silu_batch_kernel<1>, 1);
   return skinny_check_launch("gdn_conv_batch");
 }

@@ -61,6 +61,7 @@ def test_the_conv_refuses(args, fragment):
     (dict(t=0), "T=0"), (dict(b=65536), "B=65536"), (dict(t=65536), "T=65536"), (dict(qkv=ctypes.c_void_p(4104)), "16-byte"),
     (dict(ldq=6148), "16-byte"), (dict(state=ctypes.c_void_p(4104)), "16-byte"), (dict(pool=_pool(stride=STATE + 2)), "16-byte"),
     (dict(y=ctypes.c_void_p(4104)), "misaligned"), (dict(a=ODD), "misaligned"), (dict(al=ctypes.c_void_p(4098)), "misaligned"),
+    (dict(ldq=1 << 25), "too far apart"), (dict(ldab=1 << 25), "too far apart"),
 ])
 def test_the_recurrence_refuses(args, fragment):
     _expect_einval(_gdn(**args), fragment)
@@ -99,6 +100,19 @@ def test_workspace_sizes_behind_a_prefix():
                 (1, 1, 32, 8, 100, 10, 10), (1, 1, 32, 8, 128, 0, 10), (1, 1, 32, 8, 128, 10, 0), (1, 17, 32, 8, 128, 10, 10),
                 (1, 1, 32, 8, 128, (1 << 30) + 1, 10), (1, 1, 32, 0, 128, 10, 10), (1, 1 << 30, 32, 8, 128, 10, 10)):
         assert size(*bad) == 0, bad
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (16, 4, 256), (8, 8, 64), (64, 1, 128), (1, 1, 64)])
+def test_workspaces_grow_with_what_is_bounded(hq, hkv, d):
+    """The cut of a call is a rule on its sizes: any sizes within the limits have a workspace, of the rows' one part each at least and
+    of no more than a part for every 64 keys of the prefix and every 32 of the own."""
+    size = _lib.lib().skinny_paged_attn_shared_workspace_bytes
+    for b in (1, 2, 7, 64, 1000, 65535):
+        for t in {1, min(3, 64 * hkv // hq), 64 * hkv // hq}:
+            for prefix in (1, 63, 64, 65, 4096, 100001, 1 << 30):
+                for keys in (1, 31, 32, 33, 5000, 1 << 30):
+                    n = size(b, t, hq, hkv, d, prefix, keys) // (b * t * hq * (d + 2) * 4)
+                    assert 2 <= n <= -(-prefix // 64) + -(-keys // 32), (b, t, prefix, keys)
 
 
 def test_wrappers_refuse_host_tensors():
