@@ -732,7 +732,10 @@ def gdn_recurrence_batch(qkv: torch.Tensor, b: torch.Tensor, a: torch.Tensor, A_
     """gdn_recurrence of B sequences (skinny_gdn_recurrence_batch): qkv, b and a hold B*T rows, row b*T + t token t of
     sequence b; state fp32 [n_slots, H, Dv, Dk], of which sequence b begins with slots[b] (-1: zeros) and leaves the one
     after its tokens in slots_out[b] (None: in slots[b]) -> y fp32 [B*T, H, Dv]. counts and slots as for
-    gdn_conv_silu_batch."""
+    gdn_conv_silu_batch.
+
+    With T <= 16, y and the states are bitwise gdn_recurrence's on each sequence alone; longer calls go in chunks of 32
+    tokens through the matrix cores (relative error about 3e-7, token by token 1e-7), whatever the counts."""
     if not (qkv.is_cuda and qkv.dtype == BF16 and qkv.dim() == 2 and qkv.stride(1) == 1):
         raise ValueError("qkv must be a bf16 2-D GPU tensor")
     dev = qkv.get_device()
