@@ -687,7 +687,10 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
   constexpr int COLS = 16 * WC * NT, THREADS = 64 * (WC + NP);
   extern __shared__ u32x4_t chunk_lds[];
   ChunkLds<NP>& lds = *reinterpret_cast<ChunkLds<NP>*>(chunk_lds);
-  const int h = blockIdx.x, b = blockIdx.z, tid = threadIdx.x, wave = wave_id(), lane = tid & 63;
+  // Heads that follow each other to one die (they take workgroups in turn): value heads of one key head find its rows in that
+  // die's cache (8 sequences of 1024 tokens, 32 heads of 16 key heads 109 -> 103 us; a third less read past it).
+  const int x = blockIdx.x, h = H % 8 ? x : x % 8 * (H / 8) + x / 8;
+  const int b = blockIdx.z, tid = threadIdx.x, wave = wave_id(), lane = tid & 63;
   const int col0 = (int)blockIdx.y * COLS;
   const Run run = run_of(pool, b, T);
   const size_t row0 = (size_t)b * T, ystep = (size_t)H * kDv;
@@ -701,8 +704,8 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
   const int chunks = (run.count + kChunk - 1) / kChunk;
   const uint16_t* rows = qkv + (int64_t)row0 * ldq;
   if (wave >= WC) {
-    const Rows x{rows, (uint32_t)ldq, bcol + (int64_t)row0 * ldab, acol + (int64_t)row0 * ldab, (uint32_t)ldab, h, h / (H / Hk), H, Hk, run.count};
-    if (chunks) prepare_chunks(x, lds, wave - WC, chunks, -expf(A_log[h]), dt_bias[h]);
+    const Rows seq{rows, (uint32_t)ldq, bcol + (int64_t)row0 * ldab, acol + (int64_t)row0 * ldab, (uint32_t)ldab, h, h / (H / Hk), H, Hk, run.count};
+    if (chunks) prepare_chunks(seq, lds, wave - WC, chunks, -expf(A_log[h]), dt_bias[h]);
     return;
   }
   __builtin_amdgcn_s_setprio(1);  // before the preparing waves, which have time to spare: 1 to 2 %
