@@ -498,15 +498,19 @@ __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, i
   if (quad == 0) reinterpret_cast<float2*>(x.part_ml)[at] = float2{m, l};
 }
 
-// The prefix's workgroups first (a run's heads one after the other: the eight dies take workgroups in turn), then the own keys'
-// waves, the runs that a sequence turns out not to have last.
+// The prefix's workgroups first (the eight dies take them in turn), then the own keys' waves, the runs that a sequence turns out
+// not to have last.
 template <int D, int RT, int KW, int NW>
 __global__ __launch_bounds__(64 * NW, NW / 4) void shared_parts_kernel(Pages pg, Prefix px, Rows x, int row_blocks, int span, int front,
                                                                        int tiles, int runs, int run_keys, int room, float* own_o,
                                                                        float* own_ml) {
   const int i = blockIdx.x;
   if (i < front) {
-    prefix_run<D, RT, KW, NW>(pg, px, x, i % x.Hkv, i / x.Hkv % row_blocks, i / x.Hkv / row_blocks, span);
+    // a head's run (`unit`) by all its blocks of rows on one die, whose cache then reads it once (12 sequences of 4 tokens behind
+    // 5003, 192 rows of 256 dims: 34.7 -> 32.9 us)
+    const int units = front / row_blocks, dies = units % 8 == 0 ? 8 : 1, block = i / dies % row_blocks;
+    const int unit = i / dies / row_blocks * dies + i % dies;
+    prefix_run<D, RT, KW, NW>(pg, px, x, unit % x.Hkv, block, unit / x.Hkv, span);
   } else {
     uint32_t unit = __builtin_amdgcn_readfirstlane((uint32_t)(i - front) * NW + wave_id());
     const uint32_t tile = unit % tiles;
