@@ -525,6 +525,9 @@ __global__ __launch_bounds__(64 * NW, NW / 4) void shared_parts_kernel(Pages pg,
   }
 }
 
+// How many times `of` goes into n >= 1, the rest counted.
+__host__ __device__ constexpr int times(int n, int of) { return (n - 1) / of + 1; }
+
 // The parts of a row joined: those of the prefix, then those of its own keys, part i by wave i % W of the row's W, the waves in
 // order. Bound by latency for few rows, by the parts' bytes for many.
 template <int D, int W>
@@ -550,7 +553,7 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(Pages pg, Prefix px, 
     if (w == 0) *op = out_t(padding ? (uint16_t)0 : kNanBits);
     return;
   }
-  const int np = (len + span - 1) / span, n = np + (sq.len + t) / own_keys + 1;  // parts of the prefix; and of its own keys
+  const int np = len ? times(len, span) : 0, n = np + (sq.len + t) / own_keys + 1;  // parts of the prefix; and of its own keys
   // parts of the prefix [run][kv head][row], from `first` on those of the own keys [sequence][kv head][run][row of its T * G]
   const int h = head / G;
   const size_t TG = (size_t)T * G, in = (size_t)t * G + head % G;
@@ -633,9 +636,9 @@ Cut cut_of(int B, int T, int G, int Hkv, int D, int prefix_keys, int keys) {
   const int rows = B * T * G, tile = tile_keys(D);
   set_form(c, rows, D);
   const int block = 16 * c.rt * c.waves / c.kw;
-  c.row_blocks = (rows + block - 1) / block;
-  c.tiles = (T * G + 15) / 16;
-  const int tiles = (prefix_keys + tile - 1) / tile, front = Hkv * c.row_blocks, most = 256 / front > 1 ? 256 / front : 1;
+  c.row_blocks = times(rows, block);
+  c.tiles = times(T * G, 16);
+  const int tiles = times(prefix_keys, tile), front = Hkv * c.row_blocks, most = 256 / front > 1 ? 256 / front : 1;
   const float read = 4.f * tile * D / 35, form = (float)block * tile * (D + 128) * 4.8e-4f, a_tile = read > form ? read : form;
   const float a_step = c.waves * (4.f * 32 * D) / 35, a_part = 8.f * Hkv * rows * D / 4900;
   const float late = 35 / 19.f;  // what a step takes longer with all CUs at it
@@ -643,13 +646,12 @@ Cut cut_of(int B, int T, int G, int Hkv, int D, int prefix_keys, int keys) {
   float best = INFINITY;
   for (int eighths = 4; eighths <= 8; ++eighths) {
     const int runs = most * eighths / 8 > 1 ? most * eighths / 8 : 1;
-    const int span = (tiles + runs - 1) / runs, slots = (tiles + span - 1) / span;
+    const int span = times(tiles, runs), slots = times(tiles, span);
     const int64_t groups = (int64_t)front * slots;
     const float first = (6000 + span * a_tile) * ((groups + 255) / 256);
     const int64_t left = groups < 256 ? 256 - groups : 0;
     for (int n = 1;; n += (n + 1) / 2) {
-      int run = ((keys + n - 1) / n + 31) / 32 * 32;
-      const int own_runs = (keys + run - 1) / run;
+      const int run = times(times(keys, n), 32) * 32, own_runs = times(keys, run);
       const int64_t own = (all * own_runs + c.waves - 1) / c.waves;
       const float one = 3000 + run / 32 * a_step;
       // rounds of own workgroups in the CUs left over while the prefix's are at work, and then in all
