@@ -609,7 +609,8 @@ int skinny_paged_attention_shared_bf16(const uint16_t* q, int B, int T, int Hq, 
  * next: sequence b begins with state slots[b] (-1: zeros) and the one after its counts[b] tokens goes to
  * slots_out[b] (NULL: to slots[b]), of a sequence without tokens the state as it was. States that are
  * only read may be shared, such as the one after a prefix that the sequences have in common; one
- * that the call writes stands once in slots_out and no other sequence reads it. A sequence with a
+ * that the call writes stands once in slots_out and no other sequence reads it. (A sequence without
+ * tokens whose state stays in its slot touches none: a batch may be padded with any.) A sequence with a
  * state outside the pool or a count outside [0, T] has NaN rows and writes none. Padding rows are zero. */
 typedef struct {
   const int32_t* slots;      /* [B] */

@@ -414,6 +414,32 @@ def test_captured_steps_follow_slots_and_counts(dev, T):
         assert _same(y, ref) and _same(graphed[0], eager[0]) and _same(graphed[1], eager[1])
 
 
+@pytest.mark.parametrize("T", [1, 7, 40])
+def test_a_padded_batch(dev, T):
+    """Sequences without tokens that name a state which another one writes, several of them the same: they touch nothing, and the
+    others have the bits of the batch without them."""
+    m = Mixer(dev, 37 + T, 8, 4, T, [0, T, 0, max(T - 3, 1), 0])
+    one, three = m.slots[1], m.slots[3]
+    slots = [three, one, three, three, one]
+    pool = m.pool.clone()
+    y = m.run(pool, slots).view(5, T, -1)
+    small = Mixer(dev, 37 + T, 8, 4, T, [T, max(T - 3, 1)])
+    keep = torch.tensor([1, 3], device=dev)
+    small.qkv, small.wide = (t.view(5, T, -1)[keep].reshape(2 * T, -1) for t in (m.qkv, m.wide))
+    small.b, small.a, small.a_log, small.dt = small.wide[:, 1:9], small.wide[:, 10:18], m.a_log, m.dt
+    ref_pool = m.pool.clone()
+    ref = small.run(ref_pool, [one, three]).view(2, T, -1)
+    assert _same(y[keep], ref) and _same(pool, ref_pool) and (y[[0, 2, 4]] == 0).all()
+    g = torch.Generator().manual_seed(T)
+    c = 320
+    x, w = torch.randn((5 * T, c), generator=g).to(BF16).to(dev), torch.randn((c, 4), generator=g).to(BF16).to(dev)
+    state = torch.randn((6, 3, c), generator=g).to(BF16).to(dev)
+    mine, theirs = state.clone(), state.clone()
+    out = K.gdn_conv_silu_batch(x, mine, w, _ints([4, 2, 4, 4, 2], dev), counts=_ints([0, T, 0, T, 0], dev)).view(5, T, c)
+    alone = K.gdn_conv_silu_batch(x.view(5, T, c)[keep].reshape(2 * T, c), theirs, w, _ints([2, 4], dev)).view(2, T, c)
+    assert _same(out[keep], alone) and _same(mine, theirs) and (out[[0, 2, 4]] == 0).all()
+
+
 def test_two_streams_at_once(dev):
     m = [Mixer(dev, s, 4, 2, 60, [60, 41]) for s in (37, 41)]
     refs = []
