@@ -31,16 +31,16 @@ __device__ __forceinline__ int prefix_length(const Prefix& p) {
 // the prefix: NW / KW groups of 16 * RT rows, in each of which KW waves share a tile's keys. A tile of keys is staged in LDS as
 // the matrix cores' operands and read by all the row groups; the next tile's loads are in flight meanwhile. Four lanes in a row
 // load 64 bytes of a K (V) row at once (a row a lane: 96.8 us where this takes 93.7, 64 sequences of 500 behind 32768 tokens) and
-// put them where the lanes that want them read without bank conflicts: the 16 rows of an operand's quad q in order row ^ 4q. Scores are formed transposed, S^T = K Q^T, with the K rows of a 32-key step
-// taken so that a lane holds eight consecutive keys of one query row, which is the operand that O^T = V^T P^T wants: P never
-// leaves its lane.
+// put them where the lanes that want them read without bank conflicts: the 16 rows of an operand's quad q in order row ^ 4q.
+// Scores are formed transposed, S^T = K Q^T, with the K rows of a 32-key step taken so that a lane holds eight consecutive keys of
+// one query row, which is the operand that O^T = V^T P^T wants: P never leaves its lane.
 //
 // P is rounded to bf16 (2^-8 of a weight) and its sum is taken of the rounded weights, so that the error is of the differences
 // between values only. The running maximum is raised only where a score passes it by 2^8: until then weights up to 2^8
 // are as exact, and the outputs need no rescaling.
 //
-// Bound by the matrix cores, LDS reads and the exponentials, which take about as long each (256 rows of 8 heads of 128 dims: each
-// 32768 keys more 40 us, 860 TFLOP/s, for rows enough), by loads for few rows.
+// Bound by the matrix cores, LDS reads and the exponentials, which take about as long each, where rows are many (256 of 8 heads of
+// 128 dims: each 32768 keys more 40 us, 860 TFLOP/s), by loads where they are few.
 template <int D>
 struct Shape {
   static constexpr int KS = D / 32;   // dim steps of a score
@@ -324,8 +324,9 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
 
 // A wave takes a run of a sequence's own keys for 16 of its query rows of a kv head, 32 keys a step. Four lanes in
 // a row load 64 bytes of a K (V) row at once, and the wave turns them into the matrix cores' operands through LDS of its own; as
-// soon as a step's K (V) is there, its registers take the next one's loads. Bound by memory: 64 sequences of 1000 tokens, 262 MB, in
-// 52 us. (Loaded as operands, a row a lane, 54; and 16 rows of 256 dims are left no registers.) P is the sum of two bf16 terms here, as in paged.hip: products are not what it waits for.
+// soon as a step's K (V) is there, its registers take the next one's loads. Bound by memory: 64 sequences of 1000 tokens, 262 MB,
+// in 52 us. (Loaded as operands, a row a lane, 54; and 16 rows of 256 dims are left no registers.) P is the sum of two bf16 terms
+// here, as in paged.hip: products are not what it waits for.
 template <int D>
 __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, int h, int tile, int run, int runs, int run_keys, int room) {
   constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, CH = DT < 8 ? DT : 8;  // (CH: operands staged at a time)
@@ -365,7 +366,8 @@ __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, i
   const uint32_t k_lane = (8 * (lrow >> 2) + (lrow & 3)) * D + lquad * 8, v_lane = lrow * P + 8 * lquad;
   const uint32_t put = area + lquad * 16 + (lrow ^ 4 * lquad), get = area + quad * 16 + (col ^ 4 * quad);
   u32x4_t kr[DT], vr[DT];
-  // Operands c CH on of the step's K or V to LDS (an area of 16 D words a wave at most), where every lane's reads before are done: a wave's go in their order.
+  // Operands c CH on of the step's K or V to LDS (an area of 16 D words a wave at most), where every lane's reads before are done:
+  // a wave's go in their order.
   auto stage = [&](const u32x4_t (&of)[DT], int c) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -737,8 +739,8 @@ int launch_shared(const Pages& pg, const Prefix& px, const uint16_t* q, int B, i
     else rc = parts(one{}, four{}, eight{});
   }
   if (rc) return rc;
-  // Four waves a row while the rows are few (32 heads of 4 sequences behind 20000 tokens 36.8 -> 34.8 us a call, of 128 behind 16384
-  // 94.2 -> 99.0; eight waves 36.7 and 108).
+  // Four waves a row while the rows are few (32 heads of 4 sequences behind 20000 tokens 36.8 -> 34.8 us a call, of 128 behind
+  // 16384 94.2 -> 99.0; eight waves 36.7 and 108).
   const bool split = (int64_t)B * T * Hq <= 1024;
   auto merge = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(split ? Hq : (Hq + 3) / 4, T, B), dim3(256), 0, s, pg, px, T, Hq, Hq / Hkv, Hkv,
