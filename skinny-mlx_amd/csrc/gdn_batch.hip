@@ -566,7 +566,7 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
       end_period();
       {
         // T's diagonal blocks of 16 by substitution, a lane per column: row i is e_i less the rows before it times L's. Then the
-        // block below: T21 = -T22 (L21 T11), four rows a quad.
+        // block below: T21 = -T22 (L21 T11), fp32 products whose step k takes rows 4q + k, which the first one leaves in quad q.
         const int half = q & 1;
         float t[16];
 #pragma unroll
@@ -587,30 +587,15 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
         }
         lanes_meet();
         half_period();
-        auto four_rows = [&](const float (*m)[kPitch], int row, int mcol, int vcol, float (&sum)[4]) {
-          float v[16];
+        f32x4_t x = {0.f, 0.f, 0.f, 0.f}, below = x;
+        const f32x4_t l21 = *reinterpret_cast<const f32x4_t*>(&my.l[16 + r][4 * q]);
+        const f32x4_t t22 = *reinterpret_cast<const f32x4_t*>(&my.t[16 + r][16 + 4 * q]);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = my.t[j][vcol];
+        for (int k = 0; k < 4; ++k) x = __builtin_amdgcn_mfma_f32_16x16x4f32(l21[k], my.t[4 * q + k][r], x, 0, 0, 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < 4; ++k) below = __builtin_amdgcn_mfma_f32_16x16x4f32(t22[k], x[k], below, 0, 0, 0);
 #pragma unroll
-            for (int j0 = 0; j0 < 16; j0 += 4) {
-              const f32x4_t w = *reinterpret_cast<const f32x4_t*>(&m[row + e][mcol + j0]);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[j] = fmaf(w[j], v[j0 + j], acc[j]);
-            }
-            sum[e] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-          }
-        };
-        float four[4];
-        four_rows(my.l, 16 + 4 * q, 0, r, four);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) my.t[4 * q + e][16 + r] = four[e];  // T's upper block, which is zero and not stored
-        lanes_meet();
-        four_rows(my.t, 16 + 4 * q, 16, 16 + r, four);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) my.t[16 + 4 * q + e][r] = -four[e];
+        for (int e = 0; e < 4; ++e) my.t[16 + 4 * q + e][r] = -below[e];
       }
       end_period();
       {
