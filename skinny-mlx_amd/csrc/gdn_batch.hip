@@ -274,8 +274,8 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
 // last) and NP that prepare chunks. A preparing wave takes every NPth chunk, through NP periods between the workgroup's barriers:
 // its loads; the products of keys and queries, gates and L; T by substitution; everything into LDS in the matrix cores' operand
 // order, for the period after. So one chunk is ready each period, K and Q are read once a workgroup, and no wave waits on memory.
-// NP is 4, or 6 where a period's longest piece of preparing, 4500 cycles, would be longer than what a wave of 16 columns does in
-// it, 3300: then the last two are in halves (2039 tokens of 16 heads 120 -> 101 us).
+// NP is 4, or 6 where a period's longest piece of preparing, 4000 cycles, would be longer than what a wave of 16 columns does in
+// it, 3300: then the last two are in halves (2039 tokens of 16 heads 103 -> 97 us).
 //
 // Rows of the products are dealt to tokens, and rows of the state to key dims, as 8 (r / 4) + 4 (tile) + r % 4: then what one
 // product leaves in a lane (eight consecutive tokens, or dims, of one value column) is the operand that the next one takes.
@@ -290,8 +290,8 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
 // A correction that is not finite (a value, key or gate that is no number; a state that is none) would meet the rows before its
 // token as 0 * NaN: such a chunk's columns are taken token by token instead.
 //
-// Bound by the chain of a wave's products and conversions where heads are few (a prompt of 2039 tokens, 16 heads: 99 us), by the
-// issue of two waves a SIMD where they are many (16 prompts of up to 1501 tokens, 32 heads: 240 us, of which a copy's rate would take
+// Bound by the chain of a wave's products and conversions where heads are few (a prompt of 2039 tokens, 16 heads: 97 us), by the
+// issue of two waves a SIMD where they are many (16 prompts of up to 1501 tokens, 32 heads: 235 us, of which a copy's rate would take
 // 149).
 constexpr int kChunk = 32;
 
@@ -1022,8 +1022,8 @@ extern "C" int skinny_gdn_recurrence_batch(const uint16_t* qkv, int64_t ldq, con
       return launch(p, qkv, ldq, b, a, ldab, A_log, dt_bias, state, y, B, T, H, Hk, (hipStream_t)stream);
     };
     // As many workgroups to a head as still find a CU each (their registers leave no room for two): us a call for 16, 32, 64 and
-    // 128 columns a workgroup, 1024 tokens of 32 heads: 1 sequence 57.7 / 58.6 / 71.8 / 91.0, 4 sequences 217 / 116 / 74.7 / 90.2, 8:
-    // 435 / 230 / 149 / 108.
+    // 128 columns a workgroup, 1024 tokens of 32 heads: 1 sequence 55.2 / 57.0 / 67.8 / 87.8, 4 sequences 211 / 111 / 69.8 / 88.2, 8:
+    // 421 / 222 / 140 / 100.
     const int64_t heads = (int64_t)B * H;
     return heads > 128 ? chunks(launch_chunks<4, 2, 4>) : heads > 64 ? chunks(launch_chunks<4, 1, 4>) : heads > 32 ? chunks(launch_chunks<2, 1, 6>)
                                                                                                              : chunks(launch_chunks<1, 1, 6>);
