@@ -440,6 +440,26 @@ def test_a_padded_batch(dev, T):
     assert _same(out[keep], alone) and _same(mine, theirs) and (out[[0, 2, 4]] == 0).all()
 
 
+@pytest.mark.parametrize("T", [1, 9, 33])
+def test_many_sequences(dev, T):
+    """Hundreds of sequences: some of them against themselves in a small batch, bit for bit (in chunks, 2^-18 of the
+    norm: sixteen times what a product of terms is off)."""
+    rng = np.random.default_rng(T)
+    b, heads, some = 700, 2, [0, 1, 350, 698, 699]
+    m = Mixer(dev, 41 + T, heads, 1, T, [int(n) for n in rng.integers(0, T + 1, b)])
+    pool = m.pool.clone()
+    y = m.run(pool).view(b, T, heads, D)
+    small = Mixer(dev, 41 + T, heads, 1, T, [m.counts[i] for i in some])
+    keep = torch.tensor(some, device=dev)
+    small.qkv, small.wide = (t.view(b, T, -1)[keep].reshape(len(some) * T, -1) for t in (m.qkv, m.wide))
+    small.b, small.a, small.a_log, small.dt = small.wide[:, 1:1 + heads], small.wide[:, 2 + heads:2 + 2 * heads], m.a_log, m.dt
+    ref_pool = m.pool.clone()
+    ref = small.run(ref_pool, [m.slots[i] for i in some]).view(len(some), T, heads, D)
+    for i, j in enumerate(some):
+        got, want = (torch.cat([t.flatten(), p[m.slots[j]].flatten()]) for t, p in ((y[j], pool), (ref[i], ref_pool)))
+        assert _same(got, want) if T <= 16 else (got - want).norm() <= 2.0 ** -18 * want.norm()
+
+
 def test_two_streams_at_once(dev):
     m = [Mixer(dev, s, 4, 2, 60, [60, 41]) for s in (37, 41)]
     refs = []

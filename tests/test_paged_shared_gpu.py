@@ -151,6 +151,15 @@ def test_several_tokens(dev, hq, hkv, d, T, gated):
     s.check(s.run(gate), gate)
 
 
+def test_many_sequences(dev):
+    """More blocks of rows than CUs; more own runs than rows of a workgroup's waves."""
+    rng = np.random.default_rng(5)
+    s = Shared(dev, 16, 4, 1, 64, 16, 33, [int(n) for n in rng.integers(0, 20, 1500)], 1)
+    s.check(s.run(), rows=(0, 1, 700, 1498, 1499))
+    s = Shared(dev, 17, 8, 8, 128, 32, 150, [int(n) for n in rng.integers(0, 90, 500)], 3)
+    s.check(s.run(), rows=(0, 255, 499))
+
+
 def test_a_prefix_of_many_runs(dev):
     s = Shared(dev, 3, 4, 2, 128, 256, 40001, [3, 900], 1)
     s.check(s.run())
