@@ -298,6 +298,8 @@ constexpr int kChunk = 32;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
 using ::mfma16x16x32;  // of bf16
 __device__ __forceinline__ f32x4_t mfma16x16x32(f16x8_t a, f16x8_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -372,7 +374,6 @@ __device__ __forceinline__ Split split(const float (&v)[8], float one) {
 
 // Whether one of the eight is an infinity or NaN.
 __device__ __forceinline__ bool no_numbers(f16x8_t v) {
-  typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
   const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
   u16x2_t m = {0, 0};
 #pragma unroll
@@ -698,10 +699,11 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
   }
   __builtin_amdgcn_s_setprio(1);  // before the preparing waves, which have time to spare: 1 to 2 %
   const int r = lane & 15, q = lane >> 4;
-  const int col = wave * 16 * NT + r;  // of the workgroup's; + 16 nt
+  // of the workgroup's; + nt: a lane's columns are neighbours, and their values (results) one load (store)
+  const int col = wave * 16 * NT + NT * r;
   float one = 1.f;
   asm volatile("" : "+v"(one));
-  // dims 32 s + 8 q + 4 half + i of column col + 16 nt, times `inv`
+  // dims 32 s + 8 q + 4 half + i of column col + nt, times `inv`
   f32x4_t st[NT][4][2];
   float inv[NT], scale[NT], top[NT];
   const size_t at = ((size_t)h * kDv + col0 + col) * kDk + q * 8;
@@ -713,7 +715,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) st[nt][s][half] = *reinterpret_cast<const f32x4_t*>(from + nt * 16 * kDk + s * 32 + half * 4);
+        for (int half = 0; half < 2; ++half) st[nt][s][half] = *reinterpret_cast<const f32x4_t*>(from + nt * kDk + s * 32 + half * 4);
     }
   };
   auto put_state = [&]() {
@@ -723,7 +725,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-          *reinterpret_cast<f32x4_t*>(to + nt * 16 * kDk + s * 32 + half * 4) = st[nt][s][half] * scale[nt];
+          *reinterpret_cast<f32x4_t*>(to + nt * kDk + s * 32 + half * 4) = st[nt][s][half] * scale[nt];
   };
   if (run.read >= 0) {
     get_state(state + run.read * pool.stride + at);
@@ -743,15 +745,15 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
   // each wait how many are behind it.
   const uint16_t* vrow = rows + (size_t)2 * Hk * kDk + (size_t)h * kDv + col0;
   const uint32_t ld = (uint32_t)ldq * 2, yld = (uint32_t)ystep * 4;
-  uint16_t nv[NT][8];
+  uint32_t nv[8];  // of the lane's columns, 16 bits each
+  auto value = [&](int nt, int e) { return __uint_as_float(nt ? nv[e] & 0xffff0000u : nv[e] << 16); };
   auto load_v = [&](int c) {
     const int left = min(kChunk, run.count - c * kChunk);
     const auto from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(vrow + (int64_t)c * kChunk * ldq), 0, left * ld, kBuffer);
     uint32_t at = here(8 * q * ld + col * 2);
 #pragma unroll
     for (int e = 0; e < 8; ++e, at += ld)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) nv[nt][e] = __builtin_amdgcn_raw_buffer_load_b16(from, at + nt * 32, 0, 0);
+      nv[e] = NT == 1 ? __builtin_amdgcn_raw_buffer_load_b16(from, at, 0, 0) : __builtin_amdgcn_raw_buffer_load_b32(from, at, 0, 0);
   };
   if (chunks) {
     load_v(0);
@@ -762,12 +764,12 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
     const ChunkOps& ops = lds.ops[c & 1];
     const int t0 = c * kChunk, live = min(kChunk, run.count - t0);
     bool off = false;
+    u16x2_t most = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, nv[e] & 0x7fff7fffu));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, nv[nt][e] & 0x7fffu);
-      top[nt] = bf16_bits_to_f32(m) * inv[nt];  // of this lane's values
+      top[nt] = bf16_bits_to_f32(most[nt]) * inv[nt];  // of this lane's values
       off |= top[nt] > kHigh;
     }
     if (c % kLook == 0 || __any(off)) {
@@ -835,7 +837,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
       for (int nt = 0; nt < NT; ++nt) {
         float right[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], bf16_bits_to_f32(nv[nt][e]) * inv[nt], -in[e] * ks[nt][e >> 2][e & 3]);
+        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], value(nt, e) * inv[nt], -in[e] * ks[nt][e >> 2][e & 3]);
         const Split two = split(right, one);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -871,20 +873,24 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
 #pragma unroll
         for (int e = 0; e < 8; ++e) decayed[e] = d[nt][e >> 2][e & 3] * end[e];
         ends[nt] = split(decayed, one);
-        const float whole = qscale * scale[nt];
-        f32x4_t acc[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+          f32x4_t& acc = qs[nt][t];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] = qs[nt][t][i] * out[4 * t + i];
-          acc[t] = mfma16x16x32(af[0][t], dd[nt].lo, acc[t]);
-          acc[t] = mfma16x16x32(af[1][t], dd[nt].hi, acc[t]);
-          acc[t] = mfma16x16x32(af[0][t], dd[nt].hi, acc[t]);
+          for (int i = 0; i < 4; ++i) acc[i] *= out[4 * t + i];
+          acc = mfma16x16x32(af[0][t], dd[nt].lo, acc);
+          acc = mfma16x16x32(af[1][t], dd[nt].hi, acc);
+          acc = mfma16x16x32(af[0][t], dd[nt].hi, acc);
         }
-        uint32_t at = here(8 * q * yld + col * 4);
+      }
+      uint32_t at = here(8 * q * yld + col * 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e, at += yld)
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[e >> 2][e & 3] * whole), yr, at + nt * 64, 0, 0);
+      for (int e = 0; e < 8; ++e, at += yld) {
+        uint32_t y[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) y[nt] = __float_as_uint(qs[nt][e >> 2][e & 3] * (qscale * scale[nt]));
+        if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b32(y[0], yr, at, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{y[0], y[1]}, yr, at, 0, 0);
       }
       const float total = ops.sc.total;
       // K turned over, four tokens of a lane's dim at a time: the sixteen lanes of a quad give rows 4q .. 4q + 3 of a tile,
@@ -920,7 +926,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
         const int tile = i >> 2 & 1, row = 4 * (i >> 3) + (i & 3) + 16 * q;
         const float decay = ops.sc.decay[i], kn = ops.sc.k[i], qn = ops.sc.q[i] * qscale, bt = ops.sc.beta[i];
         for (int nt = 0; nt < NT; ++nt) {
-          float* mine = to + nt * 16 * kDk;
+          float* mine = to + nt * kDk;
           asm volatile("" ::: "memory");  // the state stays where it is
           float sum = 0.f, yv = 0.f;
 #pragma unroll
@@ -929,7 +935,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = fmaf((float)w[e] * kn, mine[s * 32 + e], sum);
           }
-          const float delta = bt * (bf16_bits_to_f32(vrow[(int64_t)(t0 + i) * ldq + col + nt * 16]) - decay * quads_sum(sum));
+          const float delta = bt * (bf16_bits_to_f32(vrow[(int64_t)(t0 + i) * ldq + col + nt]) - decay * quads_sum(sum));
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
             const f16x8_t w = f16x8(ops.k[tile][s][row]), z = f16x8(ops.q[tile][s][row]);
@@ -941,7 +947,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
             }
           }
           yv = quads_sum(yv);
-          if (q == 0) yb[(size_t)(t0 + i) * ystep + col + 16 * nt] = yv;
+          if (q == 0) yb[(size_t)(t0 + i) * ystep + col + nt] = yv;
         }
       }
       asm volatile("" ::: "memory");

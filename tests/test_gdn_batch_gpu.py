@@ -362,6 +362,30 @@ def test_conv_has_the_bits_of_each_sequence_alone(dev, C, T):
         assert _same(left, expected)
 
 
+@pytest.mark.parametrize("C,T", [(64, 5), (130, 21), (63, 3)])
+def test_conv_of_rows_at_odd_places(dev, C, T):
+    """Rows, states and results that begin at odd elements and lie odd strides apart: the bits of the same at even ones."""
+    g = torch.Generator().manual_seed(C)
+    b, n = 3, 5
+    x = torch.randn((b * T, C), generator=g).to(BF16).to(dev)
+    w = torch.randn((C, 4), generator=g).to(BF16).to(dev)
+    state = torch.randn((n, 3, C), generator=g).to(BF16).to(dev)
+    slots, counts = _ints([4, 0, 2], dev), _ints([T, T - 1, 1], dev)
+    ref_state = state.clone()
+    ref = K.gdn_conv_silu_batch(x, ref_state, w, slots, counts=counts)
+    wide = torch.full((b * T, (C | 1) + 2), NAN, dtype=BF16, device=dev)
+    odd_x = wide[:, 1:1 + C]
+    odd_x.copy_(x)
+    flat = torch.full((1 + n * (3 * C | 1) + 8,), NAN, dtype=BF16, device=dev)
+    odd_state = flat.as_strided((n, 3, C), (3 * C | 1, C, 1), 1)
+    odd_state.copy_(state)
+    odd_w = torch.full((4 * C + 1,), NAN, dtype=BF16, device=dev)[1:].view(C, 4)
+    odd_w.copy_(w)
+    out = torch.full((b * T * C + 1,), NAN, dtype=BF16, device=dev)[1:].view(b * T, C)
+    y = K.gdn_conv_silu_batch(odd_x, odd_state, odd_w, slots, counts=counts, out=out)
+    assert y is out and _same(y, ref) and _same(odd_state, ref_state)
+
+
 def test_conv_of_sequences_that_cannot_be(dev):
     C, T = 24, 20
     x = torch.randn((4 * T, C), device=dev).to(BF16)
