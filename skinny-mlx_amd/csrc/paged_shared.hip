@@ -30,17 +30,18 @@ __device__ __forceinline__ int prefix_length(const Prefix& p) {
 // A workgroup of NW waves takes 16 * RT * NW / KW query rows of a kv head (every sequence's, one after the other) and a run of
 // the prefix: NW / KW groups of 16 * RT rows, in each of which KW waves share a tile's keys. A tile of keys is staged in LDS as
 // the matrix cores' operands and read by all the row groups; the next tile's loads are in flight meanwhile. Four lanes in a row
-// load 64 bytes of a K (V) row at once (a row a lane: 96.8 us where this takes 93.7, 64 sequences of 500 behind 32768 tokens) and
+// load 64 bytes of a K (V) row at once (a row a lane: 3 % slower, 64 sequences of 500 behind 32768 tokens) and
 // put them where the lanes that want them read without bank conflicts: the 16 rows of an operand's quad q in order row ^ 4q.
 // Scores are formed transposed, S^T = K Q^T, with the K rows of a 32-key step taken so that a lane holds eight consecutive keys of
 // one query row, which is the operand that O^T = V^T P^T wants: P never leaves its lane.
 //
-// P is rounded to bf16 (2^-8 of a weight) and its sum is taken of the rounded weights, so that the error is of the differences
-// between values only. The running maximum is raised only where a score passes it by 2^8: until then weights up to 2^8
+// P is the sum of two bf16 terms, 2^-16 of a weight, as in paged.hip and for the own keys. (One term, 2^-8, is half of the matrix
+// products with V; it left results 2.0e-3 to 2.3e-3 off where their own rounding is 1.65e-3, and 64 sequences of 1000 behind 32768
+// tokens took 94 us for 97.) The running maximum is raised only where a score passes it by 2^8: until then weights up to 2^8
 // are as exact, and the outputs need no rescaling.
 //
 // Bound by the matrix cores, LDS reads and the exponentials, which take about as long each, where rows are many (256 of 8 heads of
-// 128 dims: each 32768 keys more 40 us, 860 TFLOP/s), by loads where they are few.
+// 128 dims: each 32768 keys more 47 us, 730 TFLOP/s of the two products), by loads where they are few.
 template <int D>
 struct Shape {
   static constexpr int KS = D / 32;   // dim steps of a score
@@ -161,18 +162,18 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
     for (int ks = 0; ks < KS; ++ks) qf[rt][ks] = *reinterpret_cast<const bf16x8_t*>(qp + ks * 32);
   }
   float m[RT];
-  f32x4_t o[RT][DT], sum[RT];  // (sum: of a row's weights, in all four)
+  float sum[RT];  // of this lane's weights of a row
+  f32x4_t o[RT][DT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -INFINITY;
-    sum[rt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    sum[rt] = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
   if (begin + TK < end) find(begin + TK);
   stage(0);
   lds_barrier();
-  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, u32x4_t{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
   constexpr int SW = ST / KW;  // a wave's steps of a tile
   const int steps = (end - begin + TK - 1) / TK * SW;
   // Scores of step `at`, past the run's end -inf.
@@ -226,22 +227,30 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
       }
       if (!fresh && __any(up)) break;
       fresh = false;
-      bf16x8_t pf[RT];
+      bf16x8_t hi[RT], lo[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        u32x4_t p;
+        u32x4_t h, l;
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
-          p[w] = two_bf16(__builtin_amdgcn_exp2f(t[rt][2 * w]), __builtin_amdgcn_exp2f(t[rt][2 * w + 1]));
-        pf[rt] = __builtin_bit_cast(bf16x8_t, p);
-        sum[rt] = mfma16x16x32(ones, pf[rt], sum[rt]);
+        for (int w = 0; w < 4; ++w) {
+          const float p0 = __builtin_amdgcn_exp2f(t[rt][2 * w]), p1 = __builtin_amdgcn_exp2f(t[rt][2 * w + 1]);
+          sum[rt] += p0;
+          sum[rt] += p1;
+          h[w] = two_bf16(p0, p1);
+          l[w] = two_bf16(p0 - __uint_as_float(h[w] << 16), p1 - __uint_as_float(h[w] & 0xffff0000u));
+        }
+        hi[rt] = __builtin_bit_cast(bf16x8_t, h);
+        lo[rt] = __builtin_bit_cast(bf16x8_t, l);
       }
       const u32x4_t* vt = lds + ((size_t)(tile & 1) * 2 + 1) * NF * 64 + (at % SW * KW + kw) * (DT * 64) + get;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, vt[dt * 64]);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma16x16x32(vf, pf[rt], o[rt][dt]);
+        for (int rt = 0; rt < RT; ++rt) {
+          o[rt][dt] = mfma16x16x32(vf, hi[rt], o[rt][dt]);
+          o[rt][dt] = mfma16x16x32(vf, lo[rt], o[rt][dt]);
+        }
       }
       if (++at % SW == 0) {
         if (more) stage((tile + 1) & 1);
@@ -276,7 +285,7 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
   lds_barrier();
   float l[RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) l[rt] = none ? __builtin_nanf("") : sum[rt][0];
+  for (int rt = 0; rt < RT; ++rt) l[rt] = none ? __builtin_nanf("") : quads_sum(sum[rt]);
   const size_t part0 = ((size_t)slot * x.Hkv + h) * rows;  // parts: [run][kv head][row]
   if constexpr (KW == 1) {
 #pragma unroll
@@ -325,8 +334,7 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
 // A wave takes a run of a sequence's own keys for 16 of its query rows of a kv head, 32 keys a step. Four lanes in
 // a row load 64 bytes of a K (V) row at once, and the wave turns them into the matrix cores' operands through LDS of its own; as
 // soon as a step's K (V) is there, its registers take the next one's loads. Bound by memory: 64 sequences of 1000 tokens, 262 MB,
-// in 52 us. (Loaded as operands, a row a lane, 54; and 16 rows of 256 dims are left no registers.) P is the sum of two bf16 terms
-// here, as in paged.hip: products are not what it waits for.
+// in 52 us. (Loaded as operands, a row a lane, 54; and 16 rows of 256 dims are left no registers.)
 template <int D>
 __device__ __forceinline__ void own_run(const Pages& pg, const Rows& x, int b, int h, int tile, int run, int runs, int run_keys, int room) {
   constexpr int KS = Shape<D>::KS, DT = Shape<D>::DT, CH = DT < 8 ? DT : 8;  // (CH: operands staged at a time)
@@ -614,11 +622,17 @@ struct Cut {
 // The form of the prefix's kernel by the query rows of a kv head: few rows want the tile's keys dealt to many waves, many rows few
 // reads of a tile. Behind 20000 tokens, us a call, (waves, row tiles, waves that share the keys):
 //   8 heads of 128 dims:   (4, 1, 4) (8, 1, 4) (8, 2, 4) (8, 2, 2) (8, 2, 1)     4 heads of 256:  (4, 1, 2) (8, 1, 2) (8, 1, 1)
-//            16 rows          22.3      22.8      24.7      30.7      39.7                           26.4      29.0      32.0
-//            32               27.9      22.9      26.1      32.0      40.4                           27.3      30.1      34.8
-//            64               42.8      30.1      27.9      32.9      41.4                           37.3      32.5      37.1
-//           128               68.9      47.1      37.2      35.3      44.2                           52.9      44.5      43.2
-//           256              122.7      74.5      54.5      49.4      49.5                           89.3      65.1      60.5
+//            16 rows          23.2      23.4      27.1      34.8      47.0                           27.1      29.8      34.7
+//            32               28.7      23.8      27.9      35.7      47.0                           27.7      31.1      36.6
+//            64               44.5      31.3      29.1      36.7      47.9                           39.0      33.1      38.9
+//           128               72.8      49.1      40.2      41.4      51.6                           55.5      47.4      46.5
+//           256              146.0      87.8      67.0      65.2      63.0                          108.0      71.5      70.8
+//   8 heads of 64 dims:
+//            16 rows          17.8      17.5      18.4      23.1      32.0
+//            32               20.7      17.0      18.8      24.0      32.4
+//            64               29.8      21.1      20.3      24.8      33.1
+//           128               47.0      32.5      30.7      28.7      35.0
+//           256               81.4      48.9      46.2      42.5      42.0
 void set_form(Cut& c, int rows, int D) {
   if (D == 256) {
     c.waves = rows > 32 ? 8 : 4;
@@ -631,11 +645,13 @@ void set_form(Cut& c, int rows, int D) {
   }
 }
 
-// The runs. A CU holds one workgroup, so the card is shared out: so many workgroups to the prefix that those left over are done
-// with the own keys in the same time, by what a CU was measured to do. It reads 35 bytes a ns, and forms 256 x 128 scores and
-// outputs of 128 dims in 4 us; a workgroup of either kind begins and ends in 6 and 3 us. Own runs have 64 keys at least, and the
-// prefix half the card: `keys` may be a loose bound. (All of the card to the prefix first, and then to runs of 128 own keys: 32
-// sequences of 500 behind 4099 tokens 36 -> 28 us, 16 of 300 behind 16384 39 -> 28, 128 of 300 behind 16384 97 -> 83.)
+// The runs. A CU holds one workgroup (of those of 64 dims and 16-row waves two, on which the cut does not count), so the card is
+// shared out: so many workgroups to the prefix that those left over are done with the own keys in the same time. What a CU does, by
+// the figures that gave the best calls over 17 sizes: it reads 35 bytes a ns; it forms 256 x 128 scores and outputs of 128 dims in 7.5
+// us (alone 6.0, by which calls where the two kinds nearly balance were up to 15 % slower); a workgroup of either kind begins and ends
+// in 6 and 3 us. Own runs have 32 keys at least, and the prefix half the card: `keys` may be a loose bound. (All of the card to the
+// prefix first, and then to runs of 128 own keys: 32 sequences of 500 behind 4099 tokens 36 -> 28 us, 16 of 300 behind 16384 39 -> 28,
+// 128 of 300 behind 16384 97 -> 83.)
 Cut cut_of(int B, int T, int G, int Hkv, int D, int prefix_keys, int keys) {
   Cut c;
   const int rows = B * T * G, tile = tile_keys(D);
@@ -644,7 +660,7 @@ Cut cut_of(int B, int T, int G, int Hkv, int D, int prefix_keys, int keys) {
   c.row_blocks = times(rows, block);
   c.tiles = times(T * G, 16);
   const int tiles = times(prefix_keys, tile), front = Hkv * c.row_blocks, most = 256 / front > 1 ? 256 / front : 1;
-  const float read = 4.f * tile * D / 35, form = (float)block * tile * (D + 128) * 4.8e-4f, a_tile = read > form ? read : form;
+  const float read = 4.f * tile * D / 35, form = (float)block * tile * (2 * D + 128) * 6e-4f, a_tile = read > form ? read : form;
   const float a_step = c.waves * (4.f * 32 * D) / 35, a_part = 8.f * Hkv * rows * D / 4900;
   const float late = 35 / 19.f;  // what a step takes longer with all CUs at it
   const int64_t all = (int64_t)B * Hkv * c.tiles;
