@@ -258,6 +258,7 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
       }
     }
     if (at == steps) break;
+    // Only of the rows that pass theirs: when another row, maybe of another sequence, raises its own is nothing to a row's bits.
     f32x4_t acc[RT][2];
     scores(at, acc);
 #pragma unroll
@@ -265,7 +266,9 @@ __device__ __forceinline__ void prefix_run(const Pages& pg, const Prefix& px, co
       float top = acc[rt][0][0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) top = fmaxf(top, acc[rt][e >> 2][e & 3]);
-      const float nm = fmaxf(m[rt], quads_max(top) * sc), f = __builtin_amdgcn_exp2f(m[rt] - (nm == -INFINITY ? 0.f : nm));
+      top = quads_max(top);
+      const bool none = m[rt] == -INFINITY, up = fmaf(top, sc, none ? 0.f : -m[rt]) > (none ? -INFINITY : kLag);
+      const float nm = up ? top * sc : m[rt], f = up ? __builtin_amdgcn_exp2f(m[rt] - nm) : 1.f;
       m[rt] = nm;
       sum[rt] *= f;
 #pragma unroll

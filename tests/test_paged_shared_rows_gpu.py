@@ -1,9 +1,10 @@
-"""Attention behind a shared prefix (csrc/paged_shared.hip), in each form of the prefix's kernel: how exact a row is."""
+"""Attention behind a shared prefix (csrc/paged_shared.hip), in each form of the prefix's kernel: how exact a row is, and that its
+bits are its own."""
 
 import pytest
 import torch
 
-from test_paged_shared_gpu import HALF, U, Shared
+from test_paged_shared_gpu import BF16, HALF, NAN, U, Shared, _bits
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,20 @@ def test_weights_of_the_prefix_are_as_exact_as_the_own_keys(dev, d, batch):
         off = (got[i, :c].double().cpu() - out).abs()
         worst = (off / (HALF * (out.abs() + err) + err)).max().item()
         assert worst <= 1, f"sequence {i}: {worst:.3f} of the bound"
+
+
+@pytest.mark.parametrize("d,batch", FORMS)
+@pytest.mark.parametrize("padding", [NAN, 3e38, 0.0])
+def test_bits_do_not_depend_on_other_rows(dev, d, batch, padding):
+    """One sequence's queries made so long that its maximum is raised all along the prefix, and padding rows that hold anything:
+    the other sequences keep their bits."""
+    s = _batch(dev, d, batch)
+    clean = _bits(s.run()).view(batch, -1)
+    for i in (0, batch // 2, batch - 1):
+        q = s.q.view(batch, 2, 4, d).clone()
+        q[i] = (q[i].float() * 20).to(BF16)
+        for j, c in enumerate(s.counts):
+            q[j, c:] = padding
+        y = _bits(s.run(q=q.view(-1, 4, d).to(dev))).view(batch, -1)
+        others = [j for j in range(batch) if j != i]
+        assert torch.equal(y[others], clean[others]), f"sequence {i}"
