@@ -274,50 +274,47 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
 // last) and NP that prepare chunks. A preparing wave takes every NPth chunk, through NP periods between the workgroup's barriers:
 // its loads; the products of keys and queries, gates and L; T by substitution; everything into LDS in the matrix cores' operand
 // order, for the period after. So one chunk is ready each period, K and Q are read once a workgroup, and no wave waits on memory.
-// NP is 4, or 6 where a period's longest piece of preparing, 4000 cycles, would be longer than what a wave of 16 columns does in
-// it, 3300: then the last two are in halves (2039 tokens of 16 heads 103 -> 97 us).
+// NP is 4, or 6 where a period's longest piece of preparing would be longer than what one or two waves of 16 columns do in it: then
+// the last two are in halves (2039 tokens of 16 heads 131 -> 124 us, 1024 of 64 heads 78 -> 73; with four waves of columns 84 and 84,
+// and 8 % slower where workgroups wait for a CU).
 //
 // Rows of the products are dealt to tokens, and rows of the state to key dims, as 8 (r / 4) + 4 (tile) + r % 4: then what one
 // product leaves in a lane (eight consecutive tokens, or dims, of one value column) is the operand that the next one takes.
 //
-// All of it is held in 32 bits. What a product takes of it is the sum of two fp16 terms, 2^-22 of the value or, for the
-// small ones, 2^-25 of 1: S, R, d, T and the products of q and k by three products of terms (the fourth is 2^-22 of them).
-// For that every value column has a power of two of its own, which keeps the larger of its state and its values near 1; keys and
-// queries are one fp16 term, exact but for what is 2^-17 of their row's length: a row is taken times the power of two below its
-// length's inverse. (With two bf16 terms, 2^-16, the results were off by 5e-6.) Decays are products of the tokens' own,
-// not exponentials of differences, which lose after a strong decay what it has taken.
+// All of it is held in 32 bits, and so is what a product takes of it: S, R, d, T and the products of q and k are each the sum of
+// three bf16 terms, which is all 24 bits of a value of any size; keys and queries are bf16 as they came, times the power of two
+// below their length's inverse. A product of two sums is six products of terms (the others are 2^-22 of it at most). Decays are
+// products of the tokens' own, not exponentials of differences, which lose after a strong decay what it has taken.
+//
+// Fewer bits are faster and do not hold. Two fp16 terms (60 matrix products a chunk and column tile for 96: 97 us where this takes
+// 124, 225 for 295) end at 2^-25 of a power of two that a column's values share: where these or the state fall inside a chunk, after
+// an outlier or by strong decays, the rows after it lose as many digits (2^-12: 1e-3 off), and setting such powers anew took a state
+// that all but vanishes to infinity. Two bf16 terms are 5e-6 off everywhere.
 //
 // A correction that is not finite (a value, key or gate that is no number; a state that is none) would meet the rows before its
 // token as 0 * NaN: such a chunk's columns are taken token by token instead.
 //
-// Bound by the chain of a wave's products and conversions where heads are few (a prompt of 2039 tokens, 16 heads: 97 us), by the
-// issue of two waves a SIMD where they are many (16 prompts of up to 1501 tokens, 32 heads: 235 us, of which a copy's rate would take
-// 149).
+// Bound by the chains of single waves, of columns and preparing, where heads are few (a prompt of 2039 tokens, 16 heads: 124 us), by
+// the issue of two waves a SIMD where they are many (16 prompts of up to 1501 tokens, 32 heads: 295 us, of which a copy's rate would
+// take 149).
 constexpr int kChunk = 32;
 
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
-typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
-using ::mfma16x16x32;  // of bf16
-__device__ __forceinline__ f32x4_t mfma16x16x32(f16x8_t a, f16x8_t b, f32x4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f16x8_t f16x8(u32x4_t v) { return __builtin_bit_cast(f16x8_t, v); }
+__device__ __forceinline__ bf16x8_t bf16x8(u32x4_t v) { return __builtin_bit_cast(bf16x8_t, v); }
 
 constexpr int kPitch = 36;  // floats of a row of L and T
 struct ChunkScalars {
   float beta[kChunk], in[kChunk], out[kChunk], end[kChunk];  // beta; beta |k| e^G; |q| e^G; |k| e^(G_C - G)
-  float decay[kChunk], k[kChunk], q[kChunk];                 // token by token: the factors that make fp16 rows unit vectors
+  float decay[kChunk], k[kChunk], q[kChunk];                 // token by token: the factors that make the rows unit vectors
   float total;                                               // e^G_C
   float pad[3];
 };
 struct ChunkOps {        // 1 KB operands: a lane's 16 bytes after its neighbour's
   u32x4_t k[2][4][64];   // [token tile][dim step]
   u32x4_t q[2][4][64];
-  u32x4_t t[2][2][64];   // [term][token tile]
-  u32x4_t a[2][2][64];
+  u32x4_t t[3][2][64];   // [term][token tile]
+  u32x4_t a[3][2][64];
   ChunkScalars sc;
 };
 struct ChunkScratch {
@@ -337,13 +334,7 @@ struct ChunkLds {
 // What one wave's lanes exchange through LDS: written before, read after.
 __device__ __forceinline__ void lanes_meet() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// The larger of, and the sum over, the four quads' values, in every lane.
-__device__ __forceinline__ float quads_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
+// The sum over the four quads' values, in every lane.
 __device__ __forceinline__ float quads_sum(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -351,34 +342,51 @@ __device__ __forceinline__ float quads_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-__device__ __forceinline__ uint32_t two_f16(float a, float b) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+// The two bf16 halves of a word.
+__device__ __forceinline__ float low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// Eight values as the sum of three bf16 terms, largest first, exact: eight bits of 24 each. `cut`: a value's first, second and third
+// eight bits, by fewer instructions one after the other; else each the nearest. Where both factors of a product are split, one is cut
+// and one not, so that what mfma_split leaves out has either sign: 1.4e-7 of the results' norm off (both cut 1.7e-7, none 1.3e-7; 16
+// prompts of up to 1501 tokens 298, 296 and 312 us).
+struct Split {
+  bf16x8_t term[3];
+};
+template <bool cut>
+__device__ __forceinline__ Split split(const float (&v)[8]) {
+  u32x4_t w[3];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+      const uint32_t word = cut ? __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u) : two_bf16(a, b);
+      w[n][i] = word;
+      a -= cut ? high(__float_as_uint(a)) : low(word);
+      b -= cut ? high(__float_as_uint(b)) : high(word);
+    }
+  }
+  return {bf16x8(w[0]), bf16x8(w[1]), bf16x8(w[2])};
 }
 
-// Eight values as the sum of two fp16 terms. `one` is 1, unknown to the compiler: the rest is then one instruction a value.
-struct Split {
-  f16x8_t hi, lo;
-};
-__device__ __forceinline__ Split split(const float (&v)[8], float one) {
-  u32x4_t hi, lo;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    uint32_t word = two_f16(v[2 * w], v[2 * w + 1]);
-    asm("" : "+v"(word));  // seen as part of a vector, the compiler subtracts the first word's halves from every pair
-    hi[w] = word;
-    const f16x2_t h = __builtin_bit_cast(f16x2_t, word);
-    lo[w] = two_f16(fmaf(v[2 * w], one, -(float)h.x), fmaf(v[2 * w + 1], one, -(float)h.y));
-  }
-  return {f16x8(hi), f16x8(lo)};
+// c + a b, of the six products of terms that hold 24 bits, the smallest first.
+__device__ __forceinline__ f32x4_t mfma_split(const bf16x8_t (&a)[3], const bf16x8_t (&b)[3], f32x4_t c) {
+  c = mfma16x16x32(a[2], b[0], c);
+  c = mfma16x16x32(a[0], b[2], c);
+  c = mfma16x16x32(a[1], b[1], c);
+  c = mfma16x16x32(a[1], b[0], c);
+  c = mfma16x16x32(a[0], b[1], c);
+  return mfma16x16x32(a[0], b[0], c);
 }
 
 // Whether one of the eight is an infinity or NaN.
-__device__ __forceinline__ bool no_numbers(f16x8_t v) {
+__device__ __forceinline__ bool no_numbers(bf16x8_t v) {
   const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
   u16x2_t m = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu));
-  return m.x >= 0x7c00 || m.y >= 0x7c00;
+  return m.x >= 0x7f80 || m.y >= 0x7f80;
 }
 
 // Lane i - N of the same eight, or 1.
@@ -394,7 +402,7 @@ __device__ __forceinline__ float times_after(float v, int lane) {
 }
 
 // Waits for loads and stores (vmcnt(0)). At the end of a rare path: where it meets the usual one, the compiler would have that one
-// wait for all that either may have in flight (16 prompts of up to 1501 tokens 271 -> 253 us).
+// wait for all that either may have in flight (7 % of 16 prompts of up to 1501 tokens).
 __device__ __forceinline__ void nothing_in_flight() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // v, which the compiler then forms again in every turn of a loop: its sums with other offsets, formed before it, take two
@@ -426,8 +434,6 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   ChunkScratch& my = lds.scratch[p];
   const int tok[2] = {8 * (r >> 2) + (r & 3), 8 * (r >> 2) + 4 + (r & 3)};  // of this lane's row in each token tile
-  float one = 1.f;
-  asm volatile("" : "+v"(one));
   uint32_t off[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) off[t] = tok[t] * x.ldq + q * 8;
@@ -558,7 +564,7 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
             a[e] = qk[ti][e >> 2][e & 3] * (wk * qn);
             w *= dj[e];
           }
-          aq[ti] = split(a, one);
+          aq[ti] = split<true>(a);
           // (L's diagonal and what is above it are not read)
           *reinterpret_cast<f32x4_t*>(&my.l[i][8 * q]) = f32x4_t{l[0], l[1], l[2], l[3]};
           *reinterpret_cast<f32x4_t*>(&my.l[i][8 * q + 4]) = f32x4_t{l[4], l[5], l[6], l[7]};
@@ -603,29 +609,27 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
         load_gates(c + NP);
         ChunkOps& to = lds.ops[c & 1];
         u32x4_t kh[2][4], qh[2][4];
-        Split two[2];
+        Split tt[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const float k2 = my.two[0][tok[t]], q2 = my.two[1][tok[t]];
-          auto f16 = [&](bf16x8_t v, float two) {  // (a mixed fma to fp16 a value: fewer instructions, 4 % slower)
+          auto times = [&](bf16x8_t v, float two) {
             const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
             u32x4_t y;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              y[i] = two_f16(__uint_as_float(w[i] << 16) * two, __uint_as_float(w[i] & 0xffff0000u) * two);
-            }
+            for (int i = 0; i < 4; ++i) y[i] = two_bf16(low(w[i]) * two, high(w[i]) * two);
             return y;
           };
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            kh[t][s] = f16(kf[t][s], k2);
-            qh[t][s] = f16(qf[t][s], q2);
+            kh[t][s] = times(kf[t][s], k2);
+            qh[t][s] = times(qf[t][s], q2);
           }
           float row[8];
           eight_of(&my.t[tok[t]][8 * q], row);
 #pragma unroll
           for (int e = 0; e < 8; ++e) row[e] = tok[t] < 16 && q >= 2 ? 0.f : row[e];
-          two[t] = split(row, one);
+          tt[t] = split<true>(row);
         }
         half_period();
 #pragma unroll
@@ -635,10 +639,11 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
             to.k[t][s][lane] = kh[t][s];
             to.q[t][s][lane] = qh[t][s];
           }
-          to.t[0][t][lane] = __builtin_bit_cast(u32x4_t, two[t].hi);
-          to.t[1][t][lane] = __builtin_bit_cast(u32x4_t, two[t].lo);
-          to.a[0][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].hi);
-          to.a[1][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].lo);
+#pragma unroll
+          for (int n = 0; n < 3; ++n) {
+            to.t[n][t][lane] = __builtin_bit_cast(u32x4_t, tt[t].term[n]);
+            to.a[n][t][lane] = __builtin_bit_cast(u32x4_t, aq[t].term[n]);
+          }
         }
         if (lane < kChunk) {
           const float beta = my.beta[lane], kr = my.rest[0][lane], qr = my.rest[1][lane], since = my.since[lane];
@@ -658,15 +663,7 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
   while (left > 0) end_period();
 }
 
-// A column's power of two: its values stay within 2^5 of it, and the larger of values and state between 2^-2 and 2^5 wherever it
-// is looked at, or the power is set anew, so that it is 4 to 8; powers within 2^-100 .. 2^100. A column's length grows by at most
-// beta |v| a token: from one look to the next it stays below 2^5 (sqrt(128) + 128), far inside fp16.
-constexpr float kLow = 0.25f, kHigh = 32.f;
 constexpr int kBuffer = 0x00020000;  // a raw buffer's words
-constexpr int kLook = 4;  // chunks from one look at the state to the next; its values are looked at in each
-__device__ __forceinline__ float power_below(float v) {  // that leaves v at 4 to 8
-  return __uint_as_float((__float_as_uint(fminf(fmaxf(v * 0.25f, 0x1p-100f), 0x1p100f))) & 0x7f800000u);
-}
 
 template <int WC, int NT, int NP>
 __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
@@ -677,7 +674,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
   extern __shared__ u32x4_t chunk_lds[];
   ChunkLds<NP>& lds = *reinterpret_cast<ChunkLds<NP>*>(chunk_lds);
   // Heads that follow each other to one die (they take workgroups in turn): value heads of one key head find its rows in that
-  // die's cache (8 sequences of 1024 tokens, 32 heads of 16 key heads 109 -> 103 us; a third less read past it).
+  // die's cache (8 sequences of 1024 tokens, 32 heads of 16 key heads 5 % less time; a third less read past it).
   const int x = blockIdx.x, h = H % 8 ? x : x % 8 * (H / 8) + x / 8;
   const int b = blockIdx.z, tid = threadIdx.x, wave = wave_id(), lane = tid & 63;
   const int col0 = (int)blockIdx.y * COLS;
@@ -701,22 +698,16 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
   const int r = lane & 15, q = lane >> 4;
   // of the workgroup's; + nt: a lane's columns are neighbours, and their values (results) one load (store)
   const int col = wave * 16 * NT + NT * r;
-  float one = 1.f;
-  asm volatile("" : "+v"(one));
-  // dims 32 s + 8 q + 4 half + i of column col + nt, times `inv`
-  f32x4_t st[NT][4][2];
-  float inv[NT], scale[NT], top[NT];
+  f32x4_t st[NT][4][2];  // dims 32 s + 8 q + 4 half + i of column col + nt
   const size_t at = ((size_t)h * kDv + col0 + col) * kDk + q * 8;
   float* to = state + run.write * pool.stride + at;
   auto get_state = [&](const float* from) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      inv[nt] = scale[nt] = 1.f;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int half = 0; half < 2; ++half) st[nt][s][half] = *reinterpret_cast<const f32x4_t*>(from + nt * kDk + s * 32 + half * 4);
-    }
   };
   auto put_state = [&]() {
 #pragma unroll
@@ -725,19 +716,17 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-          *reinterpret_cast<f32x4_t*>(to + nt * kDk + s * 32 + half * 4) = st[nt][s][half] * scale[nt];
+          *reinterpret_cast<f32x4_t*>(to + nt * kDk + s * 32 + half * 4) = st[nt][s][half];
   };
   if (run.read >= 0) {
     get_state(state + run.read * pool.stride + at);
   } else {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      inv[nt] = scale[nt] = 1.f;
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int half = 0; half < 2; ++half) st[nt][s][half] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
   }
   const float qscale = rsqrtf((float)kDk);
   // A chunk's values and results as buffers from its first row to the sequence's end, at 32-bit offsets (bytes): loads past it are
@@ -763,38 +752,6 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
   for (int c = 0; c < chunks; ++c) {
     const ChunkOps& ops = lds.ops[c & 1];
     const int t0 = c * kChunk, live = min(kChunk, run.count - t0);
-    bool off = false;
-    u16x2_t most = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, nv[e] & 0x7fff7fffu));
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      top[nt] = bf16_bits_to_f32(most[nt]) * inv[nt];  // of this lane's values
-      off |= top[nt] > kHigh;
-    }
-    if (c % kLook == 0 || __any(off)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float sm = top[nt];
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sm = fmaxf(sm, fabsf(st[nt][s][half][i]));
-        sm = quads_max(sm);
-        if (!(sm > kHigh || sm < kLow) || !(sm > 0.f && sm < INFINITY)) continue;
-        const float to = power_below(sm * scale[nt]), f = scale[nt] / to;
-        scale[nt] = to;
-        inv[nt] = 1.f / to;
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st[nt][s][half][i] *= f;
-      }
-    }
     f32x4_t ks[NT][2], qs[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -802,23 +759,23 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
       for (int t = 0; t < 2; ++t) ks[nt][t] = qs[nt][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      Split two[NT];
+      Split sp[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const f32x4_t a = st[nt][s][0], d = st[nt][s][1];
         const float eight[8] = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
-        two[nt] = split(eight, one);
+        sp[nt] = split<true>(eight);
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const f16x8_t kf = f16x8(ops.k[t][s][lane]), qf = f16x8(ops.q[t][s][lane]);
+        const bf16x8_t kf = bf16x8(ops.k[t][s][lane]), qf = bf16x8(ops.q[t][s][lane]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          ks[nt][t] = mfma16x16x32(kf, two[nt].hi, ks[nt][t]);
-          qs[nt][t] = mfma16x16x32(qf, two[nt].hi, qs[nt][t]);
-          ks[nt][t] = mfma16x16x32(kf, two[nt].lo, ks[nt][t]);
-          qs[nt][t] = mfma16x16x32(qf, two[nt].lo, qs[nt][t]);
-        }
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int n = 0; n < 3; ++n) {
+            ks[nt][t] = mfma16x16x32(kf, sp[nt].term[n], ks[nt][t]);
+            qs[nt][t] = mfma16x16x32(qf, sp[nt].term[n], qs[nt][t]);
+          }
       }
     }
     f32x4_t d[NT][2];
@@ -828,23 +785,19 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
       float beta[8], in[8];
       eight_of(ops.sc.beta + 8 * q, beta);
       eight_of(ops.sc.in + 8 * q, in);
-      f16x8_t tf[2][2];
+      bf16x8_t tf[2][3];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) tf[i][t] = f16x8(ops.t[i][t][lane]);
+        for (int n = 0; n < 3; ++n) tf[t][n] = bf16x8(ops.t[n][t][lane]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float right[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], value(nt, e) * inv[nt], -in[e] * ks[nt][e >> 2][e & 3]);
-        const Split two = split(right, one);
+        for (int e = 0; e < 8; ++e) right[e] = fmaf(beta[e], value(nt, e), -in[e] * ks[nt][e >> 2][e & 3]);
+        const Split sp = split<false>(right);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          d[nt][t] = mfma16x16x32(tf[0][t], two.lo, f32x4_t{0.f, 0.f, 0.f, 0.f});
-          d[nt][t] = mfma16x16x32(tf[1][t], two.hi, d[nt][t]);
-          d[nt][t] = mfma16x16x32(tf[0][t], two.hi, d[nt][t]);
-        }
+        for (int t = 0; t < 2; ++t) d[nt][t] = mfma_split(tf[t], sp.term, f32x4_t{0.f, 0.f, 0.f, 0.f});
       }
       if (c + 1 < chunks) load_v(c + 1);
 #pragma unroll
@@ -852,19 +805,19 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
         float eight[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) eight[e] = d[nt][e >> 2][e & 3];
-        dd[nt] = split(eight, one);
-        odd |= no_numbers(dd[nt].hi);
+        dd[nt] = split<false>(eight);
+        odd |= no_numbers(dd[nt].term[0]);
       }
     }
     if (!__any(odd)) {
       float out[8], end[8];
       eight_of(ops.sc.out + 8 * q, out);
       eight_of(ops.sc.end + 8 * q, end);
-      f16x8_t af[2][2];
+      bf16x8_t af[2][3];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) af[i][t] = f16x8(ops.a[i][t][lane]);
+        for (int n = 0; n < 3; ++n) af[t][n] = bf16x8(ops.a[n][t][lane]);
       const auto yr = __builtin_amdgcn_make_buffer_rsrc(yb + (size_t)t0 * ystep, 0, live * yld, kBuffer);
       Split ends[NT];
 #pragma unroll
@@ -872,15 +825,13 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
         float decayed[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) decayed[e] = d[nt][e >> 2][e & 3] * end[e];
-        ends[nt] = split(decayed, one);
+        ends[nt] = split<true>(decayed);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           f32x4_t& acc = qs[nt][t];
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[i] *= out[4 * t + i];
-          acc = mfma16x16x32(af[0][t], dd[nt].lo, acc);
-          acc = mfma16x16x32(af[1][t], dd[nt].hi, acc);
-          acc = mfma16x16x32(af[0][t], dd[nt].hi, acc);
+          acc = mfma_split(af[t], dd[nt].term, acc);
         }
       }
       uint32_t at = here(8 * q * yld + col * 4);
@@ -888,7 +839,7 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
       for (int e = 0; e < 8; ++e, at += yld) {
         uint32_t y[NT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) y[nt] = __float_as_uint(qs[nt][e >> 2][e & 3] * (qscale * scale[nt]));
+        for (int nt = 0; nt < NT; ++nt) y[nt] = __float_as_uint(qs[nt][e >> 2][e & 3] * qscale);
         if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b32(y[0], yr, at, 0, 0);
         else __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{y[0], y[1]}, yr, at, 0, 0);
       }
@@ -909,13 +860,13 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
             const char* from = reinterpret_cast<const char*>(&ops.k[t][s][0]) + turn + 8 * half;
             part[t] = __builtin_bit_cast(two_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)from));
           }
-          const f16x8_t kt = f16x8(u32x4_t{part[0].x, part[0].y, part[1].x, part[1].y});
+          const bf16x8_t kt = bf16x8(u32x4_t{part[0].x, part[0].y, part[1].x, part[1].y});
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) st[nt][s][half][i] *= total;
-            st[nt][s][half] = mfma16x16x32(kt, ends[nt].lo, st[nt][s][half]);
-            st[nt][s][half] = mfma16x16x32(kt, ends[nt].hi, st[nt][s][half]);
+#pragma unroll
+            for (int n = 2; n >= 0; --n) st[nt][s][half] = mfma16x16x32(kt, ends[nt].term[n], st[nt][s][half]);
           }
         }
     } else {
@@ -931,19 +882,19 @@ __global__ __launch_bounds__(64 * (WC + NP)) void gdn_batch_chunks_kernel(
           float sum = 0.f, yv = 0.f;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const f16x8_t w = f16x8(ops.k[tile][s][row]);
+            const u32x4_t w = ops.k[tile][s][row];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf((float)w[e] * kn, mine[s * 32 + e], sum);
+            for (int e = 0; e < 8; ++e) sum = fmaf((e & 1 ? high(w[e >> 1]) : low(w[e >> 1])) * kn, mine[s * 32 + e], sum);
           }
           const float delta = bt * (bf16_bits_to_f32(vrow[(int64_t)(t0 + i) * ldq + col + nt]) - decay * quads_sum(sum));
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            const f16x8_t w = f16x8(ops.k[tile][s][row]), z = f16x8(ops.q[tile][s][row]);
+            const u32x4_t w = ops.k[tile][s][row], z = ops.q[tile][s][row];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float x = fmaf((float)w[e] * kn, delta, mine[s * 32 + e] * decay);
+              const float x = fmaf((e & 1 ? high(w[e >> 1]) : low(w[e >> 1])) * kn, delta, mine[s * 32 + e] * decay);
               mine[s * 32 + e] = x;
-              yv = fmaf((float)z[e] * qn, x, yv);
+              yv = fmaf((e & 1 ? high(z[e >> 1]) : low(z[e >> 1])) * qn, x, yv);
             }
           }
           yv = quads_sum(yv);
@@ -1028,8 +979,8 @@ extern "C" int skinny_gdn_recurrence_batch(const uint16_t* qkv, int64_t ldq, con
       return launch(p, qkv, ldq, b, a, ldab, A_log, dt_bias, state, y, B, T, H, Hk, (hipStream_t)stream);
     };
     // As many workgroups to a head as still find a CU each (their registers leave no room for two): us a call for 16, 32, 64 and
-    // 128 columns a workgroup, 1024 tokens of 32 heads: 1 sequence 55.2 / 57.0 / 67.8 / 87.8, 4 sequences 211 / 111 / 69.8 / 88.2, 8:
-    // 421 / 222 / 140 / 100.
+    // 128 columns a workgroup, 1024 tokens of 32 heads: 1 sequence 68 / 71 / 84 / 114, 2 134 / 73 / 84 / 113, 4 265 / 140 / 88 / 113, 8
+    // 529 / 279 / 170 / 123.
     const int64_t heads = (int64_t)B * H;
     return heads > 128 ? chunks(launch_chunks<4, 2, 4>) : heads > 64 ? chunks(launch_chunks<4, 1, 4>) : heads > 32 ? chunks(launch_chunks<2, 1, 6>)
                                                                                                              : chunks(launch_chunks<1, 1, 6>);
