@@ -629,7 +629,8 @@ int skinny_gdn_conv_silu_batch(const uint16_t* x, int64_t ldx, int B, int T, int
  * states have skinny_gdn_recurrence's bits; with more, tokens go in chunks of 32 through the matrix cores, from
  * terms that together hold 24 bits, and sums in fp32 (1.4e-7 of the results' norm from exact ones, against
  * 1e-7 token by token, and like them in a row whose values are small against the ones before it). A
- * sequence's bits do not depend on what the others hold, in chunks at most on B. */
+ * sequence's bits do not depend on what the others hold, in chunks at most on B. A query or key whose
+ * squares pass 32 bits' range (finite values, a length of 2^64) counts as zeros, here and token by token. */
 int skinny_gdn_recurrence_batch(const uint16_t* qkv, int64_t ldq, const uint16_t* b, const uint16_t* a, int64_t ldab,
                                 const float* A_log, const float* dt_bias, int B, int T, const skinny_state_pool* pool,
                                 float* state, float* y, int H, int Hk, int Dk, int Dv, void* stream);

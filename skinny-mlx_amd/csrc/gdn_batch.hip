@@ -537,14 +537,26 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
           }
         }
         lanes_meet();
-        {  // a lane per row, keys and queries
+        bool none;  // a row whose squares are past 32 bits' range, which then is one of zeros, as token by token
+        {           // a lane per row, keys and queries
           const float ss = my.sq[0][lane], inv = rsqrtf(ss + 1e-6f);
+          none = inv == 0.f;
           const uint32_t bits = __float_as_uint(rsqrtf(fmaxf(ss, 0x1p-126f))) & 0x7f800000u;
           my.two[0][lane] = __uint_as_float(bits);
           my.rest[0][lane] = inv * __uint_as_float(0x7f000000u - bits);
           my.inv[0][lane] = inv;
         }
         lanes_meet();
+        if (__any(none)) {  // its products may be infinite
+#pragma unroll
+          for (int ti = 0; ti < 2; ++ti)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const bool key = my.inv[0][8 * q + e] == 0.f;
+              kk[ti][e >> 2][e & 3] = key || my.inv[0][tok[ti]] == 0.f ? 0.f : kk[ti][e >> 2][e & 3];
+              qk[ti][e >> 2][e & 3] = key || my.inv[1][tok[ti]] == 0.f ? 0.f : qk[ti][e >> 2][e & 3];
+            }
+        }
         const int mine = r >> 2;  // the eight that holds both rows
         const float between = (q < 1 && mine > 1 ? my.inner[15] : 1.f) * (q < 2 && mine > 2 ? my.inner[23] : 1.f);
         float dj[8], kj[8];
@@ -559,9 +571,9 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
 #pragma unroll
           for (int e = 7; e >= 0; --e) {
             w = e == at ? 1.f : w;
-            const float wk = w * kj[e];
-            l[e] = kk[ti][e >> 2][e & 3] * (wk * bk);
-            a[e] = qk[ti][e >> 2][e & 3] * (wk * qn);
+            const float wk = w * kj[e];  // (times the product first: two long rows' inverses may leave nothing of each other)
+            l[e] = kk[ti][e >> 2][e & 3] * wk * bk;
+            a[e] = qk[ti][e >> 2][e & 3] * wk * qn;
             w *= dj[e];
           }
           aq[ti] = split<true>(a);

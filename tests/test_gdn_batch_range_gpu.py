@@ -175,3 +175,27 @@ def test_values_that_are_no_numbers_in_every_form(dev, heads, key_heads, batch, 
     elif where in "ka":
         if not (where == "a" and bad > 0):  # (a decay of 0 is a number)
             assert not torch.isfinite(y[1, at:, last]).any()
+
+
+@pytest.mark.parametrize("heads,key_heads,batch", FORMS)
+@pytest.mark.parametrize("T", [9, 130])
+def test_rows_past_the_range_of_their_squares_are_zero(dev, heads, key_heads, batch, T):
+    """Queries and keys of finite values whose squares pass 32 bits count as zeros, in chunks as token by token; rows just inside
+    that range are right."""
+    m = Mixer(dev, 110 + heads, heads, key_heads, T, [T] * batch)
+    rows = m.qkv.view(batch, T, 2 * key_heads + heads, D)
+    inside = m.qkv.clone().view(rows.shape)
+    rows[:, 1::2, :2 * key_heads] *= 2.0 ** 59  # lengths of 11 * 2^59: squares of 2^125
+    pool = m.pool.clone()
+    y = m.run(pool)
+    _check(m, 1, y, pool[m.slots[1]], m.pool[m.slots[1]], heads=[0, heads - 1], what="inside")
+    rows.copy_(inside)
+    rows[:, 4::7, :key_heads] *= 2.0 ** 66
+    rows[:, 5::9, key_heads:2 * key_heads] *= 2.0 ** 100
+    long_pool = m.pool.clone()
+    long = m.run(long_pool)
+    rows[:, 4::7, :key_heads] = 0
+    rows[:, 5::9, key_heads:2 * key_heads] = 0
+    pool = m.pool.clone()
+    y = m.run(pool)
+    assert torch.isfinite(long).all() and torch.equal(long, y) and torch.equal(long_pool[m.slots], pool[m.slots])
