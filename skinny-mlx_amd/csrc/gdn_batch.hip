@@ -322,8 +322,9 @@ struct ChunkScratch {
   float beta[kChunk], decay[kChunk];
   float inner[kChunk];         // the product of the decays of a token's eight up to it
   float since[kChunk], until[kChunk];  // e^G, e^(G_C - G)
-  // of k and of q: the squares; a power of two near the length's inverse; what that leaves of 1 / sqrt(squares + 1e-6); that
-  float sq[2][kChunk], two[2][kChunk], rest[2][kChunk], inv[2][kChunk];
+  // of the keys, then the queries: the squares; a power of two near the length's inverse; what that leaves of 1 / sqrt(squares +
+  // 1e-6); that
+  float sq[2 * kChunk], two[2 * kChunk], rest[2 * kChunk], inv[2 * kChunk];
 };
 template <int NP>
 struct ChunkLds {
@@ -532,19 +533,19 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
 #pragma unroll
           for (int ti = 0; ti < 2; ++ti) {
             const int i = r & 3;
-            my.sq[0][tok[ti]] = i == 0 ? kk[ti][ti][0] : i == 1 ? kk[ti][ti][1] : i == 2 ? kk[ti][ti][2] : kk[ti][ti][3];
-            my.sq[1][tok[ti]] = i == 0 ? qq[ti][0] : i == 1 ? qq[ti][1] : i == 2 ? qq[ti][2] : qq[ti][3];
+            my.sq[tok[ti]] = i == 0 ? kk[ti][ti][0] : i == 1 ? kk[ti][ti][1] : i == 2 ? kk[ti][ti][2] : kk[ti][ti][3];
+            my.sq[kChunk + tok[ti]] = i == 0 ? qq[ti][0] : i == 1 ? qq[ti][1] : i == 2 ? qq[ti][2] : qq[ti][3];
           }
         }
         lanes_meet();
         bool none;  // a row whose squares are past 32 bits' range, which then is one of zeros, as token by token
         {           // a lane per row, keys and queries
-          const float ss = my.sq[0][lane], inv = rsqrtf(ss + 1e-6f);
+          const float ss = my.sq[lane], inv = rsqrtf(ss + 1e-6f);
           none = inv == 0.f;
           const uint32_t bits = __float_as_uint(rsqrtf(fmaxf(ss, 0x1p-126f))) & 0x7f800000u;
-          my.two[0][lane] = __uint_as_float(bits);
-          my.rest[0][lane] = inv * __uint_as_float(0x7f000000u - bits);
-          my.inv[0][lane] = inv;
+          my.two[lane] = __uint_as_float(bits);
+          my.rest[lane] = inv * __uint_as_float(0x7f000000u - bits);
+          my.inv[lane] = inv;
         }
         lanes_meet();
         if (__any(none)) {  // its products may be infinite
@@ -552,20 +553,20 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
           for (int ti = 0; ti < 2; ++ti)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const bool key = my.inv[0][8 * q + e] == 0.f;
-              kk[ti][e >> 2][e & 3] = key || my.inv[0][tok[ti]] == 0.f ? 0.f : kk[ti][e >> 2][e & 3];
-              qk[ti][e >> 2][e & 3] = key || my.inv[1][tok[ti]] == 0.f ? 0.f : qk[ti][e >> 2][e & 3];
+              const bool key = my.inv[8 * q + e] == 0.f;
+              kk[ti][e >> 2][e & 3] = key || my.inv[tok[ti]] == 0.f ? 0.f : kk[ti][e >> 2][e & 3];
+              qk[ti][e >> 2][e & 3] = key || my.inv[kChunk + tok[ti]] == 0.f ? 0.f : qk[ti][e >> 2][e & 3];
             }
         }
         const int mine = r >> 2;  // the eight that holds both rows
         const float between = (q < 1 && mine > 1 ? my.inner[15] : 1.f) * (q < 2 && mine > 2 ? my.inner[23] : 1.f);
         float dj[8], kj[8];
         eight_of(&my.decay[8 * q], dj);
-        eight_of(&my.inv[0][8 * q], kj);
+        eight_of(&my.inv[8 * q], kj);
 #pragma unroll
         for (int ti = 0; ti < 2; ++ti) {
           const int i = tok[ti], at = mine == q ? i & 7 : -1;
-          const float qn = my.inv[1][i], bk = my.beta[i] * my.inv[0][i];
+          const float qn = my.inv[kChunk + i], bk = my.beta[i] * my.inv[i];
           float l[8], a[8];
           float w = mine > q ? my.inner[i] * between : 0.f;  // e^(G_i - G_j), from j = 8q + 7 down
 #pragma unroll
@@ -624,7 +625,7 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
         Split tt[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const float k2 = my.two[0][tok[t]], q2 = my.two[1][tok[t]];
+          const float k2 = my.two[tok[t]], q2 = my.two[kChunk + tok[t]];
           auto times = [&](bf16x8_t v, float two) {
             const u32x4_t w = __builtin_bit_cast(u32x4_t, v);
             u32x4_t y;
@@ -658,7 +659,7 @@ __device__ __forceinline__ void prepare_chunks(const Rows& x, ChunkLds<NP>& lds,
           }
         }
         if (lane < kChunk) {
-          const float beta = my.beta[lane], kr = my.rest[0][lane], qr = my.rest[1][lane], since = my.since[lane];
+          const float beta = my.beta[lane], kr = my.rest[lane], qr = my.rest[kChunk + lane], since = my.since[lane];
           to.sc.beta[lane] = beta;
           to.sc.in[lane] = beta * kr * since;
           to.sc.out[lane] = qr * since;
