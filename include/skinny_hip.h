@@ -595,7 +595,8 @@ int skinny_paged_attention_bf16(const uint16_t* q, int B, int T, int Hq, const s
  * *prefix tokens in the pages prefix_pages[0 .. max_prefix_pages - 1] of the same cache; kv's lengths,
  * counts and pages are of each sequence's own tokens after it. Row b*T + t sees the prefix and its own
  * positions <= lengths[b] + t. prefix_keys is the host's bound on *prefix (at most max_prefix_pages *
- * page); a prefix outside [0, prefix_keys] or with a page that is none makes the rows NaN. Values and
+ * page); a prefix outside [0, prefix_keys] or with a page that is none makes the rows NaN. As exact as
+ * skinny_paged_attention_bf16 (weights are two bf16 terms). Values and
  * scores that are not finite as above, and the same limits. A row's bits do not depend on the other sequences, but on B, T
  * and the bounds, which cut the prefix. The workspace is always needed. */
 size_t skinny_paged_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int prefix_keys, int keys);
@@ -611,7 +612,9 @@ int skinny_paged_attention_shared_bf16(const uint16_t* q, int B, int T, int Hq, 
  * only read may be shared, such as the one after a prefix that the sequences have in common; one
  * that the call writes stands once in slots_out and no other sequence reads it. (A sequence without
  * tokens whose state stays in its slot touches none: a batch may be padded with any.) A sequence with a
- * state outside the pool or a count outside [0, T] has NaN rows and writes none. Padding rows are zero. */
+ * state outside the pool or a count outside [0, T] has NaN rows and writes none. Padding rows are zero.
+ * Only the state after all counts[b] tokens is left: to take some of them back, write to other slots and make
+ * the call again from the old ones with the smaller counts. */
 typedef struct {
   const int32_t* slots;      /* [B] */
   const int32_t* slots_out;  /* [B] or NULL */

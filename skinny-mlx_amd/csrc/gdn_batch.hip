@@ -282,7 +282,7 @@ __global__ __launch_bounds__(kStepThreads) void gdn_batch_steps_kernel(Pool pool
 // product leaves in a lane (eight consecutive tokens, or dims, of one value column) is the operand that the next one takes.
 //
 // All of it is held in 32 bits, and so is what a product takes of it: S, R, d, T and the products of q and k are each the sum of
-// three bf16 terms, which is all 24 bits of a value of any size; keys and queries are bf16 as they came, times the power of two
+// three bf16 terms, which is all 24 bits of a value down to 2^-110; keys and queries are bf16 as they came, times the power of two
 // below their length's inverse. A product of two sums is six products of terms (the others are 2^-22 of it at most). Decays are
 // products of the tokens' own, not exponentials of differences, which lose after a strong decay what it has taken.
 //

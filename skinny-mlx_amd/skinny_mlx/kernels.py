@@ -699,7 +699,8 @@ def gdn_conv_silu_batch(x: torch.Tensor, conv_state: torch.Tensor, weight: torch
 
     counts (int32 [B], None: T each) says how many of a sequence's T rows are tokens; the others are zero. A state that is
     only read may be shared; one that is written stands once in slots_out and no other sequence reads it. A sequence with a
-    slot outside the pool or a count outside [0, T] comes out NaN and writes no state."""
+    slot outside the pool or a count outside [0, T] comes out NaN and writes no state. Only the state after all tokens is left:
+    a step whose tokens may be rejected writes to other slots and is made again with the accepted counts."""
     if not (x.is_cuda and x.dtype == BF16 and x.dim() == 2 and x.stride(1) == 1):
         raise ValueError("x must be a bf16 2-D GPU tensor")
     dev = x.get_device()
