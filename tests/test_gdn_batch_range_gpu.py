@@ -4,7 +4,7 @@ and states whose size changes from token to token, and values that are no number
 import pytest
 import torch
 
-from test_gdn_batch_gpu import D, NAN, Mixer, _same
+from test_gdn_batch_gpu import D, NAN, Mixer, _ints, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -31,7 +31,7 @@ def _rule(m, i, state, heads=None):
     q, k = unit(x[:, hs // rep]) * D ** -0.5, unit(x[:, m.key_heads + hs // rep])
     v = x[:, 2 * m.key_heads + hs]
     a = (m.a.view(-1, T, m.heads)[i, :n].double().cpu() + m.dt.double().cpu())[:, hs]
-    log_decay = -m.a_log.double().cpu().exp()[hs] * torch.nn.functional.softplus(a, threshold=1e9)
+    log_decay = -m.a_log.double().cpu().exp()[hs] * torch.nn.functional.softplus(a, threshold=40)
     decay, beta = torch.exp(log_decay), torch.sigmoid(m.b.reshape(-1, T, m.heads)[i, :n].double().cpu()[:, hs])
     s = state.double().cpu()[hs].clone()
     y = torch.zeros((n, len(hs), D), dtype=torch.float64)
@@ -199,3 +199,58 @@ def test_rows_past_the_range_of_their_squares_are_zero(dev, heads, key_heads, ba
     pool = m.pool.clone()
     y = m.run(pool)
     assert torch.isfinite(long).all() and torch.equal(long, y) and torch.equal(long_pool[m.slots], pool[m.slots])
+
+
+@pytest.mark.parametrize("heads,key_heads,batch", FORMS)
+@pytest.mark.parametrize("kind", ["reset", "kept", "same", "zero"])
+def test_hard_gates_and_keys_in_every_form(dev, heads, key_heads, batch, kind):
+    """Decays of zero inside chunks, decays of one, one key for all tokens with betas of one, keys of zero."""
+    T = 170
+    m = Mixer(dev, 130 + heads, heads, key_heads, T, [T - 13 * (i % 2) for i in range(batch)])
+    keys = m.qkv.view(batch, T, 2 * key_heads + heads, D)[:, :, key_heads:2 * key_heads]
+    if kind == "reset":
+        m.a[5::7] = 3000.0
+        m.a[6::11] = 40.0
+    elif kind == "kept":
+        m.a[:] = -100.0
+    elif kind == "same":
+        keys[:] = keys[:, :1].clone()
+        m.b[:], m.a[:] = 20.0, -100.0
+    else:
+        keys[:, 3::5] = 0
+    pool = m.pool.clone()
+    y = m.run(pool)
+    assert torch.isfinite(y).all()
+    for i in (0, 1):
+        _check(m, i, y, pool[m.slots[i]], m.pool[m.slots[i]], heads=[0, heads - 1], what=kind)
+
+
+@pytest.mark.parametrize("heads,key_heads,batch", FORMS)
+def test_states_apart_in_every_form(dev, heads, key_heads, batch):
+    """Read from one shared state or from none and written elsewhere, in a pool between other layers' states; a sequence without tokens
+    passes its state on. What is only read, and what is free, stays as it was; in place and in a dense pool, the same bits."""
+    T = 70
+    counts = [T, 0, 33, T, 64, 1][:batch]
+    m = Mixer(dev, 150 + heads, heads, key_heads, T, counts, extra=batch)
+    n = m.pool.shape[0]
+    free = [s for s in range(n) if s not in m.slots]
+    read = [m.slots[0] if i % 3 < 2 else -1 for i in range(batch)]
+    pool = m.pool.clone()
+    y = m.run(pool, read, slots_out=_ints(free, dev))
+    for i, c in enumerate(counts):
+        begin = m.pool[read[i]] if read[i] >= 0 else torch.zeros_like(m.pool[0])
+        if c:
+            _check(m, i, y, pool[free[i]], begin, heads=[0, heads - 1])
+        else:
+            assert _same(pool[free[i]], begin)
+    assert _same(pool[m.slots], m.pool[m.slots])
+    wide = torch.full((n, 3, heads, D, D), 7.0, device=dev)
+    wide[:, 1] = m.pool
+    assert _same(m.run(wide[:, 1], read, slots_out=_ints(free, dev)), y) and _same(wide[:, 1], pool)
+    assert (wide[:, 0] == 7).all() and (wide[:, 2] == 7).all()
+    own = m.pool.clone()
+    for i, s in enumerate(m.slots):
+        own[s] = m.pool[read[i]] if read[i] >= 0 else 0
+    assert _same(m.run(own), y)
+    for i, s in enumerate(m.slots):
+        assert _same(own[s], pool[free[i]])
